@@ -467,6 +467,76 @@ SDPA_API int  sdpa_dev_shard_partial_bf16(const void *Qb, int ldq, const void *K
                                           int dv, void *workspace, size_t workspace_bytes,
                                           void *stream);
 
+/* ---- device level: batched attention over a cache ------------------------------------------- */
+/* Attention of GROUPED heads for hosts that serve or train language models: batches of sequences, Hq query heads of which every
+ * G = Hq / Hkv share a key/value head, causal, over a cache.  Tensors are [batch, tokens, heads, dim] with any element strides
+ * (a head-major tensor is the same with other strides); the dim elements of a row are contiguous.  Rows whose bases and strides are
+ * multiples of 16 bytes take 16-byte accesses; all others are right as well, and slower.  fp32 tensors are multiplied on the f32
+ * matrix instructions; bf16 tensors on the bf16 ones, accumulated in fp32, softmax weights rounded to bf16 as operands.
+ *
+ * Query i of sequence b (i < q_lens[b]) is at position p = kv_lens[b] - q_lens[b] + i of its sequence: the queries are the
+ * LAST tokens of the cache.  Lengths are int32 on the device, clamped there to [0, q_tokens] / [0, kv_tokens]; null = all of them.
+ * A row that sees no key: out 0, lse -inf.  Rows i >= q_lens[b] likewise, and their gradients are 0; gradients of keys
+ * j >= kv_lens[b] are 0.  A key that a row does not see has no influence on it, whatever its cache row holds (NaN included).
+ * Everything is deterministic: no result depends on the order of atomics.                                                        */
+#define SDPA_F32  0
+#define SDPA_BF16 1
+
+struct sdpa_tensor {
+    void *data;                   /* device pointer                                                  */
+    long batch, token, head;      /* strides in elements                                             */
+};
+
+struct sdpa_heads {
+    size_t size;                  /* sizeof(struct sdpa_heads) of the caller                         */
+    struct sdpa_tensor q;         /* [B, q_tokens, q_heads, dk]                                      */
+    struct sdpa_tensor k, v;      /* [B, kv_tokens, kv_heads, dk / dv]                               */
+    struct sdpa_tensor out;       /* [B, q_tokens, q_heads, dv]                                      */
+    struct sdpa_tensor k_prefix, v_prefix;   /* [prefix_tokens, kv_heads, dk / dv] (batch stride unused)        */
+    struct sdpa_tensor dout, dq, dk_out, dv_out;   /* gradients: of out (in), q, k, v (out)           */
+    float *lse;                   /* [B, q_heads, q_tokens] contiguous: log of the row's softmax sum (written forward, read backward) */
+    const int *q_lens, *kv_lens;  /* [B] device int32, or null                                       */
+    const float *weights;         /* [B, kv_heads, kv_tokens], tokens contiguous                     */
+    float *weights_out;           /* the same shape; may be `weights` itself                         */
+    long weights_batch, weights_head, weights_out_batch, weights_out_head;   /* element strides      */
+    struct sdpa_tensor k_out, v_out;         /* eviction: [B, >= budget tokens, kv_heads, dk / dv]    */
+    int *lens_out, *kept;         /* eviction: [B] and [B, kv_heads, budget] contiguous              */
+    int dtype;                    /* SDPA_F32 or SDPA_BF16                                           */
+    int batch, q_tokens, kv_tokens, q_heads, kv_heads, dk, dv;    /* dk, dv in 1..256                */
+    int window, sinks;            /* key j is seen iff j <= p and (p - j < window or j < sinks)       */
+    int prefix_tokens;
+    int budget, recent;
+    float scale;                  /* scores are scale * q.k                                          */
+};
+
+/* Scratch a call needs (0 = none; negative: the SDPA_E* code the call would return).  The scratch belongs to one call at a time:
+ * calls on different streams, and captured graphs that may replay side by side, take one each.  `op` names the call.              */
+#define SDPA_OP_WINDOW          0
+#define SDPA_OP_WINDOW_BACKWARD 1
+#define SDPA_OP_PREFIX          2
+#define SDPA_OP_SCORED          3
+#define SDPA_OP_EVICT           4
+SDPA_API long sdpa_dev_heads_workspace(int op, const struct sdpa_heads *a);
+
+/* Causal attention over a sliding window of the last `window` tokens (the query's own included) plus the first `sinks` tokens of the
+ * cache, which stay visible: out, lse.  window >= kv_tokens: plain causal attention; q_tokens = 1: one new token.                    */
+SDPA_API int sdpa_dev_attention_window(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream);
+/* Its gradients dq, dk_out, dv_out from dout, q, k, v, out and lse (those of the forward call).  Where a value that a pair reads
+ * is not finite the gradients it reaches are NaN.                                                                                 */
+SDPA_API int sdpa_dev_attention_window_backward(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream);
+/* A batch whose sequences all begin with the same `prefix_tokens` cache rows: every query sees the whole prefix, then its own
+ * sequence's k / v causally (lengths and positions count the own part only).  The prefix is read once for the batch.              */
+SDPA_API int sdpa_dev_attention_prefix(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream);
+/* Causal attention over the whole cache that also adds what every key was given:
+ * weights_out[b,h,j] = weights[b,h,j] + sum over the group's heads and the queries of the softmax weight of key j.                  */
+SDPA_API int sdpa_dev_attention_scored(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream);
+/* Cuts every (sequence, key head) of a cache to `budget` keys.  n = kv_lens[b] <= budget: all stay.  Else the first `sinks`, the
+ * last `recent` and the budget - sinks - recent of greatest weight between them stay (ties: the lower index; NaN counts below
+ * everything), in their order.  They move to the front of k_out / v_out / weights_out; kept[b,h,:] are their old indices, lens_out[b] =
+ * min(n, budget); [lens_out, budget) is filled with zeros (kept: -1), what lies behind `budget` is left as it was.  The outputs
+ * must not overlap the inputs.                                                                                                  */
+SDPA_API int sdpa_dev_evict_cache(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -111,6 +111,13 @@ _PROTOS = {
                                              _c_void_p, _c_int, _c_void_p, _c_void_p,
                                              _c_int, _c_int, _c_int, _c_int,
                                              _c_void_p, _c_size_t, _c_void_p]),
+    # batched attention over a cache: the struct travels as the bytes heads.py packs
+    "sdpa_dev_heads_workspace": (_c_long, [_c_int, ctypes.c_char_p]),
+    "sdpa_dev_attention_window": (_c_int, [ctypes.c_char_p, _c_void_p, _c_size_t, _c_void_p]),
+    "sdpa_dev_attention_window_backward": (_c_int, [ctypes.c_char_p, _c_void_p, _c_size_t, _c_void_p]),
+    "sdpa_dev_attention_prefix": (_c_int, [ctypes.c_char_p, _c_void_p, _c_size_t, _c_void_p]),
+    "sdpa_dev_attention_scored": (_c_int, [ctypes.c_char_p, _c_void_p, _c_size_t, _c_void_p]),
+    "sdpa_dev_evict_cache": (_c_int, [ctypes.c_char_p, _c_void_p, _c_size_t, _c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,90 @@
+// sdpa_heads.h -- the batched attention operators: what the C ABI hands to the launchers, and the rules both share.
+// Internal; the public interface is include/sdpa_hip.h (struct sdpa_heads).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+
+#include "../../include/sdpa_hip.h"
+
+namespace sdpa {
+
+constexpr int kHeadDimMax = 256;      // the widest head whose O^T columns stay in registers beside its Q fragments
+constexpr int kFewRows    = 32;       // query rows of one MFMA column block: up to here waves split the KEYS, beyond the rows
+
+// padded head width of the kernels' tiles
+inline int heads_pad(int dk, int dv) {
+    const int d = dk > dv ? dk : dv;
+    return d <= 64 ? 64 : d <= 128 ? 128 : 256;
+}
+inline int elem_bytes(int dtype) { return dtype == SDPA_BF16 ? 2 : 4; }
+
+// 16-byte accesses hold for a tensor whose base, strides and row length are multiples of 16 bytes
+inline bool rows_vec(const sdpa_tensor &t, int dim, int dtype) {
+    const long e = elem_bytes(dtype), bad = (t.batch * e) | (t.token * e) | (t.head * e) | (dim * e);
+    return ((bad | (long)(size_t)t.data) & 15) == 0;
+}
+
+// One launch over one set of keys: its queries, where its rows go, and what they may see.
+struct AttendArgs {
+    sdpa_tensor q, k, v, out;
+    float *lse;                       // [B][Hq][Tq]
+    const int *q_lens, *kv_lens;      // [B] or null
+    float *part;                      // [slots][B*Tq*Hq][Dv] un-normalised rows (null: the launch writes out / lse itself)
+    float2 *stat;                     // [slots][B*Tq*Hq] (reference exponent, sum)
+    int slot0, splits;                // this launch's slots
+    int B, Tq, Tk, Hq, Hkv, Dk, Dv;
+    int window, sinks;
+    int shared;                       // 1 = one set of keys for the whole batch, all of them visible (a prefix)
+    int vec, vec_out;                 // 16-byte loads of q, k, v / whole 4-element stores of out
+    float scale_log2;                 // softmax scale * log2(e): scores are kept in the exp2 domain
+};
+
+struct BackwardArgs {
+    sdpa_tensor q, k, v, out, dout, dq, dk, dv;
+    const float *lse;
+    float *delta;                     // [B][Hq][Tq] row sums of dO * O
+    float *part;                      // partial dK | dV rows of the key blocks whose queries several workgroups share
+    const int *q_lens, *kv_lens;
+    int B, Tq, Tk, Hq, Hkv, Dk, Dv;
+    int window, sinks;
+    int sink_blocks, sink_chunks;     // key blocks with sink keys, and the workgroups each of them has
+    int rest_chunks;                  // workgroups of every other key block
+    int vec, vec_out;
+    float scale, scale_log2;
+};
+
+struct WeightArgs {
+    sdpa_tensor q, k;
+    const float *lse, *w_in;
+    float *w_out;
+    long wi_batch, wi_head, wo_batch, wo_head;
+    const int *q_lens, *kv_lens;
+    int B, Tq, Tk, Hq, Hkv, Dk, vec;
+    float scale_log2;
+};
+
+struct EvictArgs {
+    sdpa_tensor k, v, k_out, v_out;
+    const float *w_in;
+    float *w_out;
+    long wi_batch, wi_head, wo_batch, wo_head;
+    const int *lens;
+    int *lens_out, *kept;
+    int B, Tk, H, Dk, Dv, budget, sinks, recent, elem;
+    int vec_k, vec_v;
+};
+
+hipError_t launch_attend(const AttendArgs &a, int dtype, hipStream_t s);
+hipError_t launch_combine(const AttendArgs &a, int slots, int dtype, hipStream_t s);
+hipError_t launch_attend_backward(const BackwardArgs &a, int dtype, hipStream_t s);
+hipError_t launch_weights(const WeightArgs &a, int dtype, hipStream_t s);
+hipError_t launch_evict(const EvictArgs &a, hipStream_t s);
+
+// workgroups a launch over `rows` rows of every (sequence, key head) has before its keys are split
+inline int attend_row_tile(long rows) { return rows <= kFewRows ? kFewRows : 128; }
+inline int attend_key_tile(int dtype, int pad) { return pad * elem_bytes(dtype) <= 256 ? 64 : 32; }
+
+constexpr int kBwdKeys = 128;         // keys of a dK / dV workgroup (4 waves x 32)
+constexpr int kBwdRows = 128;         // rows of a dQ workgroup
+
+}  // namespace sdpa

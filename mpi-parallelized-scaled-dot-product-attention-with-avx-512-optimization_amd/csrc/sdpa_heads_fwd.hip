@@ -1,0 +1,409 @@
+// sdpa_heads_fwd.hip -- attention of grouped heads over a cache: the kernels behind attention_window, attention_prefix and
+// attention_scored.
+//
+// For a query row i with visible keys j:  s_ij = scale * q_i . k_j,  lse_i = log sum_j exp(s_ij),  out_i = sum_j
+// exp(s_ij - lse_i) v_j.  One pass over the keys with a running maximum m and sum l (exp2 domain):
+//     m' = max(m, max_j s_ij);  l' = l 2^(m-m') + sum_j 2^(s_ij - m');  O' = O 2^(m-m') + sum_j 2^(s_ij - m') v_j.
+// The rows of a key head are its tokens' grouped heads, r = t * G + g, so that the G heads that share keys share the tile they
+// are multiplied with, down to a single token.
+#include "sdpa_heads_device.h"
+
+namespace sdpa {
+namespace heads {
+namespace {
+
+struct RowId { int b, t, g; bool live; };
+
+__device__ inline RowId row_id(const AttendArgs &a, int b, int r, int rows, int G) {
+    RowId x;
+    const int bt = r / G;
+    x.g = r - bt * G;
+    if (a.shared) { x.b = bt / a.Tq; x.t = bt - x.b * a.Tq; }
+    else { x.b = b; x.t = bt; }
+    x.live = r < rows && x.t < (a.q_lens ? clamp_len(a.q_lens, x.b, a.Tq) : a.Tq);
+    return x;
+}
+
+// what a lane keeps of its column: reference exponent, sum, the un-normalised row
+template <int DP> struct State {
+    float m, l;
+    f32x16 o[DP / 32];
+    __device__ void clear() {
+        m = kNegInf; l = 0.f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    }
+};
+
+// one 32-key block: scores, running statistics, O += V^T P.  `full`: every live row of the wave sees every key.
+template <typename T, int DP>
+__device__ inline void attend_block(State<DP> &st, const typename Ops<T>::Frag *q, const char *lk, const char *lv, int block,
+                                    int j0, bool full, Seen seen, int sinks, float scale_log2, int lane) {
+    constexpr int STEPS = DP / Ops<T>::kStep;
+    f32x16 s = {};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(lk, block, i, lane), q[i], s);
+    uint32_t vis = 0xffffu;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= scale_log2;
+    if (!full) {
+        vis = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int j = j0 + row_of(i, lane >> 5);
+            const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
+            vis |= ok ? 1u << i : 0u;
+            s[i] = ok ? s[i] : kNegInf;
+        }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    const float m = fmaxf(st.m, half_max(mx));
+    const float ref = m == kNegInf ? 0.f : m;          // (nothing seen yet: every weight is 2^-inf = 0)
+    const float alpha = __builtin_amdgcn_exp2f(st.m - ref);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - ref); sum += s[i]; }
+    st.l = st.l * alpha + sum;                          // (the two lane halves' sums are joined once, behind the loop)
+    st.m = m;
+    const Probs<T> p = to_probs(s, T());
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[d][i] *= alpha;
+    mma_block<T, DP, DP / 32>(st.o, lv, block, p, !full, vis, 3, lane);
+}
+
+// a finished row (or its partial triple): 4 consecutive values of row `x`, columns d .. d + 3
+template <typename T>
+__device__ inline void store4(const AttendArgs &a, const RowId &x, int hq, int d, f32x4 v) {
+    T *row = (T *)a.out.data + x.b * a.out.batch + x.t * a.out.token + hq * a.out.head;
+    if (a.vec_out) {
+        if (d >= a.Dv) return;
+        union { T e[4]; uint64_t u; f32x4 f; } y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y.e[i] = from_f32<T>(v[i]);
+        if (sizeof(T) == 2) *reinterpret_cast<uint64_t *>(row + d) = y.u;
+        else *reinterpret_cast<f32x4 *>(row + d) = y.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < a.Dv) row[d + i] = from_f32<T>(v[i]);
+    }
+}
+
+__device__ inline void store_part4(const AttendArgs &a, long slot_row, int d, f32x4 v) {
+    float *row = a.part + slot_row * a.Dv;
+    if (a.Dv % 4 == 0) {
+        if (d < a.Dv) *reinterpret_cast<f32x4 *>(row + d) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < a.Dv) row[d + i] = v[i];
+    }
+}
+
+// the statistics of a row: lse, or the slot's (m, l).  An empty row: out 0, lse -inf.
+__device__ inline void store_stat(const AttendArgs &a, const RowId &x, int hq, int slot, float m, float l) {
+    if (a.part) a.stat[((long)slot * a.B + x.b) * a.Tq * a.Hq + (long)x.t * a.Hq + hq] = make_float2(m, l);
+    else a.lse[((long)x.b * a.Hq + hq) * a.Tq + x.t] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+}
+
+template <typename T, int DP>
+__device__ inline void load_query(typename Ops<T>::Frag *q, const AttendArgs &a, const RowId &x, int hq, int lane) {
+    const T *row = (const T *)a.q.data + x.b * a.q.batch + x.t * a.q.token + hq * a.q.head;
+#pragma unroll
+    for (int s = 0; s < DP / Ops<T>::kStep; ++s) {
+        union { u32x4 u; typename Ops<T>::Frag f; } y;
+        y.u = u32x4{0, 0, 0, 0};
+        if (x.live) y.u = load_chunk(row, s * Ops<T>::kStep + (lane >> 5) * Ops<T>::kVec, a.Dk, a.vec);
+        q[s] = y.f;
+    }
+}
+
+// ---- many rows: 128 of them share every key tile, each wave owns 32 ---------------------------------------------------
+template <typename T, int DP, int BN>
+__global__ __launch_bounds__(kHeadsThreads) void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
+    using TL = Tile<T, DP>;
+    __shared__ __attribute__((aligned(16))) char lk[BN * TL::kRowBytes];
+    __shared__ __attribute__((aligned(16))) char lv[BN * TL::kRowBytes];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int id = xcd_place(blockIdx.x, gridDim.x);
+    const int tile = tiles - 1 - id % tiles;             // (the rows that see most keys first)
+    id /= tiles;
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int h = id % a.Hkv, b = id / a.Hkv;
+    const int r0 = tile * 128, rw = r0 + wave * 32;
+    const RowId x = row_id(a, b, rw + (lane & 31), rows, G);
+    const int hq = h * G + x.g;
+
+    SeenRange wg, wv;
+    Seen seen = {0, 0};
+    if (a.shared) {
+        wg = SeenRange{a.Tk, a.Tk, 0, 0};
+        wv = wg;
+        if (x.live) seen.hi = a.Tk;
+    } else {
+        const int nq = clamp_len(a.q_lens, b, a.Tq), nk = clamp_len(a.kv_lens, b, a.Tk);
+        wg = seen_range(r0 / G, min(r0 + 127, rows - 1) / G, nq, nk, a.window);
+        wv = seen_range(rw / G, min(rw + 31, rows - 1) / G, nq, nk, a.window);
+        if (x.live) seen = seen_at(nk - nq + x.t, nk, a.window);
+    }
+    const TileList list = tile_list(wg, a.sinks, BN);
+    const int it0 = (int)((long)list.count * split / a.splits), it1 = (int)((long)list.count * (split + 1) / a.splits);
+
+    typename Ops<T>::Frag q[DP / Ops<T>::kStep];
+    load_query<T, DP>(q, a, x, hq, lane);
+    State<DP> st;
+    st.clear();
+
+    constexpr int PIECES = BN * TL::kChunks / kHeadsThreads;
+    u32x4 rk[PIECES], rv[PIECES];
+    const T *kb = (const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head;
+    const T *vb = (const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head;
+    auto fetch = [&](int it) {
+        const int j0 = list.at(it) * BN;
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int c = tid + k * kHeadsThreads, j = j0 + c / TL::kChunks, d = (c % TL::kChunks) * Ops<T>::kVec;
+            rk[k] = rv[k] = u32x4{0, 0, 0, 0};
+            if (j < wg.hi_max && (j >= wg.lo_min || j < a.sinks)) {      // (keys that no row sees are not read at all)
+                rk[k] = load_chunk(kb + (long)j * a.k.token, d, a.Dk, a.vec);
+                rv[k] = load_chunk(vb + (long)j * a.v.token, d, a.Dv, a.vec);
+            }
+        }
+    };
+    if (it0 < it1) fetch(it0);
+    for (int it = it0; it < it1; ++it) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int c = tid + k * kHeadsThreads, at = TL::chunk(c / TL::kChunks, c % TL::kChunks);
+            *reinterpret_cast<u32x4 *>(lk + at) = rk[k];
+            *reinterpret_cast<u32x4 *>(lv + at) = rv[k];
+        }
+        __syncthreads();
+        const int t0 = list.at(it) * BN;
+        if (it + 1 < it1) fetch(it + 1);
+#pragma unroll
+        for (int kb2 = 0; kb2 < BN / 32; ++kb2) {
+            const int j0 = t0 + kb2 * 32, j1 = j0 + 32;
+            if (j0 >= wv.hi_max || (j1 <= wv.lo_min && j0 >= a.sinks)) continue;
+            const bool full = j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks);
+            attend_block<T, DP>(st, q, lk, lv, kb2, j0, full, seen, a.sinks, a.scale_log2, lane);
+        }
+    }
+    st.l = half_sum(st.l);
+    if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (blocks that need no mask gave weights to rows that do not exist)
+    if (rw + (lane & 31) >= rows) return;
+    const int slot = a.slot0 + split;
+    if (lane < 32) store_stat(a, x, hq, slot, st.m, st.l);
+    const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
+    const long slot_row = ((long)slot * a.B + x.b) * a.Tq * a.Hq + (long)x.t * a.Hq + hq;
+    if (a.part && st.l == 0.f) return;                   // (the join does not read an empty slot)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = d * 32 + 8 * i + 4 * (lane >> 5);
+            f32x4 v = {st.o[d][4 * i], st.o[d][4 * i + 1], st.o[d][4 * i + 2], st.o[d][4 * i + 3]};
+            if (a.part) store_part4(a, slot_row, col, v);
+            else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = st.l == 0.f ? 0.f : v[k] * inv;
+                store4<T>(a, x, hq, col, v);
+            }
+        }
+}
+
+// ---- few rows (single tokens): the waves share 32 rows and take the key tiles in turn ------------------------------------
+// (fp32 rows of 256: two waves, whose tiles fill the LDS)
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, int rows, int G) {
+    using TL = Tile<T, DP>;
+    constexpr int WAVE_BYTES = 2 * 32 * TL::kRowBytes > 32 * DP * 4 ? 2 * 32 * TL::kRowBytes : 32 * DP * 4;
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * WAVE_BYTES];
+    __shared__ float lm[WAVES][32], ll[WAVES][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int id = xcd_place(blockIdx.x, gridDim.x);
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int h = id % a.Hkv, b = id / a.Hkv;
+    const RowId x = row_id(a, b, lane & 31, rows, G);
+    const int hq = h * G + x.g;
+
+    SeenRange wg;
+    Seen seen = {0, 0};
+    if (a.shared) {
+        wg = SeenRange{a.Tk, a.Tk, 0, 0};
+        if (x.live) seen.hi = a.Tk;
+    } else {
+        const int nq = clamp_len(a.q_lens, b, a.Tq), nk = clamp_len(a.kv_lens, b, a.Tk);
+        wg = seen_range(0, a.Tq - 1, nq, nk, a.window);
+        if (x.live) seen = seen_at(nk - nq + x.t, nk, a.window);
+    }
+    const TileList list = tile_list(wg, a.sinks, 32);
+    const int it0 = (int)((long)list.count * split / a.splits), it1 = (int)((long)list.count * (split + 1) / a.splits);
+
+    typename Ops<T>::Frag q[DP / Ops<T>::kStep];
+    load_query<T, DP>(q, a, x, hq, lane);
+    State<DP> st;
+    st.clear();
+
+    char *lk = lds + wave * WAVE_BYTES, *lv = lk + 32 * TL::kRowBytes;
+    const T *kb = (const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head;
+    const T *vb = (const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head;
+    constexpr int PIECES = 32 * TL::kChunks / 64;
+    for (int it = it0 + wave; it < it1; it += WAVES) {
+        const int j0 = list.at(it) * 32, j1 = j0 + 32;
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int c = lane + k * 64, row = c / TL::kChunks, j = j0 + row, d = (c % TL::kChunks) * Ops<T>::kVec;
+            u32x4 rk = {0, 0, 0, 0}, rv = {0, 0, 0, 0};
+            if (j < wg.hi_max && (j >= wg.lo_min || j < a.sinks)) {
+                rk = load_chunk(kb + (long)j * a.k.token, d, a.Dk, a.vec);
+                rv = load_chunk(vb + (long)j * a.v.token, d, a.Dv, a.vec);
+            }
+            const int at = TL::chunk(row, c % TL::kChunks);
+            *reinterpret_cast<u32x4 *>(lk + at) = rk;
+            *reinterpret_cast<u32x4 *>(lv + at) = rv;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (a wave reads only what it wrote itself)
+        const bool full = j1 <= wg.hi_min && (j0 >= wg.lo_max || j1 <= a.sinks);
+        attend_block<T, DP>(st, q, lk, lv, 0, j0, full, seen, a.sinks, a.scale_log2, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    st.l = half_sum(st.l);
+    if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (blocks that need no mask gave weights to rows that do not exist)
+    // the waves' triples become one
+    if (lane < 32) { lm[wave][lane] = st.m; ll[wave][lane] = st.l; }
+    __syncthreads();
+    const int col = lane & 31;
+    float m = lm[0][col];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) m = fmaxf(m, lm[w][col]);
+    const float ref = m == kNegInf ? 0.f : m;
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) l += ll[w][col] * __builtin_amdgcn_exp2f(lm[w][col] - ref);
+    const float alpha = __builtin_amdgcn_exp2f(st.m - ref);
+    float *lo = reinterpret_cast<float *>(lds + wave * WAVE_BYTES);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lo[(d * 32 + row_of(i, lane >> 5)) * 32 + col] = st.l == 0.f ? 0.f : st.o[d][i] * alpha;
+    __syncthreads();
+    if (col >= rows) return;
+    const int slot = a.slot0 + split;
+    if (wave == 0 && lane < 32) store_stat(a, x, hq, slot, m, l);
+    if (a.part && l == 0.f) return;
+    const float inv = a.part ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const long slot_row = ((long)slot * a.B + x.b) * a.Tq * a.Hq + (long)x.t * a.Hq + hq;
+    constexpr int RUN = DP / (2 * WAVES);                // columns of a thread
+    const int d0 = (tid >> 5) * RUN;
+#pragma unroll
+    for (int d = 0; d < RUN; d += 4) {
+        f32x4 v = {};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float *src = reinterpret_cast<const float *>(lds + w * WAVE_BYTES);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += src[(d0 + d + i) * 32 + col];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = l == 0.f ? 0.f : v[i] * inv;
+        if (a.part) store_part4(a, slot_row, d0 + d, v);
+        else store4<T>(a, x, hq, d0 + d, v);
+    }
+}
+
+// ---- the join of the slots: the merge of partial triples ------------------------------------------------------------
+// 32 lanes to a row, 8 rows to a workgroup.
+template <typename T>
+__global__ __launch_bounds__(kHeadsThreads) void combine_kernel(AttendArgs a, int slots) {
+    const long rows = (long)a.B * a.Tq * a.Hq, r = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const int lane = threadIdx.x & 31;
+    float m = kNegInf;
+    for (int s = 0; s < slots; ++s) {
+        const float2 ml = a.stat[s * rows + r];
+        if (ml.y != 0.f) m = fmaxf(m, ml.x);
+    }
+    RowId x;
+    const int hq = (int)(r % a.Hq);
+    const long bt = r / a.Hq;
+    x.b = (int)(bt / a.Tq); x.t = (int)(bt - (long)x.b * a.Tq); x.g = 0; x.live = true;
+    float l = 0.f;
+    f32x4 acc[2] = {};
+    const float ref = m == kNegInf ? 0.f : m;
+    for (int s = 0; s < slots; ++s) {
+        const float2 ml = a.stat[s * rows + r];
+        if (ml.y == 0.f) continue;
+        const float w = __builtin_amdgcn_exp2f(ml.x - ref);
+        l += ml.y * w;
+        const float *src = a.part + (s * rows + r) * a.Dv;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int d = k * 128 + lane * 4;
+            if (a.Dv % 4 == 0) {
+                if (d < a.Dv) acc[k] += w * *reinterpret_cast<const f32x4 *>(src + d);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (d + i < a.Dv) acc[k][i] += w * src[d + i];
+            }
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int d = k * 128 + lane * 4;
+        if (d < a.Dv) store4<T>(a, x, hq, d, acc[k] * inv);
+    }
+    if (lane == 0) a.lse[((long)x.b * a.Hq + hq) * a.Tq + x.t] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+}
+
+template <typename T, int DP>
+void attend(const AttendArgs &a, int rows, int G, int groups, hipStream_t s) {
+    constexpr int BN = DP * (int)sizeof(T) <= 256 ? 64 : 32;
+    if (rows <= kFewRows) {
+        constexpr int WAVES = DP * (int)sizeof(T) > 512 ? 2 : 4;
+        attend_few_kernel<T, DP, WAVES><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
+    } else {
+        const int tiles = (rows + 127) / 128;
+        attend_rows_kernel<T, DP, BN><<<groups * a.splits * tiles, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
+    }
+}
+
+template <typename T>
+void attend_dim(const AttendArgs &a, int rows, int G, int groups, hipStream_t s) {
+    switch (heads_pad(a.Dk, a.Dv)) {
+        case 64:  attend<T, 64>(a, rows, G, groups, s); break;
+        case 128: attend<T, 128>(a, rows, G, groups, s); break;
+        default:  attend<T, 256>(a, rows, G, groups, s); break;
+    }
+}
+
+}  // namespace
+}  // namespace heads
+
+hipError_t launch_attend(const AttendArgs &a, int dtype, hipStream_t s) {
+    const int G = a.Hq / a.Hkv, rows = (a.shared ? a.B : 1) * a.Tq * G, groups = (a.shared ? 1 : a.B) * a.Hkv;
+    if (dtype == SDPA_BF16) heads::attend_dim<__bf16>(a, rows, G, groups, s);
+    else heads::attend_dim<float>(a, rows, G, groups, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_combine(const AttendArgs &a, int slots, int dtype, hipStream_t s) {
+    const long rows = (long)a.B * a.Tq * a.Hq;
+    const unsigned grid = (unsigned)((rows + 7) / 8);
+    if (dtype == SDPA_BF16) heads::combine_kernel<__bf16><<<grid, heads::kHeadsThreads, 0, s>>>(a, slots);
+    else heads::combine_kernel<float><<<grid, heads::kHeadsThreads, 0, s>>>(a, slots);
+    return hipGetLastError();
+}
+
+}  // namespace sdpa

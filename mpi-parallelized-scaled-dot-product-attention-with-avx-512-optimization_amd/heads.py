@@ -1,0 +1,286 @@
+"""Batched attention of grouped heads over a cache: the device-level operators of include/sdpa_hip.h (struct sdpa_heads) on torch
+CUDA tensors.
+
+    attention_window            causal, a sliding window plus the first `sinks` tokens; a prompt, a chunk or one new token
+    attention_window_backward   its gradients
+    attention_prefix            a batch whose sequences share the first rows of their caches
+    attention_scored            causal, and every key's weight added to a running sum
+    evict_cache                 keeps the keys of greatest accumulated weight and moves them together
+
+Tensors are [batch, tokens, heads, dim] of float32 or bfloat16, any strides with contiguous dims (a head-major tensor is passed
+transposed); q has G times as many heads as k and v, dims are 1 to 256.  `q_lens`, `kv_lens`: int32 [batch] on the device (None = all
+tokens), clamped there to the tensors' token counts.  Query i < q_lens[b] is at position kv_lens[b] - q_lens[b] + i of its cache.  Rows
+that see no key (and rows behind q_lens) get out 0, lse -inf and gradient 0; keys behind kv_lens get gradient 0.
+
+All work is enqueued on torch's current stream of the tensors' device; scratch comes from torch's allocator, a piece of its own for
+every call.  Nothing waits for the device, so every call can be captured into a graph.  The operators are not
+recorded by autograd: a tensor that requires a gradient is refused while gradients are enabled (use `detach()` and
+`attention_window_backward`).
+"""
+import math
+import struct
+
+import torch
+
+from . import _lib
+from ._lib import SdpaError, check
+
+HEAD_DIM_MAX = 256
+_OP_WINDOW, _OP_WINDOW_BACKWARD, _OP_PREFIX, _OP_SCORED, _OP_EVICT = range(5)
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_INT_MAX = (1 << 31) - 1
+# struct sdpa_heads: 60 words (size, 10 tensors, 5 pointers, 4 strides, 2 tensors, 2 pointers), 13 ints, a float
+_PACK = struct.Struct("=60q13if")
+_NO = (0, 0, 0, 0)
+
+
+def _at(x):
+    return (x.data_ptr(),) + x.stride()[:3]
+
+
+def _call(fn, name, op, device, dtype, dims, scale=1.0, q=_NO, k=_NO, v=_NO, out=_NO, prefix=_NO + _NO, grads=_NO * 4, lse=None,
+          q_lens=None, kv_lens=None, weights=None, weights_out=None, cache=_NO + _NO, lens_out=None, kept=None, window=0, sinks=0,
+          prefix_tokens=0, budget=0, recent=0):
+    """pack struct sdpa_heads, take the scratch, enqueue"""
+    lib = _lib.load()
+    w = (weights.data_ptr() if weights is not None else 0, weights_out.data_ptr() if weights_out is not None else 0)
+    ws = (weights.stride()[:2] if weights is not None else (0, 0)) + (weights_out.stride()[:2] if weights_out is not None else (0, 0))
+    args = _PACK.pack(_PACK.size, *q, *k, *v, *out, *prefix, *grads, lse.data_ptr() if lse is not None else 0,
+                      q_lens.data_ptr() if q_lens is not None else 0, kv_lens.data_ptr() if kv_lens is not None else 0, *w, *ws,
+                      *cache, lens_out.data_ptr() if lens_out is not None else 0, kept.data_ptr() if kept is not None else 0,
+                      _DTYPES[dtype], *dims, window, sinks, prefix_tokens, budget, recent, scale)
+    need = lib.sdpa_dev_heads_workspace(op, args)
+    if need < 0:
+        check(need, name)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _enqueue(fn, name, args, need, device)
+    return _enqueue(fn, name, args, need, device)
+
+
+def _enqueue(fn, name, args, need, device):
+    ws = torch.empty((need,), dtype=torch.uint8, device=device).data_ptr() if need else None
+    check(fn(args, ws, need, torch.cuda.current_stream(device).cuda_stream), name)
+
+
+def _need(ok, text):
+    if not ok:
+        raise ValueError(text)
+
+
+def _rows(x, name, shape, dtype, device=None):
+    _need(isinstance(x, torch.Tensor), "%s: expected a tensor" % name)
+    _need(tuple(x.shape) == tuple(shape), "%s: expected shape %s, got %s" % (name, tuple(shape), tuple(x.shape)))
+    _need(x.dtype == dtype, "%s: expected %s, got %s" % (name, dtype, x.dtype))
+    _need(x.shape[-1] == 1 or x.stride(-1) == 1, "%s: the elements of a row must be contiguous" % name)
+    _need(device is None or x.device == device, "%s: expected a tensor on %s, got %s" % (name, device, x.device))
+    return x
+
+
+def _span(x):
+    if x.numel() == 0:
+        return 0, 0
+    a = x.data_ptr()
+    return a, a + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+
+def _apart(outs, ins, name):
+    """a caller's own output tensor must not lie over an input"""
+    for o in outs:
+        a0, a1 = _span(o)
+        for i in ins:
+            b0, b1 = _span(i)
+            _need(a1 <= b0 or b1 <= a0, "%s: an output overlaps an input" % name)
+
+
+def _lens(x, name, batch, device):
+    if x is not None:
+        _rows(x, name, (batch,), torch.int32, device)
+        _need(x.is_contiguous(), "%s: must be contiguous" % name)
+    return x
+
+
+def _count(x, name, low=0):
+    _need(isinstance(x, int) and not isinstance(x, bool) and x >= low, "%s: expected an integer >= %d" % (name, low))
+    return min(x, _INT_MAX)
+
+
+def _qkv(q, k, v, name):
+    """the shapes every attention shares -> (B, Tq, Tk, Hq, Hkv, Dk, Dv)"""
+    for x, n in ((q, "q"), (k, "k"), (v, "v")):
+        _need(isinstance(x, torch.Tensor) and x.dim() == 4, "%s: expected [batch, tokens, heads, dim]" % n)
+        _need(not (x.requires_grad and torch.is_grad_enabled()),
+              "%s requires a gradient: %s is not recorded by autograd, pass %s.detach()" % (n, name, n))
+    _need(q.dtype in _DTYPES, "q: expected float32 or bfloat16, got %s" % q.dtype)
+    B, Tq, Hq, Dk = q.shape
+    Tk, Hkv, Dv = k.shape[1], k.shape[2], v.shape[3]
+    _need(1 <= Dk <= HEAD_DIM_MAX and 1 <= Dv <= HEAD_DIM_MAX, "head dims must be 1 to %d" % HEAD_DIM_MAX)
+    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, "q's heads (%d) must be a multiple of k's (%d)" % (Hq, Hkv))
+    _rows(q, "q", q.shape, q.dtype)
+    _rows(k, "k", (B, Tk, Hkv, Dk), q.dtype, q.device)
+    _rows(v, "v", (B, Tk, Hkv, Dv), q.dtype, q.device)
+    return B, Tq, Tk, Hq, Hkv, Dk, Dv
+
+
+def _scale(scale, dk):
+    return 1.0 / math.sqrt(dk) if scale is None else float(scale)
+
+
+def _on_gpu(x, name):
+    if not x.is_cuda:
+        raise SdpaError(_lib.SDPA_ENODEV, name)
+
+
+def _outputs(q, Dv, out, lse, ins, name):
+    B, Tq, Hq = q.shape[:3]
+    if out is not None:
+        _rows(out, "out", (B, Tq, Hq, Dv), q.dtype, q.device)
+        _apart([out], ins, name)
+    if lse is not None:
+        _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
+        _need(lse.is_contiguous(), "lse: must be contiguous")
+        _apart([lse], ins, name)
+    _on_gpu(q, name)
+    if out is None:
+        out = torch.empty((B, Tq, Hq, Dv), dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=q.device)
+    return out, lse
+
+
+def attention_window(q, k, v, window, sinks=0, q_lens=None, kv_lens=None, scale=None, out=None, lse=None):
+    """Causal attention over the last `window` tokens (the query's own included) plus the first `sinks` tokens of the cache.
+    -> (out [B, Tq, Hq, Dv], lse [B, Hq, Tq]); window >= Tk is plain causal attention.  `out`, `lse`: tensors to write into."""
+    name = "attention_window"
+    B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    window, sinks = _count(window, "window"), _count(sinks, "sinks")
+    _lens(q_lens, "q_lens", B, q.device)
+    _lens(kv_lens, "kv_lens", B, q.device)
+    out, lse = _outputs(q, Dv, out, lse, (q, k, v), name)
+    _call(_lib.load().sdpa_dev_attention_window, name, _OP_WINDOW, q.device, q.dtype, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk),
+          q=_at(q), k=_at(k), v=_at(v), out=_at(out), lse=lse, q_lens=q_lens, kv_lens=kv_lens, window=window, sinks=sinks)
+    return out, lse
+
+
+def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=None, kv_lens=None, scale=None, dq=None, dk=None,
+                              dv=None):
+    """The gradients of attention_window from what it was given, what it returned and the gradient of `out`.
+    -> (dq, dk, dv), shaped and typed like q, k, v.  Deterministic.  `dq`, `dk`, `dv`: tensors to write into."""
+    name = "attention_window_backward"
+    B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    window, sinks = _count(window, "window"), _count(sinks, "sinks")
+    _lens(q_lens, "q_lens", B, q.device)
+    _lens(kv_lens, "kv_lens", B, q.device)
+    _rows(dout, "dout", (B, Tq, Hq, Dv), q.dtype, q.device)
+    _rows(out, "out", (B, Tq, Hq, Dv), q.dtype, q.device)
+    _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
+    _need(lse.is_contiguous(), "lse: must be contiguous")
+    ins = (dout, q, k, v, out, lse)
+    for x, n, like in ((dq, "dq", q), (dk, "dk", k), (dv, "dv", v)):
+        if x is not None:
+            _rows(x, n, like.shape, q.dtype, q.device)
+            _apart([x], ins, name)
+    _on_gpu(q, name)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if dk is None else dk
+    dv = torch.empty(v.shape, dtype=q.dtype, device=q.device) if dv is None else dv
+    _call(_lib.load().sdpa_dev_attention_window_backward, name, _OP_WINDOW_BACKWARD, q.device, q.dtype,
+          (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), q=_at(q), k=_at(k), v=_at(v), out=_at(out),
+          grads=_at(dout) + _at(dq) + _at(dk) + _at(dv), lse=lse, q_lens=q_lens, kv_lens=kv_lens, window=window, sinks=sinks)
+    return dq, dk, dv
+
+
+def attention_prefix(q, k_prefix, v_prefix, k, v, q_lens=None, kv_lens=None, scale=None, out=None, lse=None):
+    """Attention of a batch whose sequences all begin with the cache rows k_prefix [P, Hkv, Dk], v_prefix [P, Hkv, Dv]: every query
+    sees the whole prefix and, causally, its own sequence's k, v (lengths count that own part only).  The prefix is read once for
+    the batch.  -> (out, lse) over both parts."""
+    name = "attention_prefix"
+    B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    for x, n in ((k_prefix, "k_prefix"), (v_prefix, "v_prefix")):
+        _need(isinstance(x, torch.Tensor) and x.dim() == 3, "%s: expected [tokens, heads, dim]" % n)
+        _need(not (x.requires_grad and torch.is_grad_enabled()),
+              "%s requires a gradient: %s is not recorded by autograd, pass %s.detach()" % (n, name, n))
+    P = k_prefix.shape[0]
+    _rows(k_prefix, "k_prefix", (P, Hkv, Dk), q.dtype, q.device)
+    _rows(v_prefix, "v_prefix", (P, Hkv, Dv), q.dtype, q.device)
+    _lens(q_lens, "q_lens", B, q.device)
+    _lens(kv_lens, "kv_lens", B, q.device)
+    out, lse = _outputs(q, Dv, out, lse, (q, k, v, k_prefix, v_prefix), name)
+    prefix = (k_prefix.data_ptr(), 0) + k_prefix.stride()[:2] + (v_prefix.data_ptr(), 0) + v_prefix.stride()[:2]
+    _call(_lib.load().sdpa_dev_attention_prefix, name, _OP_PREFIX, q.device, q.dtype, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk),
+          q=_at(q), k=_at(k), v=_at(v), out=_at(out), prefix=prefix, lse=lse, q_lens=q_lens, kv_lens=kv_lens, prefix_tokens=P)
+    return out, lse
+
+
+def _weights(x, name, shape, device):
+    _rows(x, name, shape, torch.float32, device)
+    return x
+
+
+def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, weights_out=None, out=None, lse=None):
+    """Causal attention over the whole cache that keeps account of it: weights [B, Hkv, Tk] float32 is increased, in place or into
+    `weights_out`, by the softmax weight every key was given, summed over its group's heads and the queries.
+    -> (out, lse, the increased weights).  evict_cache() goes by these sums."""
+    name = "attention_scored"
+    B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    _weights(weights, "weights", (B, Hkv, Tk), q.device)
+    _lens(q_lens, "q_lens", B, q.device)
+    _lens(kv_lens, "kv_lens", B, q.device)
+    if weights_out is None:
+        weights_out = weights
+    elif weights_out is not weights:
+        _weights(weights_out, "weights_out", (B, Hkv, Tk), q.device)
+        _apart([weights_out], (q, k, v, weights), name)
+    _need(all(n == 1 or s > 0 for n, s in zip(weights_out.shape, weights_out.stride())), "weights_out: repeats elements")
+    _apart([weights_out], (q, k, v), name)
+    out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights), name)
+    _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q.device, q.dtype, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk),
+          q=_at(q), k=_at(k), v=_at(v), out=_at(out), lse=lse, q_lens=q_lens, kv_lens=kv_lens, weights=weights, weights_out=weights_out)
+    return out, lse, weights_out
+
+
+def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_out=None, weights_out=None):
+    """Cuts the cache of every sequence and key head to `budget` keys: those of the first `sinks`, of the last `recent` and, between
+    them, of the greatest accumulated weight (ties: the lower index; NaN counts below everything), in their order.  A sequence of
+    at most `budget` keys keeps all of them.
+    -> (k, v [B, budget, Hkv, dim], weights [B, Hkv, budget], lens [B], kept [B, Hkv, budget] = the old indices, -1 behind the end).
+    Slots behind the new length are zero.  `k_out`, `v_out`, `weights_out`: tensors of their own to write into, with at least
+    `budget` tokens; what lies behind `budget` in them is left as it was."""
+    name = "evict_cache"
+    for x, n in ((k, "k"), (v, "v")):
+        _need(isinstance(x, torch.Tensor) and x.dim() == 4, "%s: expected [batch, tokens, heads, dim]" % n)
+    _need(k.dtype in _DTYPES, "k: expected float32 or bfloat16, got %s" % k.dtype)
+    B, T, H, Dk = k.shape
+    Dv = v.shape[3]
+    _need(1 <= Dk <= HEAD_DIM_MAX and 1 <= Dv <= HEAD_DIM_MAX and H > 0, "head dims must be 1 to %d" % HEAD_DIM_MAX)
+    _rows(k, "k", k.shape, k.dtype)
+    _rows(v, "v", (B, T, H, Dv), k.dtype, k.device)
+    _weights(weights, "weights", (B, H, T), k.device)
+    _need(lens is None or isinstance(lens, torch.Tensor), "lens: expected an int32 tensor or None")
+    _lens(lens, "lens", B, k.device)
+    budget, sinks, recent = _count(budget, "budget"), _count(sinks, "sinks"), _count(recent, "recent")
+    _need(sinks + recent <= budget, "sinks + recent must not exceed the budget")
+    ins = (k, v, weights)
+    for x, n, dim in ((k_out, "k_out", Dk), (v_out, "v_out", Dv)):
+        if x is not None:
+            _need(isinstance(x, torch.Tensor) and x.dim() == 4 and x.shape[1] >= budget, "%s: needs %d tokens" % (n, budget))
+            _rows(x, n, (B, x.shape[1], H, dim), k.dtype, k.device)
+            _apart([x], ins, name)
+    if weights_out is not None:
+        _need(isinstance(weights_out, torch.Tensor) and weights_out.dim() == 3 and weights_out.shape[2] >= budget,
+              "weights_out: needs %d tokens" % budget)
+        _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k.device)
+        _need(all(n == 1 or s > 0 for n, s in zip(weights_out.shape, weights_out.stride())), "weights_out: repeats elements")
+        _apart([weights_out], ins, name)
+    _on_gpu(k, name)
+    new = dict(dtype=k.dtype, device=k.device)
+    k_out = torch.empty((B, budget, H, Dk), **new) if k_out is None else k_out
+    v_out = torch.empty((B, budget, H, Dv), **new) if v_out is None else v_out
+    if weights_out is None:
+        weights_out = torch.empty((B, H, budget), dtype=torch.float32, device=k.device)
+    lens_out = torch.empty((B,), dtype=torch.int32, device=k.device)
+    kept = torch.empty((B, H, budget), dtype=torch.int32, device=k.device)
+    _call(_lib.load().sdpa_dev_evict_cache, name, _OP_EVICT, k.device, k.dtype, (B, 0, T, H, H, Dk, Dv), k=_at(k), v=_at(v),
+          kv_lens=lens, weights=weights, weights_out=weights_out, cache=_at(k_out) + _at(v_out), lens_out=lens_out, kept=kept,
+          budget=budget, sinks=sinks, recent=recent)
+    return k_out, v_out, weights_out, lens_out, kept

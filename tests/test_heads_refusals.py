@@ -1,0 +1,167 @@
+"""CPU: the batched attention operators refuse what they cannot do, before anything is enqueued, and there is no CPU fallback."""
+import ctypes
+import struct
+
+import numpy as np
+import pytest
+import torch
+
+import _heads_reference as ref
+
+
+def qkv(B=2, Tq=3, Tk=5, Hq=4, Hkv=2, Dk=8, Dv=6, dtype=torch.float32):
+    return torch.zeros(B, Tq, Hq, Dk, dtype=dtype), torch.zeros(B, Tk, Hkv, Dk, dtype=dtype), torch.zeros(B, Tk, Hkv, Dv, dtype=dtype)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=torch.zeros(2, 3, 4)), dict(q=torch.zeros(2, 3, 3, 8)), dict(q=torch.zeros(2, 3, 4, 7)), dict(q=torch.zeros(1, 3, 4, 8)),
+    dict(q=torch.zeros(2, 3, 4, 8, dtype=torch.float64)), dict(q=torch.zeros(2, 3, 4, 8, dtype=torch.bfloat16)),
+    dict(q=torch.zeros(2, 3, 4, 16)[..., ::2]), dict(k=torch.zeros(2, 5, 2, 9)), dict(v=torch.zeros(2, 4, 2, 6)),
+    dict(v=torch.zeros(2, 5, 1, 6)), dict(q=torch.zeros(2, 3, 4, 8).requires_grad_()), dict(window=-1), dict(window=1.5),
+    dict(sinks=-1), dict(window=True), dict(q_lens=torch.zeros(2)), dict(q_lens=torch.zeros(3, dtype=torch.int32)),
+    dict(kv_lens=torch.zeros(2, dtype=torch.int64)), dict(kv_lens=[5, 5]), dict(kv_lens=torch.zeros(4, dtype=torch.int32)[::2]),
+    dict(out=torch.zeros(2, 3, 4, 8)), dict(lse=torch.zeros(2, 3, 4)), dict(q=torch.zeros(2, 3, 4, 300), k=torch.zeros(2, 5, 2, 300)),
+], ids=lambda kw: "-".join("%s" % k for k in kw))
+def test_window_refuses(kw, pkg):
+    q, k, v = qkv()
+    args = dict(q=q, k=k, v=v, window=4)
+    args.update(kw)
+    with pytest.raises(ValueError):
+        pkg.attention_window(**args)
+
+
+def test_outputs_over_inputs_are_refused(pkg):
+    q, k, v = qkv(Dv=8)
+    with pytest.raises(ValueError, match="overlaps"):
+        pkg.attention_window(q, k, v, 4, out=q)
+    with pytest.raises(ValueError, match="overlaps"):
+        pkg.attention_window_backward(q, q, k, v, q.clone(), torch.zeros(2, 4, 3), 4, dk=k)
+    w = torch.zeros(2, 2, 5)
+    with pytest.raises(ValueError, match="overlaps"):
+        pkg.evict_cache(k, v, w, None, 4, k_out=k)
+    with pytest.raises(ValueError, match="overlaps"):
+        pkg.evict_cache(k, v, w, None, 4, weights_out=w)
+
+
+@pytest.mark.parametrize("kw", [dict(dout=torch.zeros(2, 3, 4, 8)), dict(out=torch.zeros(2, 3, 4, 6, dtype=torch.bfloat16)),
+                                dict(lse=torch.zeros(2, 3, 4)), dict(dq=torch.zeros(2, 3, 4, 6)), dict(dv=torch.zeros(2, 5, 2, 8))],
+                         ids=lambda kw: "-".join(kw))
+def test_backward_refuses(kw, pkg):
+    q, k, v = qkv()
+    args = dict(dout=torch.zeros(2, 3, 4, 6), q=q, k=k, v=v, out=torch.zeros(2, 3, 4, 6), lse=torch.zeros(2, 4, 3), window=4)
+    args.update(kw)
+    with pytest.raises(ValueError):
+        pkg.attention_window_backward(**args)
+
+
+@pytest.mark.parametrize("kw", [dict(k_prefix=torch.zeros(7, 2, 6)), dict(v_prefix=torch.zeros(6, 2, 6)), dict(k_prefix=torch.zeros(1, 7, 2, 8)),
+                                dict(v_prefix=torch.zeros(7, 1, 6))], ids=str)
+def test_prefix_refuses(kw, pkg):
+    q, k, v = qkv()
+    args = dict(q=q, k_prefix=torch.zeros(7, 2, 8), v_prefix=torch.zeros(7, 2, 6), k=k, v=v)
+    args.update(kw)
+    with pytest.raises(ValueError):
+        pkg.attention_prefix(**args)
+
+
+@pytest.mark.parametrize("kw", [dict(weights=torch.zeros(2, 2, 4)), dict(weights=torch.zeros(2, 2, 5, dtype=torch.bfloat16)),
+                                dict(weights=torch.zeros(1, 2, 5).expand(2, 2, 5)), dict(weights_out=torch.zeros(2, 4, 5))], ids=str)
+def test_scored_refuses(kw, pkg):
+    q, k, v = qkv()
+    args = dict(q=q, k=k, v=v, weights=torch.zeros(2, 2, 5))
+    args.update(kw)
+    with pytest.raises(ValueError):
+        pkg.attention_scored(**args)
+
+
+@pytest.mark.parametrize("kw", [dict(budget=-1), dict(budget=3, sinks=2, recent=2), dict(lens=torch.zeros(2)), dict(lens=[5, 5]),
+                                dict(weights=torch.zeros(2, 5, 2)), dict(k_out=torch.zeros(2, 3, 2, 8)), dict(v_out=torch.zeros(2, 4, 2, 8)),
+                                dict(weights_out=torch.zeros(2, 2, 3)), dict(sinks=-1), dict(recent=-1)], ids=str)
+def test_evict_refuses(kw, pkg):
+    _, k, v = qkv()
+    args = dict(k=k, v=v, weights=torch.zeros(2, 2, 5), lens=None, budget=4)
+    args.update(kw)
+    with pytest.raises(ValueError):
+        pkg.evict_cache(**args)
+
+
+def test_no_cpu_fallback(pkg):
+    q, k, v = qkv()
+    w = torch.zeros(2, 2, 5)
+    for f in (lambda: pkg.attention_window(q, k, v, 4), lambda: pkg.attention_scored(q, k, v, w),
+              lambda: pkg.attention_prefix(q, k[0], v[0], k, v), lambda: pkg.evict_cache(k, v, w, None, 4),
+              lambda: pkg.attention_window_backward(torch.zeros(2, 3, 4, 6), q, k, v, torch.zeros(2, 3, 4, 6), torch.zeros(2, 4, 3), 4)):
+        with pytest.raises(pkg.SdpaError) as e:
+            f()
+        assert e.value.code == pkg._lib.SDPA_ENODEV
+
+
+# ---- the C entries: nothing but the checks runs here -----------------------------------------------------------------------------
+def pack(**kw):
+    """struct sdpa_heads of a small valid problem (pointers that are never followed), with fields replaced"""
+    f = dict(size=None, q=(4096, 96, 32, 8), k=(4096, 80, 16, 8), v=(4096, 60, 12, 6), out=(4096, 72, 24, 6), kp=(0, 0, 0, 0), vp=(0, 0, 0, 0),
+             dout=(4096, 72, 24, 6), dq=(4096, 96, 32, 8), dk_out=(4096, 80, 16, 8), dv_out=(4096, 60, 12, 6), lse=4096, q_lens=0, kv_lens=0,
+             weights=4096, weights_out=4096, ws=(10, 5, 10, 5), k_out=(8192, 64, 16, 8), v_out=(8192, 48, 12, 6), lens_out=4096, kept=4096,
+             dtype=0, batch=2, q_tokens=3, kv_tokens=5, q_heads=4, kv_heads=2, dk=8, dv=6, window=4, sinks=1, prefix=0, budget=4, recent=1,
+             scale=0.5)
+    f.update(kw)
+    fmt = struct.Struct("=60q13if")
+    return fmt.pack(fmt.size if f["size"] is None else f["size"], *f["q"], *f["k"], *f["v"], *f["out"], *f["kp"], *f["vp"], *f["dout"], *f["dq"],
+                    *f["dk_out"], *f["dv_out"], f["lse"], f["q_lens"], f["kv_lens"], f["weights"], f["weights_out"], *f["ws"], *f["k_out"],
+                    *f["v_out"], f["lens_out"], f["kept"], f["dtype"], f["batch"], f["q_tokens"], f["kv_tokens"], f["q_heads"], f["kv_heads"],
+                    f["dk"], f["dv"], f["window"], f["sinks"], f["prefix"], f["budget"], f["recent"], f["scale"])
+
+
+ENTRIES = ["sdpa_dev_attention_window", "sdpa_dev_attention_window_backward", "sdpa_dev_attention_prefix", "sdpa_dev_attention_scored",
+           "sdpa_dev_evict_cache"]
+
+
+@pytest.mark.parametrize("op", range(5))
+@pytest.mark.parametrize("kw,code", [
+    (dict(size=8), -1), (dict(dtype=2), -1), (dict(batch=-1), -1), (dict(kv_tokens=-1), -1), (dict(kv_heads=0), -1), (dict(dk=0), -1),
+    (dict(dv=257), -6), (dict(dk=1000), -6), (dict(kv_tokens=(1 << 30) + 1), -6), (dict(sinks=-1), -1), (dict(k=(0, 80, 16, 8)), -1),
+    (dict(k=(4096, 80, -16, 8)), -1)], ids=str)
+def test_c_entries_refuse(op, kw, code, pkg):
+    lib = pkg.load()
+    assert getattr(lib, ENTRIES[op])(pack(**kw), 4096, 1 << 20, None) == code
+    if "k" not in kw:
+        assert lib.sdpa_dev_heads_workspace(op, pack(**kw)) == code
+
+
+@pytest.mark.parametrize("op,kw,code", [
+    (0, dict(q_heads=3), -1), (0, dict(window=-1), -1), (0, dict(lse=0), -1), (0, dict(out=(4096, 0, 24, 6)), -1), (0, dict(scale=float("nan")), -1),
+    (1, dict(dq=(0, 96, 32, 8)), -1), (1, dict(dv_out=(4096, 60, 0, 6)), -1), (1, dict(dout=(0, 1, 1, 1)), -1), (2, dict(prefix=4), -1),
+    (2, dict(prefix=-1), -1), (3, dict(weights=0), -1), (3, dict(ws=(10, 5, -1, 5)), -1), (4, dict(budget=1), -1), (4, dict(kept=0), -1),
+    (4, dict(lens_out=0), -1), (4, dict(k_out=(4096, 64, 0, 8)), -1), (0, dict(batch=1 << 20, q_tokens=1 << 20), -6)], ids=str)
+def test_c_entries_refuse_their_own(op, kw, code, pkg):
+    assert getattr(pkg.load(), ENTRIES[op])(pack(**kw), 4096, 1 << 20, None) == code
+
+
+def test_c_entries_refuse_null_and_too_little_scratch(pkg):
+    lib = pkg.load()
+    for op, name in enumerate(ENTRIES):
+        assert getattr(lib, name)(None, None, 0, None) == -1
+        assert lib.sdpa_dev_heads_workspace(op, None) == -1
+    need = lib.sdpa_dev_heads_workspace(1, pack())
+    assert need > 0
+    assert lib.sdpa_dev_attention_window_backward(pack(), None, need, None) == -1
+    assert lib.sdpa_dev_attention_window_backward(pack(), 4096, need - 1, None) == -1
+    assert lib.sdpa_dev_attention_window_backward(pack(), 4100, need, None) == -1
+    assert lib.sdpa_dev_heads_workspace(9, pack()) == -1
+
+
+def test_the_reference_gradient_is_the_derivative():
+    """the 64-bit formulas the GPU tests go by, against central differences"""
+    rng = np.random.default_rng(3)
+    q, k, v, g = (rng.standard_normal(s) for s in ((9, 5), (11, 5), (11, 4), (9, 4)))
+    see, scale = ref.visible(9, 11, 4, 2), 0.4
+    out, _, p, _, _, err = ref.attention(q, k, v, see, scale, "f32")
+    grads = ref.gradients(q, k, v, g, p, out, err, scale, "f32")[:3]
+
+    def loss(q, k, v):
+        return (ref.attention(q, k, v, see, scale, "f32")[0] * g).sum()
+    for i, x in enumerate((q, k, v)):
+        d, h = rng.standard_normal(x.shape), 1e-6
+        up, down = [q, k, v], [q, k, v]
+        up[i], down[i] = x + h * d, x - h * d
+        assert abs((loss(*up) - loss(*down)) / (2 * h) - (grads[i] * d).sum()) < 1e-7
