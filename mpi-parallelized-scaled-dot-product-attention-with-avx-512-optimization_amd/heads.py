@@ -32,35 +32,34 @@ _INT_MAX = (1 << 31) - 1
 # struct sdpa_heads: 60 words (size, 10 tensors, 5 pointers, 4 strides, 2 tensors, 2 pointers), 13 ints, a float
 _PACK = struct.Struct("=60q13if")
 _NO = (0, 0, 0, 0)
+_NO2, _NO4, _NO6 = _NO * 2, _NO * 4, (0,) * 6
+# (the stream's number without a Stream object around it: a microsecond and a half of a call that takes ten)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _at(x):
     return (x.data_ptr(),) + x.stride()[:3]
 
 
-def _call(fn, name, op, device, dtype, dims, scale=1.0, q=_NO, k=_NO, v=_NO, out=_NO, prefix=_NO + _NO, grads=_NO * 4, lse=None,
-          q_lens=None, kv_lens=None, weights=None, weights_out=None, cache=_NO + _NO, lens_out=None, kept=None, window=0, sinks=0,
-          prefix_tokens=0, budget=0, recent=0):
-    """pack struct sdpa_heads, take the scratch, enqueue"""
-    lib = _lib.load()
-    w = (weights.data_ptr() if weights is not None else 0, weights_out.data_ptr() if weights_out is not None else 0)
-    ws = (weights.stride()[:2] if weights is not None else (0, 0)) + (weights_out.stride()[:2] if weights_out is not None else (0, 0))
-    args = _PACK.pack(_PACK.size, *q, *k, *v, *out, *prefix, *grads, lse.data_ptr() if lse is not None else 0,
-                      q_lens.data_ptr() if q_lens is not None else 0, kv_lens.data_ptr() if kv_lens is not None else 0, *w, *ws,
-                      *cache, lens_out.data_ptr() if lens_out is not None else 0, kept.data_ptr() if kept is not None else 0,
-                      _DTYPES[dtype], *dims, window, sinks, prefix_tokens, budget, recent, scale)
-    need = lib.sdpa_dev_heads_workspace(op, args)
-    if need < 0:
-        check(need, name)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _enqueue(fn, name, args, need, device)
-    return _enqueue(fn, name, args, need, device)
+def _pack(q, dims, scale, window=0, sinks=0, prefix_tokens=0, budget=0, recent=0, k=_NO, v=_NO, out=_NO, prefix=_NO2, grads=_NO4, lse=0,
+          q_lens=None, kv_lens=None, weights=_NO6, cache=_NO2, new=(0, 0)):
+    """struct sdpa_heads as bytes"""
+    return _PACK.pack(_PACK.size, *_at(q), *k, *v, *out, *prefix, *grads, lse, 0 if q_lens is None else q_lens.data_ptr(),
+                      0 if kv_lens is None else kv_lens.data_ptr(), *weights, *cache, *new, _DTYPES[q.dtype], *dims, window, sinks,
+                      prefix_tokens, budget, recent, scale)
 
 
-def _enqueue(fn, name, args, need, device):
-    ws = torch.empty((need,), dtype=torch.uint8, device=device).data_ptr() if need else None
-    check(fn(args, ws, need, torch.cuda.current_stream(device).cuda_stream), name)
+def _call(fn, name, op, x, args):
+    """take the scratch and enqueue, on the device and current stream of tensor x"""
+    i = x.get_device()
+    if i != torch.cuda.current_device():
+        with torch.cuda.device(i):
+            return _call(fn, name, op, x, args)
+    need = _lib.load().sdpa_dev_heads_workspace(op, args)
+    ws = x.new_empty((need,), dtype=torch.uint8) if need > 0 else None          # (held until the work is enqueued)
+    code = fn(args, None if ws is None else ws.data_ptr(), need, _raw_stream(i)) if need >= 0 else need
+    if code:
+        check(code, name)
 
 
 def _need(ok, text):
@@ -93,32 +92,50 @@ def _apart(outs, ins, name):
             _need(a1 <= b0 or b1 <= a0, "%s: an output overlaps an input" % name)
 
 
-def _lens(x, name, batch, device):
-    if x is not None:
-        _rows(x, name, (batch,), torch.int32, device)
-        _need(x.is_contiguous(), "%s: must be contiguous" % name)
-    return x
+def _lens(x, name, batch, like):
+    """lengths (None = all); accepted at once where all is well, as in the other checks a small call meets"""
+    if x is None or (type(x) is torch.Tensor and x.dtype is torch.int32 and x.shape == (batch,) and x.device == like.device and
+                     x.is_contiguous()):
+        return
+    _rows(x, name, (batch,), torch.int32, like.device)
+    _need(x.is_contiguous(), "%s: must be contiguous" % name)
 
 
-def _count(x, name, low=0):
-    _need(isinstance(x, int) and not isinstance(x, bool) and x >= low, "%s: expected an integer >= %d" % (name, low))
-    return min(x, _INT_MAX)
+def _count(x, name):
+    if type(x) is not int or x < 0:
+        _need(isinstance(x, int) and not isinstance(x, bool) and x >= 0, "%s: expected an integer >= 0" % name)
+    return x if x < _INT_MAX else _INT_MAX
+
+
+def _fits(x, shape, like):
+    """an operand as it should be: shape, type, device, contiguous rows, no gradient to record"""
+    return (type(x) is torch.Tensor and x.shape == shape and x.dtype is like.dtype and x.device == like.device and
+            (x.stride(-1) == 1 or shape[-1] == 1) and not (x.requires_grad and torch.is_grad_enabled()))
+
+
+def _operand(x, name, shape, like, call):
+    if not _fits(x, shape, like):
+        _rows(x, name, shape, like.dtype, like.device)
+        _need(not (x.requires_grad and torch.is_grad_enabled()),
+              "%s requires a gradient: %s is not recorded by autograd, pass %s.detach()" % (name, call, name))
 
 
 def _qkv(q, k, v, name):
     """the shapes every attention shares -> (B, Tq, Tk, Hq, Hkv, Dk, Dv)"""
     for x, n in ((q, "q"), (k, "k"), (v, "v")):
-        _need(isinstance(x, torch.Tensor) and x.dim() == 4, "%s: expected [batch, tokens, heads, dim]" % n)
-        _need(not (x.requires_grad and torch.is_grad_enabled()),
-              "%s requires a gradient: %s is not recorded by autograd, pass %s.detach()" % (n, name, n))
-    _need(q.dtype in _DTYPES, "q: expected float32 or bfloat16, got %s" % q.dtype)
+        if not isinstance(x, torch.Tensor) or x.dim() != 4:
+            raise ValueError("%s: expected [batch, tokens, heads, dim]" % n)
     B, Tq, Hq, Dk = q.shape
     Tk, Hkv, Dv = k.shape[1], k.shape[2], v.shape[3]
-    _need(1 <= Dk <= HEAD_DIM_MAX and 1 <= Dv <= HEAD_DIM_MAX, "head dims must be 1 to %d" % HEAD_DIM_MAX)
-    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, "q's heads (%d) must be a multiple of k's (%d)" % (Hq, Hkv))
-    _rows(q, "q", q.shape, q.dtype)
-    _rows(k, "k", (B, Tk, Hkv, Dk), q.dtype, q.device)
-    _rows(v, "v", (B, Tk, Hkv, Dv), q.dtype, q.device)
+    if q.dtype not in _DTYPES:
+        raise ValueError("q: expected float32 or bfloat16, got %s" % q.dtype)
+    if not (1 <= Dk <= HEAD_DIM_MAX and 1 <= Dv <= HEAD_DIM_MAX):
+        raise ValueError("head dims must be 1 to %d" % HEAD_DIM_MAX)
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("q's heads (%d) must be a multiple of k's (%d)" % (Hq, Hkv))
+    _operand(q, "q", (B, Tq, Hq, Dk), q, name)
+    _operand(k, "k", (B, Tk, Hkv, Dk), q, name)
+    _operand(v, "v", (B, Tk, Hkv, Dv), q, name)
     return B, Tq, Tk, Hq, Hkv, Dk, Dv
 
 
@@ -142,9 +159,9 @@ def _outputs(q, Dv, out, lse, ins, name):
         _apart([lse], ins, name)
     _on_gpu(q, name)
     if out is None:
-        out = torch.empty((B, Tq, Hq, Dv), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, Tq, Hq, Dv))
     if lse is None:
-        lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((B, Hq, Tq), dtype=torch.float32)
     return out, lse
 
 
@@ -154,11 +171,12 @@ def attention_window(q, k, v, window, sinks=0, q_lens=None, kv_lens=None, scale=
     name = "attention_window"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
     window, sinks = _count(window, "window"), _count(sinks, "sinks")
-    _lens(q_lens, "q_lens", B, q.device)
-    _lens(kv_lens, "kv_lens", B, q.device)
+    _lens(q_lens, "q_lens", B, q)
+    _lens(kv_lens, "kv_lens", B, q)
     out, lse = _outputs(q, Dv, out, lse, (q, k, v), name)
-    _call(_lib.load().sdpa_dev_attention_window, name, _OP_WINDOW, q.device, q.dtype, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk),
-          q=_at(q), k=_at(k), v=_at(v), out=_at(out), lse=lse, q_lens=q_lens, kv_lens=kv_lens, window=window, sinks=sinks)
+    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), window, sinks, k=_at(k), v=_at(v), out=_at(out), lse=lse.data_ptr(),
+                 q_lens=q_lens, kv_lens=kv_lens)
+    _call(_lib.load().sdpa_dev_attention_window, name, _OP_WINDOW, q, args)
     return out, lse
 
 
@@ -169,10 +187,10 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
     name = "attention_window_backward"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
     window, sinks = _count(window, "window"), _count(sinks, "sinks")
-    _lens(q_lens, "q_lens", B, q.device)
-    _lens(kv_lens, "kv_lens", B, q.device)
-    _rows(dout, "dout", (B, Tq, Hq, Dv), q.dtype, q.device)
-    _rows(out, "out", (B, Tq, Hq, Dv), q.dtype, q.device)
+    _lens(q_lens, "q_lens", B, q)
+    _lens(kv_lens, "kv_lens", B, q)
+    _operand(dout, "dout", (B, Tq, Hq, Dv), q, name)
+    _operand(out, "out", (B, Tq, Hq, Dv), q, name)
     _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
     _need(lse.is_contiguous(), "lse: must be contiguous")
     ins = (dout, q, k, v, out, lse)
@@ -181,12 +199,12 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
             _rows(x, n, like.shape, q.dtype, q.device)
             _apart([x], ins, name)
     _on_gpu(q, name)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if dk is None else dk
-    dv = torch.empty(v.shape, dtype=q.dtype, device=q.device) if dv is None else dv
-    _call(_lib.load().sdpa_dev_attention_window_backward, name, _OP_WINDOW_BACKWARD, q.device, q.dtype,
-          (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), q=_at(q), k=_at(k), v=_at(v), out=_at(out),
-          grads=_at(dout) + _at(dq) + _at(dk) + _at(dv), lse=lse, q_lens=q_lens, kv_lens=kv_lens, window=window, sinks=sinks)
+    dq = q.new_empty(q.shape) if dq is None else dq
+    dk = q.new_empty(k.shape) if dk is None else dk
+    dv = q.new_empty(v.shape) if dv is None else dv
+    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), window, sinks, k=_at(k), v=_at(v), out=_at(out),
+                 grads=_at(dout) + _at(dq) + _at(dk) + _at(dv), lse=lse.data_ptr(), q_lens=q_lens, kv_lens=kv_lens)
+    _call(_lib.load().sdpa_dev_attention_window_backward, name, _OP_WINDOW_BACKWARD, q, args)
     return dq, dk, dv
 
 
@@ -198,23 +216,28 @@ def attention_prefix(q, k_prefix, v_prefix, k, v, q_lens=None, kv_lens=None, sca
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
     for x, n in ((k_prefix, "k_prefix"), (v_prefix, "v_prefix")):
         _need(isinstance(x, torch.Tensor) and x.dim() == 3, "%s: expected [tokens, heads, dim]" % n)
-        _need(not (x.requires_grad and torch.is_grad_enabled()),
-              "%s requires a gradient: %s is not recorded by autograd, pass %s.detach()" % (n, name, n))
     P = k_prefix.shape[0]
-    _rows(k_prefix, "k_prefix", (P, Hkv, Dk), q.dtype, q.device)
-    _rows(v_prefix, "v_prefix", (P, Hkv, Dv), q.dtype, q.device)
-    _lens(q_lens, "q_lens", B, q.device)
-    _lens(kv_lens, "kv_lens", B, q.device)
+    _operand(k_prefix, "k_prefix", (P, Hkv, Dk), q, name)
+    _operand(v_prefix, "v_prefix", (P, Hkv, Dv), q, name)
+    _lens(q_lens, "q_lens", B, q)
+    _lens(kv_lens, "kv_lens", B, q)
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, k_prefix, v_prefix), name)
     prefix = (k_prefix.data_ptr(), 0) + k_prefix.stride()[:2] + (v_prefix.data_ptr(), 0) + v_prefix.stride()[:2]
-    _call(_lib.load().sdpa_dev_attention_prefix, name, _OP_PREFIX, q.device, q.dtype, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk),
-          q=_at(q), k=_at(k), v=_at(v), out=_at(out), prefix=prefix, lse=lse, q_lens=q_lens, kv_lens=kv_lens, prefix_tokens=P)
+    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), prefix_tokens=P, k=_at(k), v=_at(v), out=_at(out), prefix=prefix,
+                 lse=lse.data_ptr(), q_lens=q_lens, kv_lens=kv_lens)
+    _call(_lib.load().sdpa_dev_attention_prefix, name, _OP_PREFIX, q, args)
     return out, lse
 
 
-def _weights(x, name, shape, device):
-    _rows(x, name, shape, torch.float32, device)
-    return x
+def _weights(x, name, shape, like, written=False):
+    """[batch, heads, tokens] float32; one that is written must not repeat elements"""
+    if not (type(x) is torch.Tensor and x.shape == shape and x.dtype is torch.float32 and x.device == like.device and x.is_contiguous()):
+        _rows(x, name, shape, torch.float32, like.device)
+        _need(not written or all(n == 1 or s > 0 for n, s in zip(x.shape, x.stride())), "%s: repeats elements" % name)
+
+
+def _sums(weights, weights_out):
+    return (weights.data_ptr(), weights_out.data_ptr()) + weights.stride()[:2] + weights_out.stride()[:2]
 
 
 def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, weights_out=None, out=None, lse=None):
@@ -223,19 +246,18 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
     -> (out, lse, the increased weights).  evict_cache() goes by these sums."""
     name = "attention_scored"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
-    _weights(weights, "weights", (B, Hkv, Tk), q.device)
-    _lens(q_lens, "q_lens", B, q.device)
-    _lens(kv_lens, "kv_lens", B, q.device)
+    _weights(weights, "weights", (B, Hkv, Tk), q, weights_out is None)
+    _lens(q_lens, "q_lens", B, q)
+    _lens(kv_lens, "kv_lens", B, q)
     if weights_out is None:
         weights_out = weights
     elif weights_out is not weights:
-        _weights(weights_out, "weights_out", (B, Hkv, Tk), q.device)
+        _weights(weights_out, "weights_out", (B, Hkv, Tk), q, True)
         _apart([weights_out], (q, k, v, weights), name)
-    _need(all(n == 1 or s > 0 for n, s in zip(weights_out.shape, weights_out.stride())), "weights_out: repeats elements")
-    _apart([weights_out], (q, k, v), name)
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights), name)
-    _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q.device, q.dtype, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk),
-          q=_at(q), k=_at(k), v=_at(v), out=_at(out), lse=lse, q_lens=q_lens, kv_lens=kv_lens, weights=weights, weights_out=weights_out)
+    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), k=_at(k), v=_at(v), out=_at(out), lse=lse.data_ptr(), q_lens=q_lens,
+                 kv_lens=kv_lens, weights=_sums(weights, weights_out))
+    _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q, args)
     return out, lse, weights_out
 
 
@@ -253,11 +275,10 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
     B, T, H, Dk = k.shape
     Dv = v.shape[3]
     _need(1 <= Dk <= HEAD_DIM_MAX and 1 <= Dv <= HEAD_DIM_MAX and H > 0, "head dims must be 1 to %d" % HEAD_DIM_MAX)
-    _rows(k, "k", k.shape, k.dtype)
-    _rows(v, "v", (B, T, H, Dv), k.dtype, k.device)
-    _weights(weights, "weights", (B, H, T), k.device)
-    _need(lens is None or isinstance(lens, torch.Tensor), "lens: expected an int32 tensor or None")
-    _lens(lens, "lens", B, k.device)
+    _operand(k, "k", (B, T, H, Dk), k, name)
+    _operand(v, "v", (B, T, H, Dv), k, name)
+    _weights(weights, "weights", (B, H, T), k)
+    _lens(lens, "lens", B, k)
     budget, sinks, recent = _count(budget, "budget"), _count(sinks, "sinks"), _count(recent, "recent")
     _need(sinks + recent <= budget, "sinks + recent must not exceed the budget")
     ins = (k, v, weights)
@@ -269,18 +290,15 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
     if weights_out is not None:
         _need(isinstance(weights_out, torch.Tensor) and weights_out.dim() == 3 and weights_out.shape[2] >= budget,
               "weights_out: needs %d tokens" % budget)
-        _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k.device)
-        _need(all(n == 1 or s > 0 for n, s in zip(weights_out.shape, weights_out.stride())), "weights_out: repeats elements")
+        _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k, True)
         _apart([weights_out], ins, name)
     _on_gpu(k, name)
-    new = dict(dtype=k.dtype, device=k.device)
-    k_out = torch.empty((B, budget, H, Dk), **new) if k_out is None else k_out
-    v_out = torch.empty((B, budget, H, Dv), **new) if v_out is None else v_out
-    if weights_out is None:
-        weights_out = torch.empty((B, H, budget), dtype=torch.float32, device=k.device)
-    lens_out = torch.empty((B,), dtype=torch.int32, device=k.device)
-    kept = torch.empty((B, H, budget), dtype=torch.int32, device=k.device)
-    _call(_lib.load().sdpa_dev_evict_cache, name, _OP_EVICT, k.device, k.dtype, (B, 0, T, H, H, Dk, Dv), k=_at(k), v=_at(v),
-          kv_lens=lens, weights=weights, weights_out=weights_out, cache=_at(k_out) + _at(v_out), lens_out=lens_out, kept=kept,
-          budget=budget, sinks=sinks, recent=recent)
+    k_out = k.new_empty((B, budget, H, Dk)) if k_out is None else k_out
+    v_out = k.new_empty((B, budget, H, Dv)) if v_out is None else v_out
+    weights_out = k.new_empty((B, H, budget), dtype=torch.float32) if weights_out is None else weights_out
+    lens_out = k.new_empty((B,), dtype=torch.int32)
+    kept = k.new_empty((B, H, budget), dtype=torch.int32)
+    args = _pack(k, (B, 0, T, H, H, Dk, Dv), 1.0, sinks=sinks, budget=budget, recent=recent, k=_at(k), v=_at(v), kv_lens=lens,
+                 weights=_sums(weights, weights_out), cache=_at(k_out) + _at(v_out), new=(lens_out.data_ptr(), kept.data_ptr()))
+    _call(_lib.load().sdpa_dev_evict_cache, name, _OP_EVICT, k, args)
     return k_out, v_out, weights_out, lens_out, kept
