@@ -18,10 +18,11 @@ inline int heads_pad(int dk, int dv) {
 }
 inline int elem_bytes(int dtype) { return dtype == SDPA_BF16 ? 2 : 4; }
 
-// 16-byte accesses hold for a tensor whose base, strides and row length are multiples of 16 bytes
+// 16-byte accesses hold for a tensor whose base, strides and row length are multiples of 16 bytes (and whose tiles of up to 128
+// rows fit 32-bit offsets)
 inline bool rows_vec(const sdpa_tensor &t, int dim, int dtype) {
     const long e = elem_bytes(dtype), bad = (t.batch * e) | (t.token * e) | (t.head * e) | (dim * e);
-    return ((bad | (long)(size_t)t.data) & 15) == 0;
+    return ((bad | (long)(size_t)t.data) & 15) == 0 && t.token < (1 << 21);
 }
 
 // One launch over one set of keys: its queries, where its rows go, and what they may see.
@@ -36,7 +37,8 @@ struct AttendArgs {
     int window, sinks;
     int shared;                       // 1 = one set of keys for the whole batch, all of them visible (a prefix)
     int vec, vec_out;                 // 16-byte loads of q, k, v / whole 4-element stores of out
-    float scale_log2;                 // softmax scale * log2(e): scores are kept in the exp2 domain
+    int q_sign;                       // the softmax scale's sign: applied to the queries
+    float scale_log2;                 // its magnitude * log2(e) (1 for a scale of 0): scores are kept in the exp2 domain
 };
 
 struct BackwardArgs {

@@ -3,6 +3,7 @@
 #include "sdpa_heads.h"
 
 #include <limits.h>
+#include <math.h>
 #include <stdint.h>
 
 namespace {
@@ -68,7 +69,8 @@ AttendArgs attend_args(const sdpa_heads *a) {
     x.splits = 1;
     x.vec = rows_vec(a->q, a->dk, a->dtype) && rows_vec(a->k, a->dk, a->dtype) && rows_vec(a->v, a->dv, a->dtype);
     x.vec_out = rows_vec(a->out, a->dv, a->dtype);
-    x.scale_log2 = a->scale * 1.44269504088896341f;
+    x.q_sign = a->scale > 0.f ? 1 : a->scale < 0.f ? -1 : 0;
+    x.scale_log2 = a->scale == 0.f ? 1.f : fabsf(a->scale) * 1.44269504088896341f;
     return x;
 }
 

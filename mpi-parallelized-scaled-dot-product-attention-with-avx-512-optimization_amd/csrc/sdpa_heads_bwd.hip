@@ -51,8 +51,8 @@ template <typename T, int DP>
 __global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
     using TL = Tile<T, DP>;
     constexpr int BN = 32, STEPS = DP / Ops<T>::kStep;
-    __shared__ __attribute__((aligned(16))) char lk[BN * TL::kRowBytes];
-    __shared__ __attribute__((aligned(16))) char lv[BN * TL::kRowBytes];
+    __shared__ __attribute__((aligned(1024))) char lk[BN * TL::kRowBytes];
+    __shared__ __attribute__((aligned(1024))) char lv[BN * TL::kRowBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int id = xcd_place(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - id % tiles;
@@ -92,6 +92,9 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardAr
 #pragma unroll
         for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
 
+    LaneMap<T, DP> map;
+    map.init(lane);
+    const unsigned tk = lds_address(lk), ak = tk + map.rows, av = lds_address(lv) + map.rows;
     constexpr int PIECES = BN * TL::kChunks / kHeadsThreads;
     u32x4 rk[PIECES], rv[PIECES];
     const TileList list = tile_list(wg, a.sinks, BN);
@@ -123,9 +126,9 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardAr
         const bool full = j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks);
         f32x16 s = {}, dp = {};
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(lk, 0, i, lane), q[i], s);
+        for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(ak, 0, i), q[i], s);
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(lv, 0, i, lane), g[i], dp);
+        for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(av, 0, i), g[i], dp);
         uint32_t vis = 0xffffu;
         if (!full) {
             vis = 0;
@@ -140,7 +143,7 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardAr
             const float p = __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - lse2);
             s[i] = (vis >> i) & 1 ? p * (dp[i] - delta) : 0.f;
         }
-        mma_block<T, DP, DP / 32>(dq, lk, 0, to_probs(s, T()), !full, vis, 1, lane);
+        mma_block<T, DP, DP / 32>(dq, tk, map, 0, to_probs(s, T()), !full, vis, 1, lane);
     }
     if (r >= rows) return;
 #pragma unroll
@@ -176,8 +179,8 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardAr
     using TL = Tile<T, DP>;
     constexpr int BQ = 32, STEPS = DP / Ops<T>::kStep;
     constexpr bool DV = (WHAT & 1) != 0, DK = (WHAT & 2) != 0;
-    __shared__ __attribute__((aligned(16))) char lq[BQ * TL::kRowBytes];
-    __shared__ __attribute__((aligned(16))) char lg[BQ * TL::kRowBytes];
+    __shared__ __attribute__((aligned(1024))) char lq[BQ * TL::kRowBytes];
+    __shared__ __attribute__((aligned(1024))) char lg[BQ * TL::kRowBytes];
     __shared__ float llse[BQ], ldelta[BQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int id = xcd_place(blockIdx.x, gridDim.x);
@@ -223,6 +226,9 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardAr
             if (DV) dv[d][i] = 0.f;
         }
 
+    LaneMap<T, DP> map;
+    map.init(lane);
+    const unsigned tq = lds_address(lq), tg = lds_address(lg), aq = tq + map.rows, ag = tg + map.rows;
     constexpr int PIECES = BQ * TL::kChunks / kHeadsThreads;
     u32x4 rq[PIECES], rg[PIECES];
     float rl = 0.f, rd = 0.f;
@@ -261,7 +267,7 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardAr
         const bool full = r0 >= full_lo && r0 + BQ <= full_hi;
         f32x16 s = {};
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(lq, 0, i, lane), kf[i], s);
+        for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(aq, 0, i), kf[i], s);
         uint32_t vis = 0xffffu;
         if (!full) {
             vis = 0;
@@ -276,14 +282,14 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardAr
             const float p = __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - llse[row_of(i, lane >> 5)]);
             s[i] = (vis >> i) & 1 ? p : 0.f;
         }
-        if constexpr (DV) mma_block<T, DP, DP / 32>(dv, lg, 0, to_probs(s, T()), !full, vis, 1, lane);
+        if constexpr (DV) mma_block<T, DP, DP / 32>(dv, tg, map, 0, to_probs(s, T()), !full, vis, 1, lane);
         if constexpr (DK) {
             f32x16 dp = {};
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(lg, 0, i, lane), vf[i], dp);
+            for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(ag, 0, i), vf[i], dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = (vis >> i) & 1 ? s[i] * (dp[i] - ldelta[row_of(i, lane >> 5)]) : 0.f;
-            mma_block<T, DP, DP / 32>(dk, lq, 0, to_probs(s, T()), !full, vis, 1, lane);
+            mma_block<T, DP, DP / 32>(dk, tq, map, 0, to_probs(s, T()), !full, vis, 1, lane);
         }
     }
     if (j >= a.Tk) return;
@@ -346,7 +352,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(kHeadsThreads) void weights_kernel(WeightArgs a, int G, int blocks) {
     using TL = Tile<T, DP>;
     constexpr int BQ = 32, STEPS = DP / Ops<T>::kStep;
-    __shared__ __attribute__((aligned(16))) char lq[BQ * TL::kRowBytes];
+    __shared__ __attribute__((aligned(1024))) char lq[BQ * TL::kRowBytes];
     __shared__ float llse[BQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int id = xcd_place(blockIdx.x, gridDim.x);
@@ -362,6 +368,9 @@ __global__ __launch_bounds__(kHeadsThreads) void weights_kernel(WeightArgs a, in
         const int r_end = nq * G;
         typename Ops<T>::Frag kf[STEPS];
         load_row<T, DP>(kf, row_at(a.k, b, j, h, sizeof(T)), a.Dk, j < nk, a.vec, lane);
+        LaneMap<T, DP> map;
+        map.init(lane);
+        const unsigned aq = lds_address(lq) + map.rows;
         for (int r0 = first.lo / BQ * BQ; r0 < r_end; r0 += BQ) {
             __syncthreads();
             for (int c = tid; c < BQ * TL::kChunks; c += kHeadsThreads) {
@@ -380,7 +389,7 @@ __global__ __launch_bounds__(kHeadsThreads) void weights_kernel(WeightArgs a, in
             __syncthreads();
             f32x16 s = {};
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(lq, 0, i, lane), kf[i], s);
+            for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(aq, 0, i), kf[i], s);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int rl = row_of(i, lane >> 5), r = r0 + rl;

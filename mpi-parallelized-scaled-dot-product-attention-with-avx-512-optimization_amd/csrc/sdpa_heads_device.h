@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "sdpa_heads.h"
+#include "sdpa_internal.h"
 
 namespace sdpa {
 namespace heads {
@@ -27,6 +28,13 @@ constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 constexpr float kNegInf = -__builtin_inff();
 
 using LdsVec4 = __attribute__((address_space(3))) s16x4;
+
+// A copy the compiler knows nothing about: what is computed from it stays where it is used.  In the kernels' rarer branches, whose lane
+// arithmetic would otherwise be moved in front of the loops and hold the registers that the frequent branch needs.
+__device__ inline int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 __device__ inline int row_of(int i, int half) { return (i & 3) + 8 * (i >> 2) + 4 * half; }
 
@@ -87,9 +95,33 @@ template <typename T> __device__ inline u32x4 load_chunk(const T *row, int d0, i
     return r;
 }
 
-// A fragment (a lane's 16 bytes of step s of row lane & 31) of a tile's 32-row block
-template <typename T, int DP> __device__ inline typename Ops<T>::Frag read_rows(const char *tile, int block, int s, int lane) {
-    return *reinterpret_cast<const typename Ops<T>::Frag *>(tile + Tile<T, DP>::chunk(block * 32 + (lane & 31), 2 * s + (lane >> 5)));
+// Where a lane reads, as byte addresses inside a tile.  The swizzle is an XOR of the chunk number, so every read of a lane is ONE
+// base address, XORed with a constant (the step or column block: bits 4..7) plus a constant (the block: an immediate of the
+// instruction); tiles begin at multiples of 256 bytes.
+template <typename T, int DP> struct LaneMap {
+    using TL = Tile<T, DP>;
+    unsigned rows;                       // row-wise: row lane & 31, the lane half's chunk
+    unsigned cols;                       // transposed: rows 4 * half + sub (bf16) / 4 * half (fp32), the lane's columns
+    __device__ void init(int lane) {
+        const int half = lane >> 5, row = lane & 31;
+        rows = (unsigned)(row * TL::kRowBytes + ((half ^ TL::swz(row)) << 4));
+        if (sizeof(T) == 2) {
+            const int sub = (lane & 15) >> 2, c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), r = 4 * half + sub;
+            cols = (unsigned)(r * TL::kRowBytes + ((c ^ TL::swz(r)) << 4) + (lane & 1) * 8);
+        } else {
+            cols = (unsigned)(4 * half * TL::kRowBytes + ((((lane & 31) >> 2) ^ TL::swz(4 * half)) << 4) + (lane & 3) * 4);
+        }
+    }
+};
+template <typename V> __device__ inline V lds_read(unsigned at, int offset) {
+    return *(__attribute__((address_space(3))) const V *)((__attribute__((address_space(3))) const char *)(uintptr_t)at + offset);
+}
+
+// A fragment (a lane's 16 bytes of step s) of a tile's 32-row block; `at` = the tile's address + LaneMap::rows
+template <typename T, int DP> __device__ inline typename Ops<T>::Frag read_rows(unsigned at, int block, int s) {
+    using TL = Tile<T, DP>;
+    constexpr int M = TL::kChunks < 16 ? TL::kChunks - 1 : 15;
+    return lds_read<typename Ops<T>::Frag>(at ^ (unsigned)(((2 * s) & M) << 4), block * 32 * TL::kRowBytes + ((2 * s) & ~M) * 16);
 }
 
 // The transposed operand of a 32-row block: columns col0 .. col0 + 31, all 32 rows as the inner index.
@@ -97,26 +129,32 @@ template <typename T> struct Cols;                 // 32 rows of one column in p
 template <> struct Cols<__bf16> { bf16x8 f[2]; };
 template <> struct Cols<float> { float f[16]; };
 
-template <int DP> __device__ inline Cols<__bf16> read_cols(const char *tile, int block, int col0, int lane, __bf16) {
+// `at` = the tile's address + LaneMap::cols; column block d = columns 32 d .. 32 d + 31
+template <int DP> __device__ inline Cols<__bf16> read_cols(unsigned at, int block, int d, __bf16) {
+    using TL = Tile<__bf16, DP>;
     Cols<__bf16> r;
-    const int col = col0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3), half = lane >> 5, sub = (lane & 15) >> 2;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
         union { s16x4 h[2]; bf16x8 f; } x;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int row = block * 32 + 16 * ks + 8 * e + 4 * half + sub;
-            x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec4 *)(tile + Tile<__bf16, DP>::elem(row, col)));
+            // (rows 8 e further: bit 1 of the swizzle)
+            const unsigned p = at ^ (unsigned)((((4 * d) & 15) ^ (2 * e)) << 4);
+            const int offset = (block * 32 + 16 * ks + 8 * e) * TL::kRowBytes + ((4 * d) & ~15) * 16;
+            x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec4 *)((__attribute__((address_space(3))) char *)(uintptr_t)p + offset));
         }
         r.f[ks] = x.f;
     }
     return r;
 }
-template <int DP> __device__ inline Cols<float> read_cols(const char *tile, int block, int col0, int lane, float) {
+template <int DP> __device__ inline Cols<float> read_cols(unsigned at, int block, int d, float) {
+    using TL = Tile<float, DP>;
     Cols<float> r;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        r.f[i] = *reinterpret_cast<const float *>(tile + Tile<float, DP>::elem(block * 32 + row_of(i, lane >> 5), col0 + (lane & 31)));
+    for (int i = 0; i < 16; ++i) {
+        const int row = row_of(i, 0), c = 8 * d;
+        r.f[i] = lds_read<float>(at ^ (unsigned)((((c & 15) ^ TL::swz(row))) << 4), (block * 32 + row) * TL::kRowBytes + (c & ~15) * 16);
+    }
     return r;
 }
 
@@ -154,12 +192,12 @@ __device__ inline f32x16 mma_cols(const Cols<float> &a, const Probs<float> &b, f
 // operand is looked at first: values that are not finite leave the product (as zeros) and come back only for the columns that
 // see them, by a second product of 0/1 indicators.  `kinds`: 3 = NaN, +inf and -inf apart (weights are positive, so the sum's
 // sign is theirs), 1 = all of them as NaN (gradients, whose weights have either sign).
-template <typename T, int DP> __device__ inline bool block_not_finite(const char *tile, int block, int lane) {
-    const u32x4 *at = reinterpret_cast<const u32x4 *>(tile + block * 32 * Tile<T, DP>::kRowBytes) + lane;
+template <typename T, int DP> __device__ inline bool block_not_finite(unsigned tile, int block, int lane) {
+    const unsigned at = tile + (unsigned)(opaque(lane) * 16);
     uint32_t bad = 0;
 #pragma unroll 4
     for (int k = 0; k < 32 * Tile<T, DP>::kChunks / 64; ++k) {
-        const u32x4 w = at[k * 64];
+        const u32x4 w = lds_read<u32x4>(at + (unsigned)(k * 1024), block * 32 * Tile<T, DP>::kRowBytes);
 #pragma unroll
         for (int i = 0; i < 4; ++i)      // an exponent of all ones carries into the sign's place
             bad |= sizeof(T) == 2 ? ((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((w[i] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
@@ -210,20 +248,22 @@ __device__ inline f32x16 mma_cols_guarded(const Cols<T> &a, const Probs<T> &b, u
 
 // acc[d] += (columns d * 32 .. of the block)^T * P for every d < N; masked: the block holds masked pairs
 template <typename T, int DP, int N>
-__device__ inline void mma_block(f32x16 *acc, const char *tile, int block, const Probs<T> &p, bool masked, uint32_t seen,
-                                 int kinds, int lane) {
-    if (masked && block_not_finite<T, DP>(tile, block, lane)) {
+__device__ inline void mma_block(f32x16 *acc, unsigned tile, const LaneMap<T, DP> &map, int block, const Probs<T> &p, bool masked,
+                                 uint32_t seen, int kinds, int lane) {
+    if (masked && __builtin_expect(block_not_finite<T, DP>(tile, block, lane), 0)) {
         // (a rare path: one body for every d, the accumulators handed round, so that it costs the other path no registers)
 #pragma unroll 1
         for (int d = 0; d < N; ++d) {
-            const f32x16 t = mma_cols_guarded<T>(read_cols<DP>(tile, block, d * 32, lane, T()), p, seen, kinds, acc[0]);
+            const unsigned at = tile + (unsigned)opaque((int)map.cols);
+            const f32x16 t = mma_cols_guarded<T>(read_cols<DP>(at, block, d, T()), p, seen, kinds, acc[0]);
 #pragma unroll
             for (int e = 0; e + 1 < N; ++e) acc[e] = acc[e + 1];
             acc[N - 1] = t;
         }
     } else {
+        const unsigned at = tile + map.cols;
 #pragma unroll
-        for (int d = 0; d < N; ++d) acc[d] = mma_cols(read_cols<DP>(tile, block, d * 32, lane, T()), p, acc[d]);
+        for (int d = 0; d < N; ++d) acc[d] = mma_cols(read_cols<DP>(at, block, d, T()), p, acc[d]);
     }
 }
 
@@ -278,8 +318,96 @@ __device__ inline int xcd_place(int id, int n) {
     return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
 }
 
-__device__ inline float half_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
-__device__ inline float half_sum(float x) { return x + __shfl_xor(x, 32); }
+// a lane's value and the other half's at the same column
+__device__ inline float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float half_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- key / value tiles from memory to LDS ---------------------------------------------------------------------------------
+// One wave instruction moves 1 KiB (16 bytes a lane) straight to LDS, lane-linear at its LDS end; the tile's swizzle is made at
+// the memory end, by the order in which the lanes ask for their row's chunks.  A lane's offsets inside a tile are the same for
+// every tile, so that a tile costs a scalar base per tensor and no vector arithmetic.
+__device__ inline unsigned lds_address(const void *p) {
+    return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
+}
+template <typename P> __device__ inline P *uniform(P *p) {
+    const uint64_t x = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (P *)(((uint64_t)hi << 32) | lo);
+}
+__device__ inline void lds_dma(const char *base, unsigned lane_off, unsigned lds_byte) {
+    asm volatile("s_mov_b32 m0, %1\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %0, %2"
+                 :
+                 : "v"(lane_off), "s"(__builtin_amdgcn_readfirstlane(lds_byte)), "s"(uniform(base))
+                 : "memory" SDPA_M0_CLOBBER);
+}
+
+// A tile of ROWS rows staged by WAVES waves: keys [j0, j0 + ROWS) of one head.  Rows that no query of the workgroup sees are
+// never followed: a row of the tile that some query sees is read in their place (their weights are masked).
+template <typename T, int DP, int ROWS, int WAVES> struct Stager {
+    using TL = Tile<T, DP>;
+    static constexpr int kPieces = ROWS * TL::kRowBytes / 1024 / WAVES;       // 1 KiB pieces of a wave
+    const char *base;                // row 0 of the head
+    long token;                      // bytes between rows
+    int dim;
+    unsigned off[kPieces];           // lane offsets inside a tile
+    __device__ static int row(int wave, int lane, int k) { return (((wave * kPieces + k) * 1024 + lane * 16) / TL::kRowBytes); }
+    __device__ static int source(int wave, int lane, int k) {                 // the chunk of its row a lane asks for
+        return (((wave * kPieces + k) * 64 + lane) % TL::kChunks) ^ TL::swz(row(wave, lane, k));
+    }
+    __device__ void init(const void *p, long tok, int d, int wave, int lane) {
+        base = uniform((const char *)p);
+        token = tok * (long)sizeof(T);
+        dim = d;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) off[k] = (unsigned)(row(wave, lane, k) * (int)token) + 16u * (unsigned)source(wave, lane, k);
+    }
+    // the key read for tile row r
+    __device__ static int key(int r, int j0, const SeenRange &w, int sinks) {
+        int j = j0 + r;
+        if (j >= w.hi_max) j = w.hi_max - 1;
+        if (j < w.lo_min && j >= sinks) j = j0 < sinks ? j0 : w.lo_min;
+        return j;
+    }
+    // asynchronous: 16-byte rows (`token` < 2^31 / ROWS)
+    __device__ void dma(unsigned lds, int j0, const SeenRange &w, int sinks, int wave, int lane) const {
+        const char *at = base + (long)j0 * token;
+        const bool inside = j0 + ROWS <= w.hi_max && (j0 >= w.lo_min || j0 + ROWS <= sinks);
+        const bool whole = dim == DP;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            unsigned o = off[k];
+            if (!inside) {
+                const int r = row(wave, opaque(lane), k);
+                o += (unsigned)((key(r, j0, w, sinks) - j0 - r) * (int)token);
+            }
+            const unsigned dst = lds + (unsigned)(wave * kPieces + k) * 1024u;
+            if (whole) lds_dma(at, o, dst);
+            else if (source(wave, opaque(lane), k) * Ops<T>::kVec < dim) lds_dma(at, o, dst);      // (the padding stays zero)
+        }
+    }
+    // element by element, for rows without 16-byte alignment
+    __device__ void copy(char *tile, int j0, const SeenRange &w, int sinks, int wave, int lane) const {
+#pragma unroll 1
+        for (int k = 0; k < kPieces; ++k) {
+            const int ln = opaque(lane), r = row(wave, ln, k), c = source(wave, ln, k);
+            const T *src = reinterpret_cast<const T *>(base + (long)key(r, j0, w, sinks) * token);
+            *reinterpret_cast<u32x4 *>(tile + (wave * kPieces + k) * 1024 + lane * 16) = load_chunk(src, c * Ops<T>::kVec, dim, false);
+        }
+    }
+};
+// LDS tiles whose padding no DMA ever writes
+__device__ inline void zero_lds(char *p, int bytes, int threads) {
+    for (int i = threadIdx.x * 16; i < bytes; i += threads * 16) *reinterpret_cast<u32x4 *>(p + i) = u32x4{0, 0, 0, 0};
+}
+__device__ inline void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 }  // namespace heads
 }  // namespace sdpa

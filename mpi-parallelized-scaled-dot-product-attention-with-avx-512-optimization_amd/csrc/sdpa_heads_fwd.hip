@@ -37,44 +37,65 @@ template <int DP> struct State {
     }
 };
 
-// one 32-key block: scores, running statistics, O += V^T P.  `full`: every live row of the wave sees every key.
-template <typename T, int DP>
-__device__ inline void attend_block(State<DP> &st, const typename Ops<T>::Frag *q, const char *lk, const char *lv, int block,
-                                    int j0, bool full, Seen seen, int sinks, float scale_log2, int lane) {
+// NB blocks of 32 keys: scores, running statistics, O += V^T P.  MASKED: some row of the wave does not see some key.
+// The reference exponent follows the maximum only when that rose by more than 2^8: a weight is then at most 2^8 instead of 1,
+// which costs no precision (fp32 sums, and operand roundings are relative), and the 16 * DP / 32 multiplications of a rescale are
+// rare.  Scores are compared unscaled (the scale is positive: load_query) and scaled inside the exponential's argument.
+template <typename T, int DP, int NB, bool MASKED>
+__device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag *q, unsigned lk, unsigned lv, const LaneMap<T, DP> &map,
+                                     int j0, Seen seen, int sinks, float scale, int lane) {
     constexpr int STEPS = DP / Ops<T>::kStep;
-    f32x16 s = {};
+    const unsigned at = lk + map.rows;
+    f32x16 s[NB];
+    uint32_t vis[NB];
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(lk, block, i, lane), q[i], s);
-    uint32_t vis = 0xffffu;
+    for (int n = 0; n < NB; ++n) {
+        s[n] = f32x16{};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] *= scale_log2;
-    if (!full) {
-        vis = 0;
+        for (int i = 0; i < STEPS; ++i) s[n] = Ops<T>::mma(read_rows<T, DP>(at, n, i), q[i], s[n]);
+    }
+    if (MASKED) {
+        const int half = opaque(lane) >> 5;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int j = j0 + row_of(i, lane >> 5);
-            const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
-            vis |= ok ? 1u << i : 0u;
-            s[i] = ok ? s[i] : kNegInf;
+        for (int n = 0; n < NB; ++n) {
+            vis[n] = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = j0 + n * 32 + row_of(i, half);
+                const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
+                vis[n] |= ok ? 1u << i : 0u;
+                s[n][i] = ok ? s[n][i] : kNegInf;
+            }
         }
     }
-    float mx = s[0];
+    float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    const float m = fmaxf(st.m, half_max(mx));
-    const float ref = m == kNegInf ? 0.f : m;          // (nothing seen yet: every weight is 2^-inf = 0)
-    const float alpha = __builtin_amdgcn_exp2f(st.m - ref);
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = n == 0 ? 1 : 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+    const float top = half_max(mx) * scale;
+    if (__any(top > st.m + 8.f)) {
+        const float m = fmaxf(st.m, top);
+        const float alpha = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+        st.m = m;
+        st.l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st.o[d][i] *= alpha;
+    }
+    const float ref = st.m == kNegInf ? 0.f : st.m;     // (nothing seen yet: every weight is 2^-inf = 0)
     float sum = 0.f;
+    Probs<T> p[NB];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - ref); sum += s[i]; }
-    st.l = st.l * alpha + sum;                          // (the two lane halves' sums are joined once, behind the loop)
-    st.m = m;
-    const Probs<T> p = to_probs(s, T());
+    for (int n = 0; n < NB; ++n) {
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+        for (int i = 0; i < 16; ++i) { s[n][i] = __builtin_amdgcn_exp2f(s[n][i] * scale - ref); sum += s[n][i]; }
+        p[n] = to_probs(s[n], T());
+    }
+    st.l += sum;                                        // (the two lane halves' sums are joined once, behind the loop)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st.o[d][i] *= alpha;
-    mma_block<T, DP, DP / 32>(st.o, lv, block, p, !full, vis, 3, lane);
+    for (int n = 0; n < NB; ++n) mma_block<T, DP, DP / 32>(st.o, lv, map, n, p[n], MASKED, MASKED ? vis[n] : 0u, 3, lane);
 }
 
 // a finished row (or its partial triple): 4 consecutive values of row `x`, columns d .. d + 3
@@ -112,25 +133,30 @@ __device__ inline void store_stat(const AttendArgs &a, const RowId &x, int hq, i
     else a.lse[((long)x.b * a.Hq + hq) * a.Tq + x.t] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
 }
 
+// A lane's column of Q.  The softmax scale is kept positive: a negative one turns the sign of the queries (exactly), and a scale of
+// zero is queries of zero.
 template <typename T, int DP>
 __device__ inline void load_query(typename Ops<T>::Frag *q, const AttendArgs &a, const RowId &x, int hq, int lane) {
     const T *row = (const T *)a.q.data + x.b * a.q.batch + x.t * a.q.token + hq * a.q.head;
+    const bool live = x.live && a.q_sign != 0;
+    const uint32_t turn = a.q_sign < 0 ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
 #pragma unroll
     for (int s = 0; s < DP / Ops<T>::kStep; ++s) {
         union { u32x4 u; typename Ops<T>::Frag f; } y;
         y.u = u32x4{0, 0, 0, 0};
-        if (x.live) y.u = load_chunk(row, s * Ops<T>::kStep + (lane >> 5) * Ops<T>::kVec, a.Dk, a.vec);
+        if (live) y.u = load_chunk(row, s * Ops<T>::kStep + (lane >> 5) * Ops<T>::kVec, a.Dk, a.vec) ^ turn;
         q[s] = y.f;
     }
 }
 
 // ---- many rows: 128 of them share every key tile, each wave owns 32 ---------------------------------------------------
-template <typename T, int DP, int BN>
-__global__ __launch_bounds__(kHeadsThreads) void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
+// Tiles are double-buffered in LDS: the next one is on its way while this one is multiplied, one barrier a tile.
+template <typename T, int DP, int BN, bool VEC>
+__global__ __launch_bounds__(kHeadsThreads, DP <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
     using TL = Tile<T, DP>;
-    __shared__ __attribute__((aligned(16))) char lk[BN * TL::kRowBytes];
-    __shared__ __attribute__((aligned(16))) char lv[BN * TL::kRowBytes];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int TILE = BN * TL::kRowBytes;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];            // K, V, K, V
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = xcd_place(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - id % tiles;             // (the rows that see most keys first)
     id /= tiles;
@@ -160,42 +186,39 @@ __global__ __launch_bounds__(kHeadsThreads) void attend_rows_kernel(AttendArgs a
     load_query<T, DP>(q, a, x, hq, lane);
     State<DP> st;
     st.clear();
+    LaneMap<T, DP> map;
+    map.init(lane);
 
-    constexpr int PIECES = BN * TL::kChunks / kHeadsThreads;
-    u32x4 rk[PIECES], rv[PIECES];
-    const T *kb = (const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head;
-    const T *vb = (const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head;
-    auto fetch = [&](int it) {
+    Stager<T, DP, BN, 4> sk, sv;
+    sk.init((const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head, a.k.token, a.Dk, wave, lane);
+    sv.init((const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head, a.v.token, a.Dv, wave, lane);
+    if (VEC && (a.Dk < DP || a.Dv < DP)) {
+        zero_lds(lds, 4 * TILE, kHeadsThreads);
+        __syncthreads();
+    }
+    const unsigned lds0 = lds_address(lds);
+    auto stage = [&](int it, int buf) {
         const int j0 = list.at(it) * BN;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = tid + k * kHeadsThreads, j = j0 + c / TL::kChunks, d = (c % TL::kChunks) * Ops<T>::kVec;
-            rk[k] = rv[k] = u32x4{0, 0, 0, 0};
-            if (j < wg.hi_max && (j >= wg.lo_min || j < a.sinks)) {      // (keys that no row sees are not read at all)
-                rk[k] = load_chunk(kb + (long)j * a.k.token, d, a.Dk, a.vec);
-                rv[k] = load_chunk(vb + (long)j * a.v.token, d, a.Dv, a.vec);
-            }
+        if (VEC) {
+            sk.dma(lds0 + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
+            sv.dma(lds0 + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
+        } else {
+            sk.copy(lds + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
+            sv.copy(lds + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
         }
     };
-    if (it0 < it1) fetch(it0);
-    for (int it = it0; it < it1; ++it) {
+    if (it0 < it1) stage(it0, 0);
+    for (int it = it0, buf = 0; it < it1; ++it, buf ^= 1) {
+        dma_wait();
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = tid + k * kHeadsThreads, at = TL::chunk(c / TL::kChunks, c % TL::kChunks);
-            *reinterpret_cast<u32x4 *>(lk + at) = rk[k];
-            *reinterpret_cast<u32x4 *>(lv + at) = rv[k];
-        }
-        __syncthreads();
-        const int t0 = list.at(it) * BN;
-        if (it + 1 < it1) fetch(it + 1);
-#pragma unroll
-        for (int kb2 = 0; kb2 < BN / 32; ++kb2) {
-            const int j0 = t0 + kb2 * 32, j1 = j0 + 32;
-            if (j0 >= wv.hi_max || (j1 <= wv.lo_min && j0 >= a.sinks)) continue;
-            const bool full = j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks);
-            attend_block<T, DP>(st, q, lk, lv, kb2, j0, full, seen, a.sinks, a.scale_log2, lane);
-        }
+        if (it + 1 < it1) stage(it + 1, buf ^ 1);
+        const int j0 = list.at(it) * BN, j1 = j0 + BN;
+        if (j0 >= wv.hi_max || (j1 <= wv.lo_min && j0 >= a.sinks)) continue;
+        const unsigned lk = lds0 + buf * 2 * TILE, lv = lk + TILE;
+        if (j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks))
+            attend_blocks<T, DP, BN / 32, false>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
+        else
+            attend_blocks<T, DP, BN / 32, true>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
     }
     st.l = half_sum(st.l);
     if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (blocks that need no mask gave weights to rows that do not exist)
@@ -226,7 +249,7 @@ template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, int rows, int G) {
     using TL = Tile<T, DP>;
     constexpr int WAVE_BYTES = 2 * 32 * TL::kRowBytes > 32 * DP * 4 ? 2 * 32 * TL::kRowBytes : 32 * DP * 4;
-    __shared__ __attribute__((aligned(16))) char lds[WAVES * WAVE_BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds[WAVES * WAVE_BYTES];
     __shared__ float lm[WAVES][32], ll[WAVES][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int id = xcd_place(blockIdx.x, gridDim.x);
@@ -253,8 +276,11 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
     load_query<T, DP>(q, a, x, hq, lane);
     State<DP> st;
     st.clear();
+    LaneMap<T, DP> map;
+    map.init(lane);
 
-    char *lk = lds + wave * WAVE_BYTES, *lv = lk + 32 * TL::kRowBytes;
+    char *wk = lds + wave * WAVE_BYTES, *wv = wk + 32 * TL::kRowBytes;
+    const unsigned lk = lds_address(wk), lv = lds_address(wv);
     const T *kb = (const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head;
     const T *vb = (const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head;
     constexpr int PIECES = 32 * TL::kChunks / 64;
@@ -269,12 +295,14 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
                 rv = load_chunk(vb + (long)j * a.v.token, d, a.Dv, a.vec);
             }
             const int at = TL::chunk(row, c % TL::kChunks);
-            *reinterpret_cast<u32x4 *>(lk + at) = rk;
-            *reinterpret_cast<u32x4 *>(lv + at) = rv;
+            *reinterpret_cast<u32x4 *>(wk + at) = rk;
+            *reinterpret_cast<u32x4 *>(wv + at) = rv;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (a wave reads only what it wrote itself)
-        const bool full = j1 <= wg.hi_min && (j0 >= wg.lo_max || j1 <= a.sinks);
-        attend_block<T, DP>(st, q, lk, lv, 0, j0, full, seen, a.sinks, a.scale_log2, lane);
+        if (j1 <= wg.hi_min && (j0 >= wg.lo_max || j1 <= a.sinks))
+            attend_blocks<T, DP, 1, false>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
+        else
+            attend_blocks<T, DP, 1, true>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     st.l = half_sum(st.l);
@@ -375,7 +403,9 @@ void attend(const AttendArgs &a, int rows, int G, int groups, hipStream_t s) {
         attend_few_kernel<T, DP, WAVES><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
     } else {
         const int tiles = (rows + 127) / 128;
-        attend_rows_kernel<T, DP, BN><<<groups * a.splits * tiles, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
+        const int grid = groups * a.splits * tiles;
+        if (a.vec) attend_rows_kernel<T, DP, BN, true><<<grid, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
+        else attend_rows_kernel<T, DP, BN, false><<<grid, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
     }
 }
 
