@@ -51,7 +51,7 @@ struct BackwardArgs {
     int window, sinks;
     int sink_blocks, sink_chunks;     // key blocks with sink keys, and the workgroups each of them has
     int rest_chunks;                  // workgroups of every other key block
-    int vec, vec_out;
+    int vec, vec_out, dma;            // 16-byte loads / stores; tiles by DMA
     float scale, scale_log2;
 };
 
@@ -82,11 +82,6 @@ hipError_t launch_attend_backward(const BackwardArgs &a, int dtype, hipStream_t 
 hipError_t launch_weights(const WeightArgs &a, int dtype, hipStream_t s);
 hipError_t launch_evict(const EvictArgs &a, hipStream_t s);
 
-// workgroups a launch over `rows` rows of every (sequence, key head) has before its keys are split
-inline int attend_row_tile(long rows) { return rows <= kFewRows ? kFewRows : 128; }
-inline int attend_key_tile(int dtype, int pad) { return pad * elem_bytes(dtype) <= 256 ? 64 : 32; }
-
-constexpr int kBwdKeys = 128;         // keys of a dK / dV workgroup (4 waves x 32)
-constexpr int kBwdRows = 128;         // rows of a dQ workgroup
+constexpr int kBwdKeys = 64;          // keys of a dK / dV workgroup
 
 }  // namespace sdpa

@@ -144,7 +144,7 @@ struct BackwardPlan { int sink_blocks, sink_chunks, rest_chunks; long delta, byt
 
 // The rows a key block walks: about (128 + window) tokens' heads, but every row for a block with sink keys -- those are cut to
 // the length of the others', so that no workgroup walks much longer than the rest; and all are cut further while the launch
-// has fewer workgroups than the chip has CUs.
+// has fewer than two workgroups a CU.
 BackwardPlan plan_backward(const sdpa_heads *a) {
     BackwardPlan p = {};
     const long G = a->q_heads / a->kv_heads, groups = (long)a->batch * a->kv_heads;
@@ -153,7 +153,7 @@ BackwardPlan plan_backward(const sdpa_heads *a) {
     const long w = (long)a->window + kBwdKeys < a->q_tokens ? (long)a->window + kBwdKeys : a->q_tokens;
     const long rest_tiles = ceil_div(w * G, 32), sink_tiles = ceil_div((long)a->q_tokens * G, 32);
     p.sink_blocks = (int)ceil_div(sinks, kBwdKeys);
-    long rest = groups * blocks < 256 ? ceil_div(256, groups * blocks < 1 ? 1 : groups * blocks) : 1;
+    long rest = groups * blocks < 512 ? ceil_div(512, groups * blocks < 1 ? 1 : groups * blocks) : 1;
     if (rest > ceil_div(rest_tiles, 8)) rest = ceil_div(rest_tiles, 8);
     if (rest > kMaxSplits) rest = kMaxSplits;
     if (rest < 1) rest = 1;
@@ -243,6 +243,9 @@ int sdpa_dev_attention_window_backward(const struct sdpa_heads *a, void *workspa
     x.sink_blocks = p.sink_blocks; x.sink_chunks = p.sink_chunks; x.rest_chunks = p.rest_chunks;
     x.vec = rows_vec(a->q, a->dk, a->dtype) && rows_vec(a->k, a->dk, a->dtype) && rows_vec(a->v, a->dv, a->dtype) &&
             rows_vec(a->out, a->dv, a->dtype) && rows_vec(a->dout, a->dv, a->dtype);
+    // a tile of 64 rows: two blocks of 32 / G tokens' heads, at 32-bit offsets
+    const long G = a->q_heads / a->kv_heads, e = elem_bytes(a->dtype);
+    x.dma = x.vec && G <= 32 && (G * a->q.head + 64 / G * a->q.token) * e < INT_MAX / 2 && (G * a->dout.head + 64 / G * a->dout.token) * e < INT_MAX / 2;
     x.vec_out = rows_vec(a->dq, a->dk, a->dtype) && rows_vec(a->dk_out, a->dk, a->dtype) && rows_vec(a->dv_out, a->dv, a->dtype);
     x.scale = a->scale;
     x.scale_log2 = a->scale * 1.44269504088896341f;

@@ -47,13 +47,40 @@ __device__ inline void load_row(typename Ops<T>::Frag *f, const void *row, int d
 }
 
 // ---- dQ: 128 rows to a workgroup, 32 to a wave -------------------------------------------------------------------------
-template <typename T, int DP>
-__global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
+// One 32-key block: S^T and dP^T with the keys as rows, dS^T kept in registers as the operand of dQ^T += K^T dS^T.
+template <typename T, int DP, bool MASKED>
+__device__ inline void grad_rows(f32x16 *dq, const typename Ops<T>::Frag *q, const typename Ops<T>::Frag *g, unsigned tk, unsigned tv,
+                                 const LaneMap<T, DP> &map, int j0, Seen seen, int sinks, float scale, float lse2, float delta, int lane) {
+    constexpr int STEPS = DP / Ops<T>::kStep;
+    f32x16 s = {}, dp = {};
+    const unsigned ak = tk + map.rows, av = tv + map.rows;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(ak, 0, i), q[i], s);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(av, 0, i), g[i], dp);
+    uint32_t vis = 0;
+    const int half = MASKED ? opaque(lane) >> 5 : 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[i] * scale - lse2);
+        s[i] = p * (dp[i] - delta);
+        if (MASKED) {
+            const int j = j0 + row_of(i, half);
+            const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
+            vis |= ok ? 1u << i : 0u;
+            s[i] = ok ? s[i] : 0.f;
+        }
+    }
+    mma_block<T, DP, DP / 32>(dq, tk, map, 0, to_probs(s, T()), MASKED, vis, 1, lane);
+}
+
+template <typename T, int DP, int BN, bool VEC>
+__global__ __launch_bounds__(kHeadsThreads, DP * (int)sizeof(T) <= 256 ? 2 : 1)
+void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
     using TL = Tile<T, DP>;
-    constexpr int BN = 32, STEPS = DP / Ops<T>::kStep;
-    __shared__ __attribute__((aligned(1024))) char lk[BN * TL::kRowBytes];
-    __shared__ __attribute__((aligned(1024))) char lv[BN * TL::kRowBytes];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int STEPS = DP / Ops<T>::kStep, TILE = BN * TL::kRowBytes;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];            // K, V, K, V
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = xcd_place(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - id % tiles;
     id /= tiles;
@@ -65,6 +92,26 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardAr
     const SeenRange wg = seen_range(r0 / G, min(r0 + 127, rows - 1) / G, nq, nk, a.window);
     const SeenRange wv = seen_range(rw / G, min(rw + 31, rows - 1) / G, nq, nk, a.window);
     const Seen seen = live ? seen_at(nk - nq + t, nk, a.window) : Seen{0, 0};
+    const TileList list = tile_list(wg, a.sinks, BN);
+    Stager<T, DP, BN, 4> sk, sv;
+    sk.init(row_at(a.k, b, 0, h, sizeof(T)), a.k.token, a.Dk, wave, lane);
+    sv.init(row_at(a.v, b, 0, h, sizeof(T)), a.v.token, a.Dv, wave, lane);
+    if (VEC && (a.Dk < DP || a.Dv < DP)) {
+        zero_lds(lds, 4 * TILE, kHeadsThreads);
+        __syncthreads();
+    }
+    const unsigned lds0 = lds_address(lds);
+    auto stage = [&](int it, int buf) {
+        const int j0 = list.at(it) * BN;
+        if (VEC) {
+            sk.dma(lds0 + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
+            sv.dma(lds0 + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
+        } else {
+            sk.copy(lds + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
+            sv.copy(lds + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
+        }
+    };
+    if (list.count > 0) stage(0, 0);
 
     typename Ops<T>::Frag q[STEPS], g[STEPS];
     load_row<T, DP>(q, row_at(a.q, b, t, hq, sizeof(T)), a.Dk, live, a.vec, lane);
@@ -91,59 +138,22 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardAr
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-
     LaneMap<T, DP> map;
     map.init(lane);
-    const unsigned tk = lds_address(lk), ak = tk + map.rows, av = lds_address(lv) + map.rows;
-    constexpr int PIECES = BN * TL::kChunks / kHeadsThreads;
-    u32x4 rk[PIECES], rv[PIECES];
-    const TileList list = tile_list(wg, a.sinks, BN);
-    auto fetch = [&](int it) {
-        const int j0 = list.at(it) * BN;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = tid + k * kHeadsThreads, j = j0 + c / TL::kChunks, d = (c % TL::kChunks) * Ops<T>::kVec;
-            rk[k] = rv[k] = u32x4{0, 0, 0, 0};
-            if (j < wg.hi_max && (j >= wg.lo_min || j < a.sinks)) {
-                rk[k] = load_chunk((const T *)row_at(a.k, b, j, h, sizeof(T)), d, a.Dk, a.vec);
-                rv[k] = load_chunk((const T *)row_at(a.v, b, j, h, sizeof(T)), d, a.Dv, a.vec);
-            }
-        }
-    };
-    if (list.count > 0) fetch(0);
-    for (int it = 0; it < list.count; ++it) {
+    for (int it = 0, buf = 0; it < list.count; ++it, buf ^= 1) {
+        dma_wait();
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = tid + k * kHeadsThreads, p = TL::chunk(c / TL::kChunks, c % TL::kChunks);
-            *reinterpret_cast<u32x4 *>(lk + p) = rk[k];
-            *reinterpret_cast<u32x4 *>(lv + p) = rv[k];
+        if (it + 1 < list.count) stage(it + 1, buf ^ 1);
+#pragma unroll 1
+        for (int n = 0; n < BN / 32; ++n) {
+            const int j0 = list.at(it) * BN + n * 32, j1 = j0 + 32;
+            if (j0 >= wv.hi_max || (j1 <= wv.lo_min && j0 >= a.sinks)) continue;
+            const unsigned tk = lds0 + buf * 2 * TILE + n * 32 * TL::kRowBytes, tv = tk + TILE;
+            if (j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks))
+                grad_rows<T, DP, false>(dq, q, g, tk, tv, map, j0, seen, a.sinks, a.scale_log2, lse2, delta, lane);
+            else
+                grad_rows<T, DP, true>(dq, q, g, tk, tv, map, j0, seen, a.sinks, a.scale_log2, lse2, delta, lane);
         }
-        __syncthreads();
-        const int j0 = list.at(it) * BN, j1 = j0 + BN;
-        if (it + 1 < list.count) fetch(it + 1);
-        if (j0 >= wv.hi_max || (j1 <= wv.lo_min && j0 >= a.sinks)) continue;
-        const bool full = j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks);
-        f32x16 s = {}, dp = {};
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(ak, 0, i), q[i], s);
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(av, 0, i), g[i], dp);
-        uint32_t vis = 0xffffu;
-        if (!full) {
-            vis = 0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = j0 + row_of(i, lane >> 5);
-                if (j < seen.hi && (j >= seen.lo || j < a.sinks)) vis |= 1u << i;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - lse2);
-            s[i] = (vis >> i) & 1 ? p * (dp[i] - delta) : 0.f;
-        }
-        mma_block<T, DP, DP / 32>(dq, tk, map, 0, to_probs(s, T()), !full, vis, 1, lane);
     }
     if (r >= rows) return;
 #pragma unroll
@@ -157,32 +167,142 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_rows_kernel(BackwardAr
         }
 }
 
-// which rows (tokens' grouped heads) a key is seen by: [lo, hi)
+// which queries see a key: tokens [lo, hi)
 struct SeenBy { int lo, hi; };
-__device__ inline SeenBy seen_by(int j, int nq, int nk, int G, int window, int sinks) {
+__device__ inline SeenBy seen_by(int j, int nq, int nk, int window, int sinks) {
     SeenBy s = {0, 0};
     if (j >= nk || nq <= 0) return s;
     const int p0 = nk - nq;                             // the first query's position (below 0: it has seen nothing yet)
     const int lo = j - p0 > 0 ? j - p0 : 0;
-    int hi = j < sinks || j - p0 + window > nq ? nq : j - p0 + window;
-    if (hi < lo || lo > nq) hi = 0;
-    if (hi == 0) return s;
-    s.lo = lo * G; s.hi = hi * G;
+    const int hi = j < sinks || j - p0 + window > nq ? nq : j - p0 + window;
+    if (hi <= lo) return s;
+    s.lo = lo; s.hi = hi;
     return s;
 }
 
-// ---- dK, dV: 128 keys to a workgroup, 32 to a wave ------------------------------------------------------------------------
-// WHAT: 3 = both; fp32 rows of 256 do them one after the other (1 = dV, 2 = dK): two accumulators and two operands of 256
-// columns do not fit the 512 registers of a lane.
-template <typename T, int DP, int WHAT>
-__global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardArgs a, int rows, int G, int items) {
+// The rows a key head's queries are walked in: blocks of 32, whole tokens' grouped heads to a block (the rows a block has left
+// over are zeros), or, for groups of more than 32 heads, blocks of one token.  So a row's place inside its block is the same in
+// every block, and a tile of blocks costs the DMA no vector arithmetic.
+struct RowBlocks {
+    int G, tokens, split;                               // tokens of a block, blocks of a token: one of them is 1
+    __device__ explicit RowBlocks(int g) : G(g), tokens(g <= 32 ? 32 / g : 1), split(g <= 32 ? 1 : (g + 31) / 32) {}
+    __device__ int row(int t) const { return (split > 1 ? t * split : t / tokens) * 32 + (split > 1 ? 0 : t % tokens * G); }
+    __device__ int token(int block, int i) const { return split > 1 ? block / split : block * tokens + i / G; }
+    __device__ int head(int block, int i) const { return split > 1 ? block % split * 32 + i : i % G; }
+    __device__ bool used(int block, int i) const { return split > 1 ? head(block, i) < G : i < tokens * G; }
+};
+
+// Tiles of two such blocks of one tensor, staged by four waves
+template <typename T, int DP> struct RowStager {
     using TL = Tile<T, DP>;
-    constexpr int BQ = 32, STEPS = DP / Ops<T>::kStep;
+    static constexpr int kPieces = 64 * TL::kRowBytes / 1024 / 4;
+    const char *base;
+    long token, head;
+    int dim;
+    unsigned off[kPieces];
+    __device__ static int row(int wave, int lane, int k) { return ((wave * kPieces + k) * 1024 + lane * 16) / TL::kRowBytes; }
+    __device__ static int source(int wave, int lane, int k) {
+        return (((wave * kPieces + k) * 64 + lane) % TL::kChunks) ^ TL::swz(row(wave, lane, k));
+    }
+    __device__ void init(const void *p, const sdpa_tensor &t, int d, const RowBlocks &rb, int wave, int lane) {
+        base = uniform((const char *)p);
+        token = t.token * (long)sizeof(T);
+        head = t.head * (long)sizeof(T);
+        dim = d;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const int r = row(wave, lane, k), i = r & 31;
+            off[k] = (unsigned)(((r >> 5) * rb.tokens + i / rb.G) * (int)token + i % rb.G * (int)head) + 16u * (unsigned)source(wave, lane, k);
+        }
+    }
+    // (groups of at most 32 heads) rows behind the last query are read as the last query's: their weights are masked
+    __device__ void dma(unsigned lds, int block, int nq, const RowBlocks &rb, int wave, int lane) const {
+        const int t0 = block * rb.tokens;
+        const char *at = base + (long)t0 * token;
+        const bool plain = dim == DP && rb.tokens * rb.G == 32, inside = t0 + 2 * rb.tokens <= nq;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            unsigned o = off[k];
+            const unsigned dst = lds + (unsigned)(wave * kPieces + k) * 1024u;
+            if (plain && inside) { lds_dma(at, o, dst); continue; }
+            const int ln = opaque(lane), r = row(wave, ln, k), i = r & 31, t = t0 + (r >> 5) * rb.tokens + i / rb.G;
+            if (t >= nq) o += (unsigned)((nq - 1 - t) * (int)token);
+            if (i < rb.tokens * rb.G && source(wave, ln, k) * Ops<T>::kVec < dim) lds_dma(at, o, dst);     // (the rest stays zero)
+        }
+    }
+    __device__ void copy(char *tile, int block, int nq, const RowBlocks &rb, bool vec, int wave, int lane) const {
+#pragma unroll 1
+        for (int k = 0; k < kPieces; ++k) {
+            const int ln = opaque(lane), r = row(wave, ln, k), blk = block + (r >> 5), i = r & 31, t = rb.token(blk, i);
+            u32x4 x = {0, 0, 0, 0};
+            if (t < nq && rb.used(blk, i))
+                x = load_chunk(reinterpret_cast<const T *>(base + t * token + rb.head(blk, i) * head), source(wave, ln, k) * Ops<T>::kVec, dim, vec);
+            *reinterpret_cast<u32x4 *>(tile + (wave * kPieces + k) * 1024 + ln * 16) = x;
+        }
+    }
+};
+
+// One block of 32 rows against a wave's 32 keys: P, dP, dS have the rows as rows and a key to a lane, and stay in registers as the
+// operands of dV^T += dO^T P and dK^T += Q^T dS.
+template <typename T, int DP, int WHAT, bool MASKED>
+__device__ inline void grad_keys(f32x16 *dk, f32x16 *dv, const typename Ops<T>::Frag *kf, const typename Ops<T>::Frag *vf, unsigned tq,
+                                 unsigned tg, const LaneMap<T, DP> &map, unsigned stats, int r0, SeenBy by, float scale, int lane) {
+    constexpr int STEPS = DP / Ops<T>::kStep;
+    const unsigned aq = tq + map.rows, ag = tg + map.rows, st = stats + (lane >> 5) * 16;
+    f32x16 s = {};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(aq, 0, i), kf[i], s);
+    uint32_t vis = 0;
+    const int half = MASKED ? opaque(lane) >> 5 : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x4 lse2 = lds_read<f32x4>(st, i * 32);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int x = 4 * i + k;
+            s[x] = __builtin_amdgcn_exp2f(s[x] * scale - lse2[k]);
+            if (MASKED) {
+                const int r = r0 + row_of(x, half);
+                const bool ok = r >= by.lo && r < by.hi;
+                vis |= ok ? 1u << x : 0u;
+                s[x] = ok ? s[x] : 0.f;
+            }
+        }
+    }
+    if constexpr ((WHAT & 1) != 0) mma_block<T, DP, DP / 32>(dv, tg, map, 0, to_probs(s, T()), MASKED, vis, 1, lane);
+    if constexpr ((WHAT & 2) != 0) {
+        f32x16 dp = {};
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(ag, 0, i), vf[i], dp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 delta = lds_read<f32x4>(st, 256 + i * 32);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int x = 4 * i + k;
+                const float ds = s[x] * (dp[x] - delta[k]);
+                s[x] = MASKED && !((vis >> x) & 1) ? 0.f : ds;
+            }
+        }
+        mma_block<T, DP, DP / 32>(dk, tq, map, 0, to_probs(s, T()), MASKED, vis, 1, lane);
+    }
+}
+
+// ---- dK, dV: 64 keys to a workgroup -----------------------------------------------------------------------------------------
+// Waves 0 and 1 take 32 keys each on the even row blocks, waves 2 and 3 the same keys on the odd ones; the two sums are added in LDS
+// at the end.  (Against four waves of 32 keys: twice the workgroups, so that two share a CU and one's exponentials run beside the
+// other's products, for a second reading of Q and dO out of L2.)
+// WHAT: 3 = both; heads of 256 do them one after the other (1 = dV, 2 = dK): two accumulators and two operands of 256 columns leave
+// no registers for the scores.
+template <typename T, int DP, int WHAT, bool VEC>
+__global__ __launch_bounds__(kHeadsThreads, DP * (int)sizeof(T) <= 128 ? 2 : 1)
+void backward_keys_kernel(BackwardArgs a, int G, int items) {
+    using TL = Tile<T, DP>;
+    constexpr int STEPS = DP / Ops<T>::kStep, TILE = 64 * TL::kRowBytes, NBUF = 4 * TILE <= 131072 ? 2 : 1;
     constexpr bool DV = (WHAT & 1) != 0, DK = (WHAT & 2) != 0;
-    __shared__ __attribute__((aligned(1024))) char lq[BQ * TL::kRowBytes];
-    __shared__ __attribute__((aligned(1024))) char lg[BQ * TL::kRowBytes];
-    __shared__ float llse[BQ], ldelta[BQ];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * TILE * NBUF];     // Q, dO, Q, dO
+    __shared__ __attribute__((aligned(16))) float lstat[2][2][64];            // [buffer][lse, delta][row]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = xcd_place(blockIdx.x, gridDim.x);
     const int item = id % items;
     id /= items;
@@ -192,27 +312,61 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardAr
     const int block = item < sink_items ? item / chunks : a.sink_blocks + (item - sink_items) / chunks;
     const int chunk = item < sink_items ? item % chunks : (item - sink_items) % chunks;
     const int nq = clamp_len(a.q_lens, b, a.Tq), nk = clamp_len(a.kv_lens, b, a.Tk);
-    const int k0 = block * kBwdKeys, kw = k0 + wave * 32, j = kw + (lane & 31);
-    const SeenBy by = seen_by(j, nq, nk, G, a.window, a.sinks);
-    // the rows that any of the workgroup's keys is seen by: contiguous, from the first key's first to the last key's last (or to
-    // the end, with a sink key among them)
+    const int k0 = block * kBwdKeys, kw = k0 + (wave & 1) * 32, phase = wave >> 1, j = kw + (lane & 31);
+    const RowBlocks rb(G);
+
+    // the tokens that see any of the workgroup's keys: contiguous, from the first key's first to the last key's last (or, with a sink key
+    // among them, to the end)
     const int klast = min(k0 + kBwdKeys, nk) - 1;
     SeenBy all = {0, 0};
-    if (k0 < nk) {
-        all = seen_by(k0, nq, nk, G, a.window, a.sinks);
-        const SeenBy last = seen_by(klast, nq, nk, G, a.window, a.sinks);
-        if (all.hi == 0) all.lo = max(0, k0 - (nk - nq)) * G;      // (the first keys may lie before every window)
-        all.hi = max(all.hi, last.hi);
-        if (k0 < a.sinks) all.hi = max(all.hi, seen_by(min(a.sinks - 1, klast), nq, nk, G, a.window, a.sinks).hi);
+    if (k0 < nk && nq > 0) {
+        const SeenBy first = seen_by(k0, nq, nk, a.window, a.sinks), last = seen_by(klast, nq, nk, a.window, a.sinks);
+        all.lo = max(0, k0 - (nk - nq));
+        all.hi = max(first.hi, last.hi);
     }
-    const int w_last = min(kw + 31, nk - 1);
+    const SeenBy tok = seen_by(j, nq, nk, a.window, a.sinks);
+    const SeenBy by = {rb.row(tok.lo), tok.hi > tok.lo ? rb.row(tok.hi) : 0};
     // rows that see every key of the wave: from the last key's first to the smallest end, which is the first key's that is no sink
-    const int f_first_key = kw < a.sinks ? min(a.sinks, w_last) : kw;
-    const SeenBy f_first = seen_by(f_first_key, nq, nk, G, a.window, a.sinks), f_last = seen_by(w_last, nq, nk, G, a.window, a.sinks);
-    const int full_lo = f_last.lo, full_hi = kw + 32 <= nk ? min(f_first.hi, f_last.hi) : 0;
-    const int n_tiles = all.hi > all.lo ? (all.hi - all.lo / BQ * BQ + BQ - 1) / BQ : 0;
-    const int first = all.lo / BQ;
-    const int it0 = (int)((long)n_tiles * chunk / chunks), it1 = (int)((long)n_tiles * (chunk + 1) / chunks);
+    SeenBy full = {0, 0};
+    if (kw + 32 <= nk) {
+        const SeenBy f = seen_by(kw < a.sinks ? min(a.sinks, kw + 31) : kw, nq, nk, a.window, a.sinks);
+        const SeenBy l = seen_by(kw + 31, nq, nk, a.window, a.sinks);
+        if (f.hi > 0 && l.hi > 0) full = SeenBy{rb.row(l.lo), rb.row(min(f.hi, l.hi))};
+    }
+    const int blk0 = rb.row(all.lo) / 64 * 2;            // row blocks come in pairs
+    const int pairs = all.hi > all.lo ? ((rb.row(all.hi) + 31) / 32 - blk0 + 1) / 2 : 0;
+    const int it0 = (int)((long)pairs * chunk / chunks), it1 = (int)((long)pairs * (chunk + 1) / chunks);
+
+    RowStager<T, DP> sq, sg;
+    sq.init(row_at(a.q, b, 0, h * G, sizeof(T)), a.q, a.Dk, rb, wave, lane);
+    sg.init(row_at(a.dout, b, 0, h * G, sizeof(T)), a.dout, a.Dv, rb, wave, lane);
+    if (VEC && (a.Dk < DP || a.Dv < DP || rb.tokens * G < 32)) {
+        zero_lds(lds, 2 * TILE * NBUF, kHeadsThreads);
+        __syncthreads();
+    }
+    const unsigned lds0 = lds_address(lds), stat0 = lds_address(&lstat[0][0][0]);
+    float rl = 0.f, rd = 0.f;
+    auto stage = [&](int it, int buf) {
+        const int blk = blk0 + 2 * it;
+        if (VEC) {
+            sq.dma(lds0 + buf * 2 * TILE, blk, nq, rb, wave, lane);
+            sg.dma(lds0 + buf * 2 * TILE + TILE, blk, nq, rb, wave, lane);
+        } else {
+            sq.copy(lds + buf * 2 * TILE, blk, nq, rb, a.vec, wave, lane);
+            sg.copy(lds + buf * 2 * TILE + TILE, blk, nq, rb, a.vec, wave, lane);
+        }
+        if (tid < 64) {                                  // a row that does not exist: weight 2^(0 - inf) = 0
+            const int i = tid & 31, bl = blk + (tid >> 5), t = rb.token(bl, i);
+            const bool live = t < nq && rb.used(bl, i);
+            const long at = ((long)b * a.Hq + h * G + rb.head(bl, i)) * a.Tq + t;
+            rl = live ? a.lse[at] * kLog2e : __builtin_inff();
+            rd = live ? a.delta[at] : 0.f;
+        }
+    };
+    auto put_stat = [&](int buf) {
+        if (tid < 64) { lstat[buf][0][tid] = rl; lstat[buf][1][tid] = rd; }
+    };
+    if (NBUF == 2 && it0 < it1) { stage(it0, 0); put_stat(0); }
 
     typename Ops<T>::Frag kf[STEPS], vf[DK ? STEPS : 1];
     load_row<T, DP>(kf, row_at(a.k, b, j, h, sizeof(T)), a.Dk, j < nk, a.vec, lane);
@@ -225,74 +379,50 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardAr
             if (DK) dk[d][i] = 0.f;
             if (DV) dv[d][i] = 0.f;
         }
-
     LaneMap<T, DP> map;
     map.init(lane);
-    const unsigned tq = lds_address(lq), tg = lds_address(lg), aq = tq + map.rows, ag = tg + map.rows;
-    constexpr int PIECES = BQ * TL::kChunks / kHeadsThreads;
-    u32x4 rq[PIECES], rg[PIECES];
-    float rl = 0.f, rd = 0.f;
-    auto fetch = [&](int it) {
-        const int r0 = (first + it) * BQ;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = tid + k * kHeadsThreads, r = r0 + c / TL::kChunks, d = (c % TL::kChunks) * Ops<T>::kVec;
-            rq[k] = rg[k] = u32x4{0, 0, 0, 0};
-            if (r < all.hi) {
-                const int t = r / G, hq = h * G + r - t * G;
-                rq[k] = load_chunk((const T *)row_at(a.q, b, t, hq, sizeof(T)), d, a.Dk, a.vec);
-                rg[k] = load_chunk((const T *)row_at(a.dout, b, t, hq, sizeof(T)), d, a.Dv, a.vec);
-            }
+    for (int it = it0, buf = 0; it < it1; ++it) {
+        if (NBUF == 1) {
+            __syncthreads();
+            stage(it, 0);
+            put_stat(0);
         }
-        if (tid < BQ && r0 + tid < all.hi) {
-            const int r = r0 + tid, t = r / G, hq = h * G + r - t * G;
-            const long at = ((long)b * a.Hq + hq) * a.Tq + t;
-            rl = a.lse[at] * kLog2e;
-            rd = a.delta[at];
-        }
-    };
-    if (it0 < it1) fetch(it0);
-    for (int it = it0; it < it1; ++it) {
+        dma_wait();
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = tid + k * kHeadsThreads, p = TL::chunk(c / TL::kChunks, c % TL::kChunks);
-            *reinterpret_cast<u32x4 *>(lq + p) = rq[k];
-            *reinterpret_cast<u32x4 *>(lg + p) = rg[k];
-        }
-        if (tid < BQ) { llse[tid] = rl; ldelta[tid] = rd; }
-        __syncthreads();
-        const int r0 = (first + it) * BQ;
-        if (it + 1 < it1) fetch(it + 1);
-        const bool full = r0 >= full_lo && r0 + BQ <= full_hi;
-        f32x16 s = {};
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(aq, 0, i), kf[i], s);
-        uint32_t vis = 0xffffu;
-        if (!full) {
-            vis = 0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int r = r0 + row_of(i, lane >> 5);
-                if (r >= by.lo && r < by.hi) vis |= 1u << i;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - llse[row_of(i, lane >> 5)]);
-            s[i] = (vis >> i) & 1 ? p : 0.f;
-        }
-        if constexpr (DV) mma_block<T, DP, DP / 32>(dv, tg, map, 0, to_probs(s, T()), !full, vis, 1, lane);
-        if constexpr (DK) {
-            f32x16 dp = {};
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(ag, 0, i), vf[i], dp);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = (vis >> i) & 1 ? s[i] * (dp[i] - ldelta[row_of(i, lane >> 5)]) : 0.f;
-            mma_block<T, DP, DP / 32>(dk, tq, map, 0, to_probs(s, T()), !full, vis, 1, lane);
+        if (NBUF == 2 && it + 1 < it1) stage(it + 1, buf ^ 1);
+        const int r0 = (blk0 + 2 * it + phase) * 32;
+        const unsigned tq = lds0 + buf * 2 * TILE + phase * 32 * TL::kRowBytes, tg = tq + TILE;
+        const unsigned stats = stat0 + buf * 512 + phase * 128;
+        if (r0 >= full.lo && r0 + 32 <= full.hi)
+            grad_keys<T, DP, WHAT, false>(dk, dv, kf, vf, tq, tg, map, stats, r0, by, a.scale_log2, lane);
+        else
+            grad_keys<T, DP, WHAT, true>(dk, dv, kf, vf, tq, tg, map, stats, r0, by, a.scale_log2, lane);
+        if (NBUF == 2) {
+            buf ^= 1;
+            if (it + 1 < it1) put_stat(buf);
         }
     }
-    if (j >= a.Tk) return;
+    // the odd blocks' sums join the even ones'
+    float *sum = reinterpret_cast<float *>(lds) + (wave & 1) * DP * 32 + lane;
+    auto join = [&](f32x16 *acc) {
+        __syncthreads();
+        if (phase == 1) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[(d * 16 + i) * 64] = acc[d][i];
+        }
+        __syncthreads();
+        if (phase == 0) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] += sum[(d * 16 + i) * 64];
+        }
+    };
+    if constexpr (DK) join(dk);
+    if constexpr (DV) join(dv);
+    if (phase == 1 || j >= a.Tk) return;
     float *part = nullptr;
     if (chunks > 1) {
         // partial rows lie item by item: first the sink blocks' (if they are shared), then the rest's
@@ -327,20 +457,22 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_keys_kernel(BackwardAr
         }
 }
 
-// the chunks of a key block become its gradient: a workgroup per key block, the chunks added in their order
+// the chunks of key blocks become their gradients, added in their order: four keys to a workgroup
 template <typename T>
 __global__ __launch_bounds__(kHeadsThreads) void backward_join_kernel(BackwardArgs a, int block0, int blocks, long item0, int chunks,
                                                                       long per) {
+    const int w = a.Dk + a.Dv;
     int id = blockIdx.x;
+    const int quad = id % (kBwdKeys / 4);
+    id /= kBwdKeys / 4;
     const int blk = id % blocks;
     id /= blocks;
-    const int h = id % a.Hkv, b = id / a.Hkv, k0 = (block0 + blk) * kBwdKeys, w = a.Dk + a.Dv;
-    const float *src = a.part + (((long)b * a.Hkv + h) * per + item0 + (long)blk * chunks) * kBwdKeys * w;
-    for (int i = threadIdx.x; i < kBwdKeys * w; i += kHeadsThreads) {
-        const int key = i / w, c = i - key * w, j = k0 + key;
-        if (j >= a.Tk) break;
+    const int h = id % a.Hkv, b = id / a.Hkv, key = quad * 4 + (threadIdx.x >> 6), j = (block0 + blk) * kBwdKeys + key;
+    if (j >= a.Tk) return;
+    const float *src = a.part + ((((long)b * a.Hkv + h) * per + item0 + (long)blk * chunks) * kBwdKeys + key) * w;
+    for (int c = threadIdx.x & 63; c < w; c += 64) {
         float sum = 0.f;
-        for (int x = 0; x < chunks; ++x) sum += src[(long)x * kBwdKeys * w + i];
+        for (int x = 0; x < chunks; ++x) sum += src[(long)x * kBwdKeys * w + c];
         T *row = c < a.Dk ? (T *)row_at(a.dk, b, j, h, sizeof(T)) + c : (T *)row_at(a.dv, b, j, h, sizeof(T)) + (c - a.Dk);
         *row = from_f32<T>(sum);
     }
@@ -356,22 +488,22 @@ __global__ __launch_bounds__(kHeadsThreads) void weights_kernel(WeightArgs a, in
     __shared__ float llse[BQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int id = xcd_place(blockIdx.x, gridDim.x);
-    const int k0 = (id % blocks) * kBwdKeys, kw = k0 + wave * 32, j = kw + (lane & 31);
+    const int k0 = (id % blocks) * 128, j = k0 + wave * 32 + (lane & 31);
     id /= blocks;
     const int h = id % a.Hkv, b = id / a.Hkv;
     const int nq = clamp_len(a.q_lens, b, a.Tq), nk = clamp_len(a.kv_lens, b, a.Tk);
     const int everything = 1 << 30;
-    const SeenBy by = seen_by(j, nq, nk, G, everything, 0);
+    const SeenBy tok = seen_by(j, nq, nk, everything, 0), by = {tok.lo * G, tok.hi * G};
     float sum = 0.f;
     if (k0 < nk) {
-        const SeenBy first = seen_by(k0, nq, nk, G, everything, 0);
+        const int first = max(0, k0 - (nk - nq)) * G;
         const int r_end = nq * G;
         typename Ops<T>::Frag kf[STEPS];
         load_row<T, DP>(kf, row_at(a.k, b, j, h, sizeof(T)), a.Dk, j < nk, a.vec, lane);
         LaneMap<T, DP> map;
         map.init(lane);
         const unsigned aq = lds_address(lq) + map.rows;
-        for (int r0 = first.lo / BQ * BQ; r0 < r_end; r0 += BQ) {
+        for (int r0 = first / BQ * BQ; r0 < r_end; r0 += BQ) {
             __syncthreads();
             for (int c = tid; c < BQ * TL::kChunks; c += kHeadsThreads) {
                 const int r = r0 + c / TL::kChunks;
@@ -404,30 +536,36 @@ __global__ __launch_bounds__(kHeadsThreads) void weights_kernel(WeightArgs a, in
     }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 void backward(const BackwardArgs &a, hipStream_t s) {
-    const int G = a.Hq / a.Hkv, rows = a.Tq * G, groups = a.B * a.Hkv;
-    const int tiles = (rows + kBwdRows - 1) / kBwdRows;
-    if (tiles > 0) backward_rows_kernel<T, DP><<<groups * tiles, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
+    constexpr int BN = DP * (int)sizeof(T) <= 256 ? 64 : 32;
+    const int G = a.Hq / a.Hkv, rows = a.Tq * G, groups = a.B * a.Hkv, tiles = (rows + 127) / 128;
+    if (tiles > 0) backward_rows_kernel<T, DP, BN, VEC><<<groups * tiles, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
     const int blocks = (a.Tk + kBwdKeys - 1) / kBwdKeys, rest = blocks - a.sink_blocks;
     const int sink_items = a.sink_blocks * a.sink_chunks, items = sink_items + rest * a.rest_chunks;
     if (items == 0) return;
-    if constexpr (DP * (int)sizeof(T) > 512) {
-        backward_keys_kernel<T, DP, 1><<<groups * items, kHeadsThreads, 0, s>>>(a, rows, G, items);
-        backward_keys_kernel<T, DP, 2><<<groups * items, kHeadsThreads, 0, s>>>(a, rows, G, items);
+    if constexpr (DP > 128) {
+        backward_keys_kernel<T, DP, 1, VEC><<<groups * items, kHeadsThreads, 0, s>>>(a, G, items);
+        backward_keys_kernel<T, DP, 2, VEC><<<groups * items, kHeadsThreads, 0, s>>>(a, G, items);
     } else {
-        backward_keys_kernel<T, DP, 3><<<groups * items, kHeadsThreads, 0, s>>>(a, rows, G, items);
+        backward_keys_kernel<T, DP, 3, VEC><<<groups * items, kHeadsThreads, 0, s>>>(a, G, items);
     }
     const long base = a.sink_chunks > 1 ? 0 : sink_items, per = items - base - (a.rest_chunks > 1 ? 0 : items - sink_items);
+    constexpr int quads = kBwdKeys / 4;
     if (a.sink_chunks > 1 && a.sink_blocks > 0)
-        backward_join_kernel<T><<<groups * a.sink_blocks, kHeadsThreads, 0, s>>>(a, 0, a.sink_blocks, 0, a.sink_chunks, per);
+        backward_join_kernel<T><<<groups * a.sink_blocks * quads, kHeadsThreads, 0, s>>>(a, 0, a.sink_blocks, 0, a.sink_chunks, per);
     if (a.rest_chunks > 1 && rest > 0)
-        backward_join_kernel<T><<<groups * rest, kHeadsThreads, 0, s>>>(a, a.sink_blocks, rest, sink_items - base, a.rest_chunks, per);
+        backward_join_kernel<T><<<groups * rest * quads, kHeadsThreads, 0, s>>>(a, a.sink_blocks, rest, sink_items - base, a.rest_chunks, per);
+}
+template <typename T, int DP>
+void backward(const BackwardArgs &a, hipStream_t s) {
+    if (a.dma) backward<T, DP, true>(a, s);
+    else backward<T, DP, false>(a, s);
 }
 
 template <typename T, int DP>
 void weights(const WeightArgs &a, hipStream_t s) {
-    const int blocks = (a.Tk + kBwdKeys - 1) / kBwdKeys;
+    const int blocks = (a.Tk + 127) / 128;
     if (blocks > 0) weights_kernel<T, DP><<<a.B * a.Hkv * blocks, kHeadsThreads, 0, s>>>(a, a.Hq / a.Hkv, blocks);
 }
 
