@@ -129,31 +129,42 @@ template <typename T> struct Cols;                 // 32 rows of one column in p
 template <> struct Cols<__bf16> { bf16x8 f[2]; };
 template <> struct Cols<float> { float f[16]; };
 
-// `at` = the tile's address + LaneMap::cols; column block d = columns 32 d .. 32 d + 31
-template <int DP> __device__ inline Cols<__bf16> read_cols(unsigned at, int block, int d, __bf16) {
+// `at` = the tile's address + LaneMap::cols; column block d = columns 32 d .. 32 d + 31.  In pieces of 16 bytes: bf16 the 16-row half
+// `part`, fp32 the rows row_of(4 part .. 4 part + 3).
+template <int DP> __device__ inline bf16x8 read_cols_part(unsigned at, int block, int d, int part, __bf16) {
     using TL = Tile<__bf16, DP>;
+    union { s16x4 h[2]; bf16x8 f; } x;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const unsigned p = at ^ (unsigned)((((4 * d) & 15) ^ (2 * e)) << 4);      // (rows 8 e further: bit 1 of the swizzle)
+        const int offset = (block * 32 + 16 * part + 8 * e) * TL::kRowBytes + ((4 * d) & ~15) * 16;
+        x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec4 *)((__attribute__((address_space(3))) char *)(uintptr_t)p + offset));
+    }
+    return x.f;
+}
+template <int DP> __device__ inline f32x4 read_cols_part(unsigned at, int block, int d, int part, float) {
+    using TL = Tile<float, DP>;
+    f32x4 f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = row_of(4 * part + i, 0), c = 8 * d;
+        f[i] = lds_read<float>(at ^ (unsigned)(((c & 15) ^ TL::swz(row)) << 4), (block * 32 + row) * TL::kRowBytes + (c & ~15) * 16);
+    }
+    return f;
+}
+template <int DP> __device__ inline Cols<__bf16> read_cols(unsigned at, int block, int d, __bf16) {
     Cols<__bf16> r;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-        union { s16x4 h[2]; bf16x8 f; } x;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            // (rows 8 e further: bit 1 of the swizzle)
-            const unsigned p = at ^ (unsigned)((((4 * d) & 15) ^ (2 * e)) << 4);
-            const int offset = (block * 32 + 16 * ks + 8 * e) * TL::kRowBytes + ((4 * d) & ~15) * 16;
-            x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec4 *)((__attribute__((address_space(3))) char *)(uintptr_t)p + offset));
-        }
-        r.f[ks] = x.f;
-    }
+    for (int k = 0; k < 2; ++k) r.f[k] = read_cols_part<DP>(at, block, d, k, __bf16());
     return r;
 }
 template <int DP> __device__ inline Cols<float> read_cols(unsigned at, int block, int d, float) {
-    using TL = Tile<float, DP>;
     Cols<float> r;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int row = row_of(i, 0), c = 8 * d;
-        r.f[i] = lds_read<float>(at ^ (unsigned)((((c & 15) ^ TL::swz(row))) << 4), (block * 32 + row) * TL::kRowBytes + (c & ~15) * 16);
+    for (int k = 0; k < 4; ++k) {
+        const f32x4 f = read_cols_part<DP>(at, block, d, k, float());
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.f[4 * k + i] = f[i];
     }
     return r;
 }
@@ -177,6 +188,19 @@ __device__ inline Probs<float> to_probs(const f32x16 &p, float) {
     return r;
 }
 
+// value i (bf16: and i - 1) takes its place
+__device__ inline void put_prob(Probs<__bf16> &p, const f32x16 &s, int i) {
+    p.f[i >> 3][(i & 7) - 1] = (__bf16)s[i - 1];
+    p.f[i >> 3][i & 7] = (__bf16)s[i];
+}
+__device__ inline void put_prob(Probs<float> &p, const f32x16 &s, int i) { p.f[i] = s[i]; }
+
+__device__ inline f32x16 mma_part(bf16x8 a, const Probs<__bf16> &b, int part, f32x16 c) { return Ops<__bf16>::mma(a, b.f[part], c); }
+__device__ inline f32x16 mma_part(f32x4 a, const Probs<float> &b, int part, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b.f[4 * part + i], c, 0, 0, 0);
+    return c;
+}
 __device__ inline f32x16 mma_cols(const Cols<__bf16> &a, const Probs<__bf16> &b, f32x16 c) {
     c = Ops<__bf16>::mma(a.f[0], b.f[0], c);
     return Ops<__bf16>::mma(a.f[1], b.f[1], c);
@@ -246,20 +270,29 @@ __device__ inline f32x16 mma_cols_guarded(const Cols<T> &a, const Probs<T> &b, u
     return c;
 }
 
-// acc[d] += (columns d * 32 .. of the block)^T * P for every d < N; masked: the block holds masked pairs
+// acc[d] += (columns d * 32 .. of the block)^T * P for every d < N, where the block holds values that are not finite.
+// (A rare path: one body for every d, the accumulators handed round, so that it costs the frequent path no registers.)
+template <typename T, int DP, int N>
+__device__ inline void mma_block_guarded(f32x16 *acc, unsigned tile, const LaneMap<T, DP> &map, int block, const Probs<T> &p,
+                                         uint32_t seen, int kinds) {
+#pragma unroll 1
+    for (int d = 0; d < N; ++d) {
+        // (the column block as a run-time number: its place is the XOR and the offset of read_cols at d = 0)
+        const int c = d * 32 * (int)sizeof(T) / 16;
+        const unsigned at = (tile + (unsigned)opaque((int)map.cols)) ^ (unsigned)((c & 15) << 4);
+        const f32x16 t = mma_cols_guarded<T>(read_cols<DP>(at + (unsigned)((c & ~15) * 16), block, 0, T()), p, seen, kinds, acc[0]);
+#pragma unroll
+        for (int e = 0; e + 1 < N; ++e) acc[e] = acc[e + 1];
+        acc[N - 1] = t;
+    }
+}
+
+// the same, masked: the block holds masked pairs
 template <typename T, int DP, int N>
 __device__ inline void mma_block(f32x16 *acc, unsigned tile, const LaneMap<T, DP> &map, int block, const Probs<T> &p, bool masked,
                                  uint32_t seen, int kinds, int lane) {
     if (masked && __builtin_expect(block_not_finite<T, DP>(tile, block, lane), 0)) {
-        // (a rare path: one body for every d, the accumulators handed round, so that it costs the other path no registers)
-#pragma unroll 1
-        for (int d = 0; d < N; ++d) {
-            const unsigned at = tile + (unsigned)opaque((int)map.cols);
-            const f32x16 t = mma_cols_guarded<T>(read_cols<DP>(at, block, d, T()), p, seen, kinds, acc[0]);
-#pragma unroll
-            for (int e = 0; e + 1 < N; ++e) acc[e] = acc[e + 1];
-            acc[N - 1] = t;
-        }
+        mma_block_guarded<T, DP, N>(acc, tile, map, block, p, seen, kinds);
     } else {
         const unsigned at = tile + map.cols;
 #pragma unroll

@@ -37,42 +37,49 @@ template <int DP> struct State {
     }
 };
 
-// NB blocks of 32 keys: scores, running statistics, O += V^T P.  MASKED: some row of the wave does not see some key.
-// The reference exponent follows the maximum only when that rose by more than 2^8: a weight is then at most 2^8 instead of 1,
-// which costs no precision (fp32 sums, and operand roundings are relative), and the 16 * DP / 32 multiplications of a rescale are
-// rare.  Scores are compared unscaled (the scale is positive: load_query) and scaled inside the exponential's argument.
-template <typename T, int DP, int NB, bool MASKED>
-__device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag *q, unsigned lk, unsigned lv, const LaneMap<T, DP> &map,
-                                     int j0, Seen seen, int sinks, float scale, int lane) {
-    constexpr int STEPS = DP / Ops<T>::kStep;
+// ---- one tile of NB blocks of 32 keys against a wave's 32 rows, in three parts that a pipeline can take apart ------------------
+
+// raw scores S^T = K Q^T
+template <typename T, int DP, int NB>
+__device__ inline void scores(f32x16 *s, const typename Ops<T>::Frag *q, unsigned lk, const LaneMap<T, DP> &map) {
     const unsigned at = lk + map.rows;
-    f32x16 s[NB];
-    uint32_t vis[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         s[n] = f32x16{};
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) s[n] = Ops<T>::mma(read_rows<T, DP>(at, n, i), q[i], s[n]);
+        for (int i = 0; i < DP / Ops<T>::kStep; ++i) s[n] = Ops<T>::mma(read_rows<T, DP>(at, n, i), q[i], s[n]);
     }
-    if (MASKED) {
-        const int half = opaque(lane) >> 5;
+}
+
+// what a lane's column does not see becomes -inf; vis[n] = what it sees
+template <int NB> __device__ inline void hide(f32x16 *s, uint32_t *vis, int j0, Seen seen, int sinks, int lane) {
+    const int half = opaque(lane) >> 5;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            vis[n] = 0;
+    for (int n = 0; n < NB; ++n) {
+        vis[n] = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = j0 + n * 32 + row_of(i, half);
-                const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
-                vis[n] |= ok ? 1u << i : 0u;
-                s[n][i] = ok ? s[n][i] : kNegInf;
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int j = j0 + n * 32 + row_of(i, half);
+            const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
+            vis[n] |= ok ? 1u << i : 0u;
+            s[n][i] = ok ? s[n][i] : kNegInf;
         }
     }
+}
+
+// The reference exponent follows the maximum only when that rose by more than 2^8: a weight is then at most 2^8 instead of 1,
+// which costs no precision (fp32 sums, and operand roundings are relative), and the 16 * DP / 32 multiplications of a rescale are
+// rare.  Scores are compared unscaled (the scale is positive: load_query) and scaled inside the exponential's argument.
+// -> the exponent the tile's weights refer to
+template <int NB> __device__ inline float largest(const f32x16 *s) {
     float mx = s[0][0];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int i = n == 0 ? 1 : 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+    return mx;
+}
+template <int DP> __device__ inline float raise(State<DP> &st, float mx, float scale) {
     const float top = half_max(mx) * scale;
     if (__any(top > st.m + 8.f)) {
         const float m = fmaxf(st.m, top);
@@ -84,16 +91,32 @@ __device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag 
 #pragma unroll
             for (int i = 0; i < 16; ++i) st.o[d][i] *= alpha;
     }
-    const float ref = st.m == kNegInf ? 0.f : st.m;     // (nothing seen yet: every weight is 2^-inf = 0)
+    return st.m == kNegInf ? 0.f : st.m;                // (nothing seen yet: every weight is 2^-inf = 0)
+}
+
+// weights and their sum (the two lane halves' sums are joined once, behind the loop)
+template <typename T, int DP, int NB>
+__device__ inline void weigh(State<DP> &st, f32x16 *s, Probs<T> *p, float ref, float scale) {
     float sum = 0.f;
-    Probs<T> p[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) { s[n][i] = __builtin_amdgcn_exp2f(s[n][i] * scale - ref); sum += s[n][i]; }
         p[n] = to_probs(s[n], T());
     }
-    st.l += sum;                                        // (the two lane halves' sums are joined once, behind the loop)
+    st.l += sum;
+}
+
+template <typename T, int DP, int NB, bool MASKED>
+__device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag *q, unsigned lk, unsigned lv, const LaneMap<T, DP> &map,
+                                     int j0, Seen seen, int sinks, float scale, int lane) {
+    f32x16 s[NB];
+    uint32_t vis[NB];
+    scores<T, DP, NB>(s, q, lk, map);
+    if (MASKED) hide<NB>(s, vis, j0, seen, sinks, lane);
+    const float ref = raise<DP>(st, largest<NB>(s), scale);
+    Probs<T> p[NB];
+    weigh<T, DP, NB>(st, s, p, ref, scale);
 #pragma unroll
     for (int n = 0; n < NB; ++n) mma_block<T, DP, DP / 32>(st.o, lv, map, n, p[n], MASKED, MASKED ? vis[n] : 0u, 3, lane);
 }
@@ -149,13 +172,70 @@ __device__ inline void load_query(typename Ops<T>::Frag *q, const AttendArgs &a,
     }
 }
 
-// ---- many rows: 128 of them share every key tile, each wave owns 32 ---------------------------------------------------
-// Tiles are double-buffered in LDS: the next one is on its way while this one is multiplied, one barrier a tile.
+// ---- the steady state: scores of the next tile beside the weights of this one ---------------------------------------------------
+// The tile's products are a list of units -- for each 32-key block the K units (a step of the next tile's scores), then the V units
+// (a piece of O += V^T P) -- and a unit is written down as it is to be issued: the LDS read of the unit three ahead, this unit's
+// matrix instructions, and a few of the vector instructions that are due.  hipcc left alone puts all exponentials first and every
+// read right in front of its use (5000 cycles a tile and wave of 64 keys and 128 columns, against 1024 of its matrix instructions).
+template <typename T, int DP, int NB> struct Pipe {
+    static constexpr int KU = DP / Ops<T>::kStep, VK = sizeof(T) == 2 ? 2 : 4, VU = DP / 32 * VK, PER = KU + VU, UNITS = NB * PER, AHEAD = 3;
+    using Frag = typename Ops<T>::Frag;
+    __device__ static Frag fetch(int u, unsigned ak, unsigned av) {
+        const int n = u / PER, x = u % PER;
+        if (x < KU) return read_rows<T, DP>(ak, n, x);
+        return read_cols_part<DP>(av, n, (x - KU) / VK, (x - KU) % VK, T());
+    }
+    // -> the maximum of the next tile's scores in s2
+    __device__ static float run(State<DP> &st, const Frag *q, f32x16 *s, f32x16 *s2, unsigned ak, unsigned av, float ref, float scale) {
+        Frag ring[AHEAD + 1];
+        Probs<T> p[NB];
+        float sum = 0.f, mx = kNegInf;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s2[n] = f32x16{};
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) ring[u] = fetch(u, ak, av);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const int n = u / PER, x = u % PER;
+            if (u + AHEAD < UNITS) ring[(u + AHEAD) % (AHEAD + 1)] = fetch(u + AHEAD, ak, av);
+            const Frag f = ring[u % (AHEAD + 1)];
+            if (x < KU) s2[n] = Ops<T>::mma(f, q[x], s2[n]);
+            else st.o[(x - KU) / VK] = mma_part(f, p[n], (x - KU) % VK, st.o[(x - KU) / VK]);
+            // weights: block 0's beside its K units, block n's between the V units of block n - 1 and its own
+#pragma unroll
+            for (int m = 0; m < NB; ++m) {
+                const int first = m == 0 ? 0 : (m - 1) * PER + KU, count = m == 0 ? KU : PER;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (first + i * count / 16 == u) {
+                        s[m][i] = __builtin_amdgcn_exp2f(s[m][i] * scale - ref);
+                        sum += s[m][i];
+                        if (sizeof(T) == 4 || (i & 1)) put_prob(p[m], s[m], i);
+                    }
+            }
+            // the next tile's maximum, beside the last V units
+            if (u >= UNITS - VU) {
+#pragma unroll
+                for (int i = 0; i < 16 * NB; ++i)
+                    if (i * VU / (16 * NB) == u - (UNITS - VU)) mx = fmaxf(mx, s2[i / 16][i % 16]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        st.l += sum;
+        return mx;
+    }
+};
+
+// ---- many rows: a workgroup's four waves share every key tile, each owns 32 rows -------------------------------------------------
+// The loop is a pipeline over the tiles.  LDS holds two K tiles and two V tiles; K runs one tile ahead of V, the DMA one ahead of both,
+// one barrier a tile.
 template <typename T, int DP, int BN, bool VEC>
-__global__ __launch_bounds__(kHeadsThreads, DP <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
+__global__ __launch_bounds__(kHeadsThreads, DP <= 128 ? 2 : 1)
+void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
     using TL = Tile<T, DP>;
-    constexpr int TILE = BN * TL::kRowBytes;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];            // K, V, K, V
+    constexpr int TILE = BN * TL::kRowBytes, NB = BN / 32, STEPS = DP / Ops<T>::kStep;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];            // K, K, V, V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = xcd_place(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - id % tiles;             // (the rows that see most keys first)
@@ -181,14 +261,6 @@ __global__ __launch_bounds__(kHeadsThreads, DP <= 128 ? 2 : 1) void attend_rows_
     }
     const TileList list = tile_list(wg, a.sinks, BN);
     const int it0 = (int)((long)list.count * split / a.splits), it1 = (int)((long)list.count * (split + 1) / a.splits);
-
-    typename Ops<T>::Frag q[DP / Ops<T>::kStep];
-    load_query<T, DP>(q, a, x, hq, lane);
-    State<DP> st;
-    st.clear();
-    LaneMap<T, DP> map;
-    map.init(lane);
-
     Stager<T, DP, BN, 4> sk, sv;
     sk.init((const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head, a.k.token, a.Dk, wave, lane);
     sv.init((const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head, a.v.token, a.Dv, wave, lane);
@@ -197,31 +269,91 @@ __global__ __launch_bounds__(kHeadsThreads, DP <= 128 ? 2 : 1) void attend_rows_
         __syncthreads();
     }
     const unsigned lds0 = lds_address(lds);
-    auto stage = [&](int it, int buf) {
-        const int j0 = list.at(it) * BN;
-        if (VEC) {
-            sk.dma(lds0 + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
-            sv.dma(lds0 + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
-        } else {
-            sk.copy(lds + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
-            sv.copy(lds + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
-        }
+    auto stage_k = [&](int it) {
+        if (it >= it1) return;
+        const int j0 = list.at(it) * BN, buf = (it - it0) & 1;
+        if (VEC) sk.dma(lds0 + buf * TILE, j0, wg, a.sinks, wave, lane);
+        else sk.copy(lds + buf * TILE, j0, wg, a.sinks, wave, lane);
     };
-    if (it0 < it1) stage(it0, 0);
-    for (int it = it0, buf = 0; it < it1; ++it, buf ^= 1) {
+    auto stage_v = [&](int it) {
+        if (it >= it1) return;
+        const int j0 = list.at(it) * BN, buf = (it - it0) & 1;
+        if (VEC) sv.dma(lds0 + (2 + buf) * TILE, j0, wg, a.sinks, wave, lane);
+        else sv.copy(lds + (2 + buf) * TILE, j0, wg, a.sinks, wave, lane);
+    };
+    stage_k(it0);
+
+    typename Ops<T>::Frag q[STEPS];
+    load_query<T, DP>(q, a, x, hq, lane);
+    State<DP> st;
+    st.clear();
+    LaneMap<T, DP> map;
+    map.init(lane);
+    // does the wave see the tile at all / every key of it with every row
+    auto sees = [&](int it) {
+        const int j0 = list.at(it) * BN;
+        return j0 < wv.hi_max && (j0 + BN > wv.lo_min || j0 < a.sinks);
+    };
+    f32x16 s[NB];
+    float mx = kNegInf;
+    bool cur = false;
+    if (it0 < it1) {
         dma_wait();
         __syncthreads();
-        if (it + 1 < it1) stage(it + 1, buf ^ 1);
-        const int j0 = list.at(it) * BN, j1 = j0 + BN;
-        if (j0 >= wv.hi_max || (j1 <= wv.lo_min && j0 >= a.sinks)) continue;
-        const unsigned lk = lds0 + buf * 2 * TILE, lv = lk + TILE;
-        if (j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks))
-            attend_blocks<T, DP, BN / 32, false>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
-        else
-            attend_blocks<T, DP, BN / 32, true>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
+        stage_k(it0 + 1);
+        stage_v(it0);
+        cur = sees(it0);
+        if (cur) {
+            scores<T, DP, NB>(s, q, lds0, map);
+            mx = largest<NB>(s);
+        }
+    }
+    for (int it = it0; it < it1; ++it) {
+        const int buf = (it - it0) & 1;
+        dma_wait();
+        __syncthreads();
+        stage_k(it + 2);
+        stage_v(it + 1);
+        const unsigned lk = lds0 + (buf ^ 1) * TILE, lv = lds0 + (2 + buf) * TILE;
+        const bool next = it + 1 < it1 && sees(it + 1), had = cur;
+        cur = next;
+        if (!had) {
+            if (next) {
+                scores<T, DP, NB>(s, q, lk, map);
+                mx = largest<NB>(s);
+            }
+            continue;
+        }
+        const int j0 = list.at(it) * BN;
+        if (j0 + BN > wv.hi_min || (j0 < wv.lo_max && j0 + BN > a.sinks)) {          // some row does not see some key
+            uint32_t vis[NB];
+            hide<NB>(s, vis, j0, seen, a.sinks, lane);
+            mx = largest<NB>(s);
+            bool odd = false;
+#pragma unroll 1
+            for (int n = 0; n < NB; ++n) odd = odd || block_not_finite<T, DP>(lv, n, lane);
+            if (__builtin_expect(odd, 0)) {
+                const float ref = raise<DP>(st, mx, a.scale_log2);
+                Probs<T> p[NB];
+                weigh<T, DP, NB>(st, s, p, ref, a.scale_log2);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) mma_block_guarded<T, DP, DP / 32>(st.o, lv, map, n, p[n], vis[n], 3);
+                if (next) {
+                    scores<T, DP, NB>(s, q, lk, map);
+                    mx = largest<NB>(s);
+                }
+                continue;
+            }
+        }
+        const float ref = raise<DP>(st, mx, a.scale_log2);
+        // (behind the last tile the scores of a stale tile are multiplied and dropped)
+        f32x16 s2[NB];
+        mx = Pipe<T, DP, NB>::run(st, q, s, s2, lk + map.rows, lv + map.cols, ref, a.scale_log2);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n] = s2[n];
     }
     st.l = half_sum(st.l);
-    if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (blocks that need no mask gave weights to rows that do not exist)
+    if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (tiles that need no mask gave weights to rows that do not exist)
     if (rw + (lane & 31) >= rows) return;
     const int slot = a.slot0 + split;
     if (lane < 32) store_stat(a, x, hq, slot, st.m, st.l);
@@ -402,8 +534,7 @@ void attend(const AttendArgs &a, int rows, int G, int groups, hipStream_t s) {
         constexpr int WAVES = DP * (int)sizeof(T) > 512 ? 2 : 4;
         attend_few_kernel<T, DP, WAVES><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
     } else {
-        const int tiles = (rows + 127) / 128;
-        const int grid = groups * a.splits * tiles;
+        const int tiles = (rows + 127) / 128, grid = groups * a.splits * tiles;
         if (a.vec) attend_rows_kernel<T, DP, BN, true><<<grid, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
         else attend_rows_kernel<T, DP, BN, false><<<grid, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
     }
