@@ -92,7 +92,8 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
     const SeenRange wg = seen_range(r0 / G, min(r0 + 127, rows - 1) / G, nq, nk, a.window);
     const SeenRange wv = seen_range(rw / G, min(rw + 31, rows - 1) / G, nq, nk, a.window);
     const Seen seen = live ? seen_at(nk - nq + t, nk, a.window) : Seen{0, 0};
-    const TileList list = tile_list(wg, a.sinks, BN);
+    const KeyList list = key_list(wg, a.sinks);
+    const int count = list.tiles(BN);
     Stager<T, DP, BN, 4> sk, sv;
     sk.init(row_at(a.k, b, 0, h, sizeof(T)), a.k.token, a.Dk, wave, lane);
     sv.init(row_at(a.v, b, 0, h, sizeof(T)), a.v.token, a.Dv, wave, lane);
@@ -102,16 +103,15 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
     }
     const unsigned lds0 = lds_address(lds);
     auto stage = [&](int it, int buf) {
-        const int j0 = list.at(it) * BN;
         if (VEC) {
-            sk.dma(lds0 + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
-            sv.dma(lds0 + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
+            sk.dma(lds0 + buf * 2 * TILE, it * BN, list, wave, lane);
+            sv.dma(lds0 + buf * 2 * TILE + TILE, it * BN, list, wave, lane);
         } else {
-            sk.copy(lds + buf * 2 * TILE, j0, wg, a.sinks, wave, lane);
-            sv.copy(lds + buf * 2 * TILE + TILE, j0, wg, a.sinks, wave, lane);
+            sk.copy(lds + buf * 2 * TILE, it * BN, list, wave, lane);
+            sv.copy(lds + buf * 2 * TILE + TILE, it * BN, list, wave, lane);
         }
     };
-    if (list.count > 0) stage(0, 0);
+    if (count > 0) stage(0, 0);
 
     typename Ops<T>::Frag q[STEPS], g[STEPS];
     load_row<T, DP>(q, row_at(a.q, b, t, hq, sizeof(T)), a.Dk, live, a.vec, lane);
@@ -140,19 +140,17 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
         for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
     LaneMap<T, DP> map;
     map.init(lane);
-    for (int it = 0, buf = 0; it < list.count; ++it, buf ^= 1) {
+    for (int it = 0, buf = 0; it < count; ++it, buf ^= 1) {
         dma_wait();
         __syncthreads();
-        if (it + 1 < list.count) stage(it + 1, buf ^ 1);
+        if (it + 1 < count) stage(it + 1, buf ^ 1);
 #pragma unroll 1
         for (int n = 0; n < BN / 32; ++n) {
-            const int j0 = list.at(it) * BN + n * 32, j1 = j0 + 32;
-            if (j0 >= wv.hi_max || (j1 <= wv.lo_min && j0 >= a.sinks)) continue;
+            const Frame f = list.frame(it * BN + n * 32, 32);
+            if (!sees_some(wv, f, 32)) continue;
             const unsigned tk = lds0 + buf * 2 * TILE + n * 32 * TL::kRowBytes, tv = tk + TILE;
-            if (j1 <= wv.hi_min && (j0 >= wv.lo_max || j1 <= a.sinks))
-                grad_rows<T, DP, false>(dq, q, g, tk, tv, map, j0, seen, a.sinks, a.scale_log2, lse2, delta, lane);
-            else
-                grad_rows<T, DP, true>(dq, q, g, tk, tv, map, j0, seen, a.sinks, a.scale_log2, lse2, delta, lane);
+            if (sees_all(wv, f, 32)) grad_rows<T, DP, false>(dq, q, g, tk, tv, map, f.j0, seen, f.sinks, a.scale_log2, lse2, delta, lane);
+            else grad_rows<T, DP, true>(dq, q, g, tk, tv, map, f.j0, seen, f.sinks, a.scale_log2, lse2, delta, lane);
         }
     }
     if (r >= rows) return;

@@ -17,7 +17,7 @@ namespace sdpa {
 namespace heads {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -218,15 +218,18 @@ __device__ inline f32x16 mma_cols(const Cols<float> &a, const Probs<float> &b, f
 // sign is theirs), 1 = all of them as NaN (gradients, whose weights have either sign).
 template <typename T, int DP> __device__ inline bool block_not_finite(unsigned tile, int block, int lane) {
     const unsigned at = tile + (unsigned)(opaque(lane) * 16);
-    uint32_t bad = 0;
+    // (0 * x is NaN for what is not finite, and 0 otherwise: one instruction for two bf16 values)
+    float bad = 0.f;
 #pragma unroll 4
     for (int k = 0; k < 32 * Tile<T, DP>::kChunks / 64; ++k) {
         const u32x4 w = lds_read<u32x4>(at + (unsigned)(k * 1024), block * 32 * Tile<T, DP>::kRowBytes);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)      // an exponent of all ones carries into the sign's place
-            bad |= sizeof(T) == 2 ? ((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((w[i] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) bad = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[i]), bf16x2{0, 0}, bad, false);
+            else bad = __builtin_fmaf(__uint_as_float(w[i]), 0.f, bad);
+        }
     }
-    return __any(bad != 0);
+    return __any(bad != bad);
 }
 // kind 0: the finite values; 1: NaN (kinds == 1: anything not finite); 2: +inf; 3: -inf -- 1.0 there, 0 elsewhere
 __device__ inline float pick(float x, int kind, int kinds) {
@@ -328,20 +331,36 @@ __device__ inline SeenRange seen_range(int t0, int t1, int nq, int nk, int windo
     r.hi_min = a.hi; r.hi_max = b.hi; r.lo_min = a.lo; r.lo_max = b.lo;
     return r;
 }
-// the key tiles a run of rows visits: [0, sink_tiles) and [first, end) -- ONE list of `count`, never a tile twice
-struct TileList {
-    int sink_tiles, first, count;
-    __device__ int at(int i) const { return i < sink_tiles ? i : first + (i - sink_tiles); }
+// The keys a run of rows visits as ONE list without a gap: the sinks, then the window from its first key on (or, where the two meet,
+// everything from key 0) -- so that tiles begin at the window's first key and the sinks share a tile with it.
+// A tile of the list is looked at in a frame: its row r is key j0 + r and sinks are what lies below `sinks` -- true for the tiles on
+// either side, and for the tile with both (j0 counted back from the window) the sink rows lie below the window's first key.
+struct Frame { int j0, sinks; };
+struct KeyList {
+    int s, shift, n;                 // entries below s are keys 0 .. s - 1, the others entry + shift; n entries
+    int sinks;
+    __device__ int tiles(int rows) const { return (n + rows - 1) / rows; }
+    __device__ int key(int v) const { return v < s ? v : v + shift; }
+    __device__ Frame frame(int v0, int rows) const {
+        return s == 0 || v0 + rows <= s ? Frame{v0 + (s == 0 ? shift : 0), sinks} : Frame{v0 + shift, s + shift};
+    }
 };
-__device__ inline TileList tile_list(const SeenRange &r, int sinks, int bn) {
-    TileList l;
-    const int sh = sinks < r.hi_max ? sinks : r.hi_max;
-    l.sink_tiles = (sh + bn - 1) / bn;
-    l.first = r.lo_min / bn;
-    if (l.first < l.sink_tiles) l.first = l.sink_tiles;
-    const int end = r.lo_min < r.hi_max ? (r.hi_max + bn - 1) / bn : 0;
-    l.count = l.sink_tiles + (end > l.first ? end - l.first : 0);
+__device__ inline KeyList key_list(const SeenRange &r, int sinks) {
+    KeyList l;
+    const int sh = sinks < r.hi_max ? sinks : r.hi_max, lo = r.lo_min < r.hi_max ? r.lo_min : r.hi_max;
+    const bool gap = sh < lo;
+    l.s = gap ? sh : 0;
+    l.shift = gap ? lo - sh : 0;
+    l.n = gap ? sh + r.hi_max - lo : r.hi_max;
+    l.sinks = sinks;
     return l;
+}
+// does a run of rows see the frame's tile at all / all of it
+__device__ inline bool sees_some(const SeenRange &w, Frame f, int rows) {
+    return f.j0 < w.hi_max && (f.j0 + rows > w.lo_min || f.j0 < f.sinks);
+}
+__device__ inline bool sees_all(const SeenRange &w, Frame f, int rows) {
+    return f.j0 + rows <= w.hi_min && (f.j0 >= w.lo_max || f.j0 + rows <= f.sinks);
 }
 
 // Consecutive workgroups go to the 8 XCDs in turn, and each XCD has an L2 of its own: workgroups that read the same keys are
@@ -382,57 +401,57 @@ __device__ inline void lds_dma(const char *base, unsigned lane_off, unsigned lds
                  : "memory" SDPA_M0_CLOBBER);
 }
 
-// A tile of ROWS rows staged by WAVES waves: keys [j0, j0 + ROWS) of one head.  Rows that no query of the workgroup sees are
-// never followed: a row of the tile that some query sees is read in their place (their weights are masked).
+// A tile of ROWS rows of a key list, staged by WAVES waves.  Rows behind the list's end are read as its last key (their weights are
+// masked), so that nothing is read that no query of the workgroup sees.
+// The waves take the tile's 1 KiB pieces in turn: with four waves a wave's pieces lie 4 KiB apart, where the swizzle (period 16
+// rows) repeats, or nearly so -- kKinds lane offsets serve all of them, the rest of a piece's place is uniform.
 template <typename T, int DP, int ROWS, int WAVES> struct Stager {
     using TL = Tile<T, DP>;
-    static constexpr int kPieces = ROWS * TL::kRowBytes / 1024 / WAVES;       // 1 KiB pieces of a wave
+    static constexpr int kPieces = ROWS * TL::kRowBytes / 1024 / WAVES;       // pieces of a wave
+    static constexpr int kKinds = TL::kRowBytes * 16 / 1024 / WAVES < 1 ? 1 : TL::kRowBytes * 16 / 1024 / WAVES;
     const char *base;                // row 0 of the head
     long token;                      // bytes between rows
     int dim;
-    unsigned off[kPieces];           // lane offsets inside a tile
-    __device__ static int row(int wave, int lane, int k) { return (((wave * kPieces + k) * 1024 + lane * 16) / TL::kRowBytes); }
+    unsigned off[kKinds];            // lane offsets inside a tile
+    __device__ static int row(int wave, int lane, int k) { return (((wave + k * WAVES) * 1024 + lane * 16) / TL::kRowBytes); }
     __device__ static int source(int wave, int lane, int k) {                 // the chunk of its row a lane asks for
-        return (((wave * kPieces + k) * 64 + lane) % TL::kChunks) ^ TL::swz(row(wave, lane, k));
+        return (((wave + k * WAVES) * 64 + lane) % TL::kChunks) ^ TL::swz(row(wave, lane, k));
     }
     __device__ void init(const void *p, long tok, int d, int wave, int lane) {
         base = uniform((const char *)p);
         token = tok * (long)sizeof(T);
         dim = d;
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) off[k] = (unsigned)(row(wave, lane, k) * (int)token) + 16u * (unsigned)source(wave, lane, k);
+        for (int k = 0; k < kKinds; ++k) off[k] = (unsigned)(row(wave, lane, k) * (int)token) + 16u * (unsigned)source(wave, lane, k);
     }
-    // the key read for tile row r
-    __device__ static int key(int r, int j0, const SeenRange &w, int sinks) {
-        int j = j0 + r;
-        if (j >= w.hi_max) j = w.hi_max - 1;
-        if (j < w.lo_min && j >= sinks) j = j0 < sinks ? j0 : w.lo_min;
-        return j;
-    }
-    // asynchronous: 16-byte rows (`token` < 2^31 / ROWS)
-    __device__ void dma(unsigned lds, int j0, const SeenRange &w, int sinks, int wave, int lane) const {
-        const char *at = base + (long)j0 * token;
-        const bool inside = j0 + ROWS <= w.hi_max && (j0 >= w.lo_min || j0 + ROWS <= sinks);
-        const bool whole = dim == DP;
+    // asynchronous: 16-byte rows (a tile's offsets fit 32 bits)
+    __device__ void dma(unsigned lds, int v0, const KeyList &l, int wave, int lane) const {
+        const char *at = base + (long)l.key(v0) * token;
+        lds += (unsigned)wave * 1024u;
+        if (dim == DP && v0 + ROWS <= l.n && (v0 >= l.s || v0 + ROWS <= l.s)) {
+            const long step = token * (kKinds * WAVES * 1024 / TL::kRowBytes);
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            unsigned o = off[k];
-            if (!inside) {
-                const int r = row(wave, opaque(lane), k);
-                o += (unsigned)((key(r, j0, w, sinks) - j0 - r) * (int)token);
+            for (int k = 0; k < kPieces; ++k) lds_dma(at + k / kKinds * step, off[k % kKinds], lds + k * WAVES * 1024u);
+        } else {
+            const int ln = opaque(lane), split = v0 < l.s && l.s < l.n ? l.s : l.n;     // entries of either side: a base each
+            const char *above = base + (long)l.key(split < l.n ? split : v0) * token;
+#pragma unroll 1
+            for (int k = 0; k < kPieces; ++k) {
+                const int r = row(wave, ln, k), c = source(wave, ln, k), v = v0 + r < l.n ? v0 + r : l.n - 1;
+                if (c * Ops<T>::kVec < dim) {                                            // (the padding stays zero)
+                    if (v < split) lds_dma(at, (unsigned)((v - v0) * (int)token) + 16u * (unsigned)c, lds + k * WAVES * 1024u);
+                    else lds_dma(above, (unsigned)((v - split) * (int)token) + 16u * (unsigned)c, lds + k * WAVES * 1024u);
+                }
             }
-            const unsigned dst = lds + (unsigned)(wave * kPieces + k) * 1024u;
-            if (whole) lds_dma(at, o, dst);
-            else if (source(wave, opaque(lane), k) * Ops<T>::kVec < dim) lds_dma(at, o, dst);      // (the padding stays zero)
         }
     }
     // element by element, for rows without 16-byte alignment
-    __device__ void copy(char *tile, int j0, const SeenRange &w, int sinks, int wave, int lane) const {
+    __device__ void copy(char *tile, int v0, const KeyList &l, int wave, int lane) const {
 #pragma unroll 1
         for (int k = 0; k < kPieces; ++k) {
-            const int ln = opaque(lane), r = row(wave, ln, k), c = source(wave, ln, k);
-            const T *src = reinterpret_cast<const T *>(base + (long)key(r, j0, w, sinks) * token);
-            *reinterpret_cast<u32x4 *>(tile + (wave * kPieces + k) * 1024 + lane * 16) = load_chunk(src, c * Ops<T>::kVec, dim, false);
+            const int ln = opaque(lane), r = row(wave, ln, k), c = source(wave, ln, k), v = v0 + r < l.n ? v0 + r : l.n - 1;
+            const T *src = reinterpret_cast<const T *>(base + (long)l.key(v) * token);
+            *reinterpret_cast<u32x4 *>(tile + (wave + k * WAVES) * 1024 + ln * 16) = load_chunk(src, c * Ops<T>::kVec, dim, false);
         }
     }
 };

@@ -51,19 +51,35 @@ __device__ inline void scores(f32x16 *s, const typename Ops<T>::Frag *q, unsigne
     }
 }
 
-// what a lane's column does not see becomes -inf; vis[n] = what it sees
-template <int NB> __device__ inline void hide(f32x16 *s, uint32_t *vis, int j0, Seen seen, int sinks, int lane) {
+// bit i: the lane's column sees row i of the block
+__device__ inline uint32_t seen_bits(int j0, Seen seen, int sinks, int lane) {
     const int half = opaque(lane) >> 5;
+    uint32_t vis = 0;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        vis[n] = 0;
+    for (int i = 0; i < 16; ++i) {
+        const int j = j0 + row_of(i, half);
+        vis |= j < seen.hi && (j >= seen.lo || j < sinks) ? 1u << i : 0u;
+    }
+    return vis;
+}
+// what a lane's column does not see becomes -inf: the future, then what lies before the window (`low`: some of the tile may)
+template <int NB> __device__ inline void hide(f32x16 *s, int j0, Seen seen, int sinks, bool low, int lane) {
+    const int at = j0 + 4 * (opaque(lane) >> 5), hi = seen.hi - at, lo = seen.lo - at, sk = sinks - at;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int j = j0 + n * 32 + row_of(i, half);
-            const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
-            vis[n] |= ok ? 1u << i : 0u;
-            s[n][i] = ok ? s[n][i] : kNegInf;
-        }
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = n * 32 + row_of(i, 0) < hi ? s[n][i] : kNegInf;
+    if (!low) return;
+    if (j0 >= sinks) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = n * 32 + row_of(i, 0) >= lo ? s[n][i] : kNegInf;
+    } else {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = n * 32 + row_of(i, 0) >= lo || n * 32 + row_of(i, 0) < sk ? s[n][i] : kNegInf;
     }
 }
 
@@ -111,14 +127,18 @@ template <typename T, int DP, int NB, bool MASKED>
 __device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag *q, unsigned lk, unsigned lv, const LaneMap<T, DP> &map,
                                      int j0, Seen seen, int sinks, float scale, int lane) {
     f32x16 s[NB];
-    uint32_t vis[NB];
     scores<T, DP, NB>(s, q, lk, map);
-    if (MASKED) hide<NB>(s, vis, j0, seen, sinks, lane);
+    if (MASKED) hide<NB>(s, j0, seen, sinks, true, lane);
     const float ref = raise<DP>(st, largest<NB>(s), scale);
     Probs<T> p[NB];
     weigh<T, DP, NB>(st, s, p, ref, scale);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) mma_block<T, DP, DP / 32>(st.o, lv, map, n, p[n], MASKED, MASKED ? vis[n] : 0u, 3, lane);
+    for (int n = 0; n < NB; ++n) {
+        if (MASKED && __builtin_expect(block_not_finite<T, DP>(lv, n, lane), 0))
+            mma_block_guarded<T, DP, DP / 32>(st.o, lv, map, n, p[n], seen_bits(j0 + n * 32, seen, sinks, lane), 3);
+        else
+            mma_block<T, DP, DP / 32>(st.o, lv, map, n, p[n], false, 0u, 3, lane);
+    }
 }
 
 // a finished row (or its partial triple): 4 consecutive values of row `x`, columns d .. d + 3
@@ -185,43 +205,52 @@ template <typename T, int DP, int NB> struct Pipe {
         if (x < KU) return read_rows<T, DP>(ak, n, x);
         return read_cols_part<DP>(av, n, (x - KU) / VK, (x - KU) % VK, T());
     }
-    // -> the maximum of the next tile's scores in s2
-    __device__ static float run(State<DP> &st, const Frag *q, f32x16 *s, f32x16 *s2, unsigned ak, unsigned av, float ref, float scale) {
-        Frag ring[AHEAD + 1];
-        Probs<T> p[NB];
-        float sum = 0.f, mx = kNegInf;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) s2[n] = f32x16{};
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) ring[u] = fetch(u, ak, av);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const int n = u / PER, x = u % PER;
-            if (u + AHEAD < UNITS) ring[(u + AHEAD) % (AHEAD + 1)] = fetch(u + AHEAD, ak, av);
-            const Frag f = ring[u % (AHEAD + 1)];
-            if (x < KU) s2[n] = Ops<T>::mma(f, q[x], s2[n]);
+    Frag ring[AHEAD + 1];
+    Probs<T> p[NB];
+    float sum, mx;
+    template <int U>
+    __device__ inline __attribute__((always_inline)) void unit(State<DP> &st, const Frag *q, f32x16 *s, f32x16 *s2, unsigned ak, unsigned av,
+                                                               float ref, float scale) {
+        if constexpr (U < UNITS) {
+            constexpr int n = U / PER, x = U % PER;
+            if constexpr (U + AHEAD < UNITS) ring[(U + AHEAD) % (AHEAD + 1)] = fetch(U + AHEAD, ak, av);
+            const Frag f = ring[U % (AHEAD + 1)];
+            if constexpr (x < KU) s2[n] = Ops<T>::mma(f, q[x], s2[n]);
             else st.o[(x - KU) / VK] = mma_part(f, p[n], (x - KU) % VK, st.o[(x - KU) / VK]);
-            // weights: block 0's beside its K units, block n's between the V units of block n - 1 and its own
+            // weights: block 0's beside its K units, block m's between the V units of block m - 1 and its own
 #pragma unroll
             for (int m = 0; m < NB; ++m) {
                 const int first = m == 0 ? 0 : (m - 1) * PER + KU, count = m == 0 ? KU : PER;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (first + i * count / 16 == u) {
+                    if (first + i * count / 16 == U) {
                         s[m][i] = __builtin_amdgcn_exp2f(s[m][i] * scale - ref);
                         sum += s[m][i];
                         if (sizeof(T) == 4 || (i & 1)) put_prob(p[m], s[m], i);
                     }
             }
             // the next tile's maximum, beside the last V units
-            if (u >= UNITS - VU) {
+            if constexpr (U >= UNITS - VU) {
 #pragma unroll
                 for (int i = 0; i < 16 * NB; ++i)
-                    if (i * VU / (16 * NB) == u - (UNITS - VU)) mx = fmaxf(mx, s2[i / 16][i % 16]);
+                    if (i * VU / (16 * NB) == U - (UNITS - VU)) mx = fmaxf(mx, s2[i / 16][i % 16]);
+                asm volatile("" : "+v"(mx));             // (here, and not behind the last unit)
             }
             __builtin_amdgcn_sched_barrier(0);
+            unit<U + 1>(st, q, s, s2, ak, av, ref, scale);
         }
+    }
+    // -> the maximum of the next tile's scores in s2
+    __device__ inline __attribute__((always_inline)) float run(State<DP> &st, const Frag *q, f32x16 *s, f32x16 *s2, unsigned ak, unsigned av,
+                                                               float ref, float scale) {
+        sum = 0.f;
+        mx = kNegInf;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s2[n] = f32x16{};
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) ring[u] = fetch(u, ak, av);
+        __builtin_amdgcn_sched_barrier(0);
+        unit<0>(st, q, s, s2, ak, av, ref, scale);
         st.l += sum;
         return mx;
     }
@@ -259,8 +288,8 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
         wv = seen_range(rw / G, min(rw + 31, rows - 1) / G, nq, nk, a.window);
         if (x.live) seen = seen_at(nk - nq + x.t, nk, a.window);
     }
-    const TileList list = tile_list(wg, a.sinks, BN);
-    const int it0 = (int)((long)list.count * split / a.splits), it1 = (int)((long)list.count * (split + 1) / a.splits);
+    const KeyList list = key_list(wg, a.sinks);
+    const int count = list.tiles(BN), it0 = (int)((long)count * split / a.splits), it1 = (int)((long)count * (split + 1) / a.splits);
     Stager<T, DP, BN, 4> sk, sv;
     sk.init((const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head, a.k.token, a.Dk, wave, lane);
     sv.init((const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head, a.v.token, a.Dv, wave, lane);
@@ -269,18 +298,12 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
         __syncthreads();
     }
     const unsigned lds0 = lds_address(lds);
-    auto stage_k = [&](int it) {
-        if (it >= it1) return;
-        const int j0 = list.at(it) * BN, buf = (it - it0) & 1;
-        if (VEC) sk.dma(lds0 + buf * TILE, j0, wg, a.sinks, wave, lane);
-        else sk.copy(lds + buf * TILE, j0, wg, a.sinks, wave, lane);
+    auto stage_at = [&](const Stager<T, DP, BN, 4> &stager, int it, int place) {
+        if (VEC) stager.dma(lds0 + place * TILE, it * BN, list, wave, lane);
+        else stager.copy(lds + place * TILE, it * BN, list, wave, lane);
     };
-    auto stage_v = [&](int it) {
-        if (it >= it1) return;
-        const int j0 = list.at(it) * BN, buf = (it - it0) & 1;
-        if (VEC) sv.dma(lds0 + (2 + buf) * TILE, j0, wg, a.sinks, wave, lane);
-        else sv.copy(lds + (2 + buf) * TILE, j0, wg, a.sinks, wave, lane);
-    };
+    auto stage_k = [&](int it) { if (it < it1) stage_at(sk, it, (it - it0) & 1); };
+    auto stage_v = [&](int it) { if (it < it1) stage_at(sv, it, 2 + ((it - it0) & 1)); };
     stage_k(it0);
 
     typename Ops<T>::Frag q[STEPS];
@@ -289,25 +312,21 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
     st.clear();
     LaneMap<T, DP> map;
     map.init(lane);
-    // does the wave see the tile at all / every key of it with every row
-    auto sees = [&](int it) {
-        const int j0 = list.at(it) * BN;
-        return j0 < wv.hi_max && (j0 + BN > wv.lo_min || j0 < a.sinks);
-    };
     f32x16 s[NB];
     float mx = kNegInf;
-    bool cur = false;
+    bool cur = false, odd = false;                       // odd: a tile with masked pairs holds values that are no numbers
     if (it0 < it1) {
         dma_wait();
         __syncthreads();
         stage_k(it0 + 1);
         stage_v(it0);
-        cur = sees(it0);
+        cur = sees_some(wv, list.frame(it0 * BN, BN), BN);
         if (cur) {
             scores<T, DP, NB>(s, q, lds0, map);
             mx = largest<NB>(s);
         }
     }
+#pragma unroll 1
     for (int it = it0; it < it1; ++it) {
         const int buf = (it - it0) & 1;
         dma_wait();
@@ -315,42 +334,45 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
         stage_k(it + 2);
         stage_v(it + 1);
         const unsigned lk = lds0 + (buf ^ 1) * TILE, lv = lds0 + (2 + buf) * TILE;
-        const bool next = it + 1 < it1 && sees(it + 1), had = cur;
-        cur = next;
+        const bool had = cur;
+        cur = it + 1 < it1 && sees_some(wv, list.frame((it + 1) * BN, BN), BN);
         if (!had) {
-            if (next) {
+            if (cur) {
                 scores<T, DP, NB>(s, q, lk, map);
                 mx = largest<NB>(s);
             }
             continue;
         }
-        const int j0 = list.at(it) * BN;
-        if (j0 + BN > wv.hi_min || (j0 < wv.lo_max && j0 + BN > a.sinks)) {          // some row does not see some key
-            uint32_t vis[NB];
-            hide<NB>(s, vis, j0, seen, a.sinks, lane);
+        const Frame f = list.frame(it * BN, BN);
+        if (!sees_all(wv, f, BN)) {
+            hide<NB>(s, f.j0, seen, f.sinks, f.j0 < wv.lo_max, lane);
             mx = largest<NB>(s);
-            bool odd = false;
 #pragma unroll 1
             for (int n = 0; n < NB; ++n) odd = odd || block_not_finite<T, DP>(lv, n, lane);
-            if (__builtin_expect(odd, 0)) {
-                const float ref = raise<DP>(st, mx, a.scale_log2);
-                Probs<T> p[NB];
-                weigh<T, DP, NB>(st, s, p, ref, a.scale_log2);
-#pragma unroll
-                for (int n = 0; n < NB; ++n) mma_block_guarded<T, DP, DP / 32>(st.o, lv, map, n, p[n], vis[n], 3);
-                if (next) {
-                    scores<T, DP, NB>(s, q, lk, map);
-                    mx = largest<NB>(s);
-                }
-                continue;
-            }
         }
         const float ref = raise<DP>(st, mx, a.scale_log2);
         // (behind the last tile the scores of a stale tile are multiplied and dropped)
         f32x16 s2[NB];
-        mx = Pipe<T, DP, NB>::run(st, q, s, s2, lk + map.rows, lv + map.cols, ref, a.scale_log2);
+        Pipe<T, DP, NB> pipe;
+        mx = pipe.run(st, q, s, s2, lk + map.rows, lv + map.cols, ref, a.scale_log2);
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[n] = s2[n];
+    }
+    // Such a tile gave NaN to rows that do not see it: the workgroup does its rows once more, with a guarded product and
+    // otherwise the same arithmetic.
+    if (__syncthreads_or(odd)) {
+        st.clear();
+#pragma unroll 1
+        for (int it = it0; it < it1; ++it) {
+            __syncthreads();
+            stage_at(sk, it, 0);
+            stage_at(sv, it, 2);
+            dma_wait();
+            __syncthreads();
+            const Frame f = list.frame(it * BN, BN);
+            if (sees_some(wv, f, BN))
+                attend_blocks<T, DP, NB, true>(st, q, lds0, lds0 + 2 * TILE, map, f.j0, seen, f.sinks, a.scale_log2, lane);
+        }
     }
     st.l = half_sum(st.l);
     if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (tiles that need no mask gave weights to rows that do not exist)
@@ -401,8 +423,8 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
         wg = seen_range(0, a.Tq - 1, nq, nk, a.window);
         if (x.live) seen = seen_at(nk - nq + x.t, nk, a.window);
     }
-    const TileList list = tile_list(wg, a.sinks, 32);
-    const int it0 = (int)((long)list.count * split / a.splits), it1 = (int)((long)list.count * (split + 1) / a.splits);
+    const KeyList list = key_list(wg, a.sinks);
+    const int count = list.tiles(32), it0 = (int)((long)count * split / a.splits), it1 = (int)((long)count * (split + 1) / a.splits);
 
     typename Ops<T>::Frag q[DP / Ops<T>::kStep];
     load_query<T, DP>(q, a, x, hq, lane);
@@ -417,12 +439,13 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
     const T *vb = (const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head;
     constexpr int PIECES = 32 * TL::kChunks / 64;
     for (int it = it0 + wave; it < it1; it += WAVES) {
-        const int j0 = list.at(it) * 32, j1 = j0 + 32;
+        const int v0 = it * 32;
 #pragma unroll
         for (int k = 0; k < PIECES; ++k) {
-            const int c = lane + k * 64, row = c / TL::kChunks, j = j0 + row, d = (c % TL::kChunks) * Ops<T>::kVec;
+            const int c = lane + k * 64, row = c / TL::kChunks, d = (c % TL::kChunks) * Ops<T>::kVec;
             u32x4 rk = {0, 0, 0, 0}, rv = {0, 0, 0, 0};
-            if (j < wg.hi_max && (j >= wg.lo_min || j < a.sinks)) {
+            if (v0 + row < list.n) {
+                const int j = list.key(v0 + row);
                 rk = load_chunk(kb + (long)j * a.k.token, d, a.Dk, a.vec);
                 rv = load_chunk(vb + (long)j * a.v.token, d, a.Dv, a.vec);
             }
@@ -431,10 +454,9 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
             *reinterpret_cast<u32x4 *>(wv + at) = rv;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (a wave reads only what it wrote itself)
-        if (j1 <= wg.hi_min && (j0 >= wg.lo_max || j1 <= a.sinks))
-            attend_blocks<T, DP, 1, false>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
-        else
-            attend_blocks<T, DP, 1, true>(st, q, lk, lv, map, j0, seen, a.sinks, a.scale_log2, lane);
+        const Frame f = list.frame(v0, 32);
+        if (sees_all(wg, f, 32)) attend_blocks<T, DP, 1, false>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane);
+        else attend_blocks<T, DP, 1, true>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     st.l = half_sum(st.l);
