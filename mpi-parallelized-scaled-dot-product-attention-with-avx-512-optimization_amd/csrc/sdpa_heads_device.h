@@ -424,14 +424,15 @@ template <typename T, int DP, int ROWS, int WAVES> struct Stager {
 #pragma unroll
         for (int k = 0; k < kKinds; ++k) off[k] = (unsigned)(row(wave, lane, k) * (int)token) + 16u * (unsigned)source(wave, lane, k);
     }
-    // asynchronous: 16-byte rows (a tile's offsets fit 32 bits)
-    __device__ void dma(unsigned lds, int v0, const KeyList &l, int wave, int lane) const {
+    // asynchronous: 16-byte rows (a tile's offsets fit 32 bits).  -> true: exactly kPieces instructions are on their way
+    __device__ bool dma(unsigned lds, int v0, const KeyList &l, int wave, int lane) const {
         const char *at = base + (long)l.key(v0) * token;
         lds += (unsigned)wave * 1024u;
         if (dim == DP && v0 + ROWS <= l.n && (v0 >= l.s || v0 + ROWS <= l.s)) {
             const long step = token * (kKinds * WAVES * 1024 / TL::kRowBytes);
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) lds_dma(at + k / kKinds * step, off[k % kKinds], lds + k * WAVES * 1024u);
+            return true;
         } else {
             const int ln = opaque(lane), split = v0 < l.s && l.s < l.n ? l.s : l.n;     // entries of either side: a base each
             const char *above = base + (long)l.key(split < l.n ? split : v0) * token;
@@ -443,6 +444,7 @@ template <typename T, int DP, int ROWS, int WAVES> struct Stager {
                     else lds_dma(above, (unsigned)((v - split) * (int)token) + 16u * (unsigned)c, lds + k * WAVES * 1024u);
                 }
             }
+            return false;
         }
     }
     // element by element, for rows without 16-byte alignment
@@ -460,6 +462,7 @@ __device__ inline void zero_lds(char *p, int bytes, int threads) {
     for (int i = threadIdx.x * 16; i < bytes; i += threads * 16) *reinterpret_cast<u32x4 *>(p + i) = u32x4{0, 0, 0, 0};
 }
 __device__ inline void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N> __device__ inline void dma_wait_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 }  // namespace heads
 }  // namespace sdpa

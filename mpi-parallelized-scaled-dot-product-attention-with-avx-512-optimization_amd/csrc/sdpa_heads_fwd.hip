@@ -398,14 +398,21 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
 }
 
 // ---- few rows (single tokens): the waves share 32 rows and take the key tiles in turn ------------------------------------
-// (fp32 rows of 256: two waves, whose tiles fill the LDS)
-template <typename T, int DP, int WAVES>
+// Bound by the reading of the cache.  Every wave stages its own tiles of 32 keys (no barriers), the next one on its way by DMA while this
+// one is multiplied: 64 KiB in flight on a CU.  (fp32 tiles are bound by their matrix instructions and are not double-buffered.)
+template <typename T, int DP> struct FewShape {
+    static constexpr int kPair = 2 * 32 * DP * (int)sizeof(T);                              // a K and a V tile
+    static constexpr int kBufs = sizeof(T) == 2 || DP == 64 ? 2 : 1;
+    static constexpr int kWaves = kPair * kBufs * 4 <= 131072 ? 4 : 2;
+};
+template <typename T, int DP, int WAVES, bool VEC>
 __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, int rows, int G) {
     using TL = Tile<T, DP>;
-    constexpr int WAVE_BYTES = 2 * 32 * TL::kRowBytes > 32 * DP * 4 ? 2 * 32 * TL::kRowBytes : 32 * DP * 4;
+    constexpr int TILE = 32 * TL::kRowBytes, NBUF = FewShape<T, DP>::kBufs, WAVE_BYTES = 2 * TILE * NBUF;
+    static_assert(WAVE_BYTES >= 32 * DP * 4, "the waves' rows are joined in the same memory");
     __shared__ __attribute__((aligned(1024))) char lds[WAVES * WAVE_BYTES];
     __shared__ float lm[WAVES][32], ll[WAVES][32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = xcd_place(blockIdx.x, gridDim.x);
     const int split = id % a.splits;
     id /= a.splits;
@@ -426,38 +433,46 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
     const KeyList list = key_list(wg, a.sinks);
     const int count = list.tiles(32), it0 = (int)((long)count * split / a.splits), it1 = (int)((long)count * (split + 1) / a.splits);
 
+    char *mine = lds + wave * WAVE_BYTES;
+    const unsigned lds0 = lds_address(mine);
+    Stager<T, DP, 32, 1> sk, sv;
+    sk.init((const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head, a.k.token, a.Dk, 0, lane);
+    sv.init((const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head, a.v.token, a.Dv, 0, lane);
+    if (VEC && (a.Dk < DP || a.Dv < DP)) {               // (its own part only: no barrier)
+        for (int i = lane * 16; i < WAVE_BYTES; i += 1024) *reinterpret_cast<u32x4 *>(mine + i) = u32x4{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    // -> true: exactly 2 * kPieces instructions are on their way
+    auto stage = [&](int it, int buf) {
+        if (VEC) {
+            const bool p = sk.dma(lds0 + buf * 2 * TILE, it * 32, list, 0, lane);
+            return sv.dma(lds0 + buf * 2 * TILE + TILE, it * 32, list, 0, lane) && p;
+        }
+        sk.copy(mine + buf * 2 * TILE, it * 32, list, 0, lane);
+        sv.copy(mine + buf * 2 * TILE + TILE, it * 32, list, 0, lane);
+        return false;
+    };
+    if (NBUF == 2 && it0 + wave < it1) stage(it0 + wave, 0);
     typename Ops<T>::Frag q[DP / Ops<T>::kStep];
     load_query<T, DP>(q, a, x, hq, lane);
     State<DP> st;
     st.clear();
     LaneMap<T, DP> map;
     map.init(lane);
-
-    char *wk = lds + wave * WAVE_BYTES, *wv = wk + 32 * TL::kRowBytes;
-    const unsigned lk = lds_address(wk), lv = lds_address(wv);
-    const T *kb = (const T *)a.k.data + (a.shared ? 0 : b * a.k.batch) + h * a.k.head;
-    const T *vb = (const T *)a.v.data + (a.shared ? 0 : b * a.v.batch) + h * a.v.head;
-    constexpr int PIECES = 32 * TL::kChunks / 64;
-    for (int it = it0 + wave; it < it1; it += WAVES) {
-        const int v0 = it * 32;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = lane + k * 64, row = c / TL::kChunks, d = (c % TL::kChunks) * Ops<T>::kVec;
-            u32x4 rk = {0, 0, 0, 0}, rv = {0, 0, 0, 0};
-            if (v0 + row < list.n) {
-                const int j = list.key(v0 + row);
-                rk = load_chunk(kb + (long)j * a.k.token, d, a.Dk, a.vec);
-                rv = load_chunk(vb + (long)j * a.v.token, d, a.Dv, a.vec);
-            }
-            const int at = TL::chunk(row, c % TL::kChunks);
-            *reinterpret_cast<u32x4 *>(wk + at) = rk;
-            *reinterpret_cast<u32x4 *>(wv + at) = rv;
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (a wave reads only what it wrote itself)
-        const Frame f = list.frame(v0, 32);
+#pragma unroll 1
+    for (int it = it0 + wave, buf = 0; it < it1; it += WAVES) {
+        bool exact = false;
+        if (NBUF == 1) stage(it, 0);
+        else if (it + WAVES < it1) exact = stage(it + WAVES, buf ^ 1);
+        if (NBUF == 2 && exact) dma_wait_but<2 * Stager<T, DP, 32, 1>::kPieces>();
+        else dma_wait();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (a wave reads only what it staged itself)
+        const unsigned lk = lds0 + buf * 2 * TILE, lv = lk + TILE;
+        const Frame f = list.frame(it * 32, 32);
         if (sees_all(wg, f, 32)) attend_blocks<T, DP, 1, false>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane);
         else attend_blocks<T, DP, 1, true>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // (its reads are over before the tile is written again)
+        if (NBUF == 2) buf ^= 1;
     }
     st.l = half_sum(st.l);
     if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (blocks that need no mask gave weights to rows that do not exist)
@@ -473,7 +488,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) l += ll[w][col] * __builtin_amdgcn_exp2f(lm[w][col] - ref);
     const float alpha = __builtin_amdgcn_exp2f(st.m - ref);
-    float *lo = reinterpret_cast<float *>(lds + wave * WAVE_BYTES);
+    float *lo = reinterpret_cast<float *>(mine);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -553,8 +568,9 @@ template <typename T, int DP>
 void attend(const AttendArgs &a, int rows, int G, int groups, hipStream_t s) {
     constexpr int BN = DP * (int)sizeof(T) <= 256 ? 64 : 32;
     if (rows <= kFewRows) {
-        constexpr int WAVES = DP * (int)sizeof(T) > 512 ? 2 : 4;
-        attend_few_kernel<T, DP, WAVES><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
+        constexpr int WAVES = FewShape<T, DP>::kWaves;
+        if (a.vec) attend_few_kernel<T, DP, WAVES, true><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
+        else attend_few_kernel<T, DP, WAVES, false><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
     } else {
         const int tiles = (rows + 127) / 128, grid = groups * a.splits * tiles;
         if (a.vec) attend_rows_kernel<T, DP, BN, true><<<grid, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
