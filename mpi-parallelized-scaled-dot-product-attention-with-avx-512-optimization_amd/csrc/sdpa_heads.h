@@ -32,6 +32,8 @@ struct AttendArgs {
     const int *q_lens, *kv_lens;      // [B] or null
     float *part;                      // [slots][B*Tq*Hq][Dv] un-normalised rows (null: the launch writes out / lse itself)
     float2 *stat;                     // [slots][B*Tq*Hq] (reference exponent, sum)
+    float *scores;                    // [B][Hkv][Tq * G][score_ld] raw scores for the weights (launches over few rows; may be null)
+    long score_ld;
     int slot0, splits;                // this launch's slots
     int B, Tq, Tk, Hq, Hkv, Dk, Dv;
     int window, sinks;
@@ -55,10 +57,15 @@ struct BackwardArgs {
     float scale, scale_log2;
 };
 
+// attention_scored: the weights every key was given, from the scores that were kept or from the products once more
 struct WeightArgs {
     sdpa_tensor q, k;
     const float *lse, *w_in;
     float *w_out;
+    const float *scores;
+    const float2 *stat;               // the slots of the rows (null: lse holds)
+    long score_ld;
+    int slots;
     long wi_batch, wi_head, wo_batch, wo_head;
     const int *q_lens, *kv_lens;
     int B, Tq, Tk, Hq, Hkv, Dk, vec;
@@ -78,6 +85,8 @@ struct EvictArgs {
 
 hipError_t launch_attend(const AttendArgs &a, int dtype, hipStream_t s);
 hipError_t launch_combine(const AttendArgs &a, int slots, int dtype, hipStream_t s);
+// the same and, in the same launch, w_out from the scores kept by launch_attend
+hipError_t launch_combine_scored(const AttendArgs &a, const WeightArgs &w, int slots, int dtype, hipStream_t s);
 hipError_t launch_attend_backward(const BackwardArgs &a, int dtype, hipStream_t s);
 hipError_t launch_weights(const WeightArgs &a, int dtype, hipStream_t s);
 hipError_t launch_evict(const EvictArgs &a, hipStream_t s);

@@ -12,7 +12,7 @@ using namespace sdpa;
 
 constexpr int kMaxTokens = 1 << 30;
 constexpr int kMaxSplits = 64;
-constexpr double kMaxRows = (1 << 27) - 1, kMaxGroups = (1 << 24) - 1;
+constexpr double kMaxRows = (1 << 24) - 1, kMaxGroups = (1 << 24) - 1;
 
 bool bad_tensor(const sdpa_tensor &t, bool needed) {
     return (needed && !t.data) || t.batch < 0 || t.token < 0 || t.head < 0;
@@ -38,7 +38,7 @@ int check_attention(const sdpa_heads *a) {
     if (a->q_heads < 1 || a->q_heads % a->kv_heads != 0) return SDPA_EINVAL;
     if (a->window < 0 || a->sinks < 0 || a->prefix_tokens < 0 || !(a->scale == a->scale)) return SDPA_EINVAL;
     if (a->prefix_tokens > kMaxTokens) return SDPA_EUNSUP;
-    // a launch has less than 2^32 threads: 32 for each row of the join, 256 for each 128 keys or rows of a head
+    // a launch has less than 2^32 threads: 256 for each row of the join (where keys are split), for each 128 keys or rows of a head
     const double rows = (double)a->batch * a->q_tokens * a->q_heads, groups = (double)a->batch * a->kv_heads;
     if (rows > kMaxRows || groups * (ceil_div(a->kv_tokens, 128) + 1) > kMaxGroups) return SDPA_EUNSUP;
     return SDPA_OK;
@@ -48,12 +48,12 @@ bool empty(const sdpa_heads *a) { return a->batch == 0 || a->q_tokens == 0; }
 
 // How many workgroups share the keys of a row tile.  A launch wants about two workgroups on each of the 256 CUs; a split costs a
 // partial row (4 * dv + 8 bytes written and read) per query row and needs keys enough to be worth its start: one 32-key tile
-// for each of its waves.
+// for each of its waves where they take the keys in turn, a tile of 64 where they share it.
 int pick_splits(long groups, long rows, long keys) {
     const long tiles = rows <= kFewRows ? 1 : ceil_div(rows, 128);
     const long have = groups * tiles;
     long want = ceil_div(512, have < 1 ? 1 : have);
-    const long most = ceil_div(keys, 128);
+    const long most = ceil_div(keys, rows <= kFewRows ? 128 : 64);
     if (want > most) want = most;
     if (want > kMaxSplits) want = kMaxSplits;
     return want < 1 ? 1 : (int)want;
@@ -83,19 +83,22 @@ long keys_seen(const sdpa_heads *a, long rows) {
 
 struct Slots {
     int own, prefix;              // slots of the sequences' own keys and of the prefix
-    long rows, bytes;
-    void size(const sdpa_heads *a) {
+    long rows, part, bytes;       // bytes of the slots, and of everything
+    long score_ld;                // kept scores (attention_scored over few rows): their row, 0 = none
+    void size(const sdpa_heads *a, bool scored) {
         rows = (long)a->batch * a->q_tokens * a->q_heads;
         const int n = own + prefix;
-        bytes = n > 1 ? n * rows * ((long)a->dv * 4 + 8) + 32 : 0;
+        part = n > 1 ? ((n * rows * 8 + 15) / 16 * 16 + n * rows * (long)a->dv * 4 + 15) / 16 * 16 : 0;
+        score_ld = scored && (long)a->q_tokens * (a->q_heads / a->kv_heads) <= kFewRows ? ceil_div(a->kv_tokens, 32) * 32 : 0;
+        bytes = part + rows * score_ld * 4;
     }
 };
 
-Slots plan_window(const sdpa_heads *a) {
+Slots plan_window(const sdpa_heads *a, bool scored) {
     Slots s = {};
     const long rows = (long)a->q_tokens * (a->q_heads / a->kv_heads);
     s.own = pick_splits((long)a->batch * a->kv_heads, rows, keys_seen(a, rows));
-    s.size(a);
+    s.size(a, scored);
     return s;
 }
 
@@ -104,7 +107,7 @@ Slots plan_prefix(const sdpa_heads *a) {
     const long rows = (long)a->q_tokens * (a->q_heads / a->kv_heads);
     s.own = pick_splits((long)a->batch * a->kv_heads, rows, a->kv_tokens);
     s.prefix = a->prefix_tokens > 0 ? pick_splits(a->kv_heads, rows * a->batch, a->prefix_tokens) : 0;
-    s.size(a);
+    s.size(a, false);
     return s;
 }
 
@@ -203,7 +206,7 @@ long sdpa_dev_heads_workspace(int op, const struct sdpa_heads *a) {
     sdpa_heads x = *a;
     if (op == SDPA_OP_PREFIX || op == SDPA_OP_SCORED) { x.window = kMaxTokens; x.sinks = 0; }
     switch (op) {
-        case SDPA_OP_WINDOW: case SDPA_OP_SCORED: return plan_window(&x).bytes;
+        case SDPA_OP_WINDOW: case SDPA_OP_SCORED: return plan_window(&x, op == SDPA_OP_SCORED).bytes;
         case SDPA_OP_PREFIX: return plan_prefix(&x).bytes;
         default: return SDPA_EINVAL;
     }
@@ -212,7 +215,7 @@ long sdpa_dev_heads_workspace(int op, const struct sdpa_heads *a) {
 int sdpa_dev_attention_window(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream) {
     SDPA_TRY(check_forward(a));
     if (empty(a)) return SDPA_OK;
-    const Slots s = plan_window(a);
+    const Slots s = plan_window(a, false);
     SDPA_TRY(check_scratch(s.bytes, workspace, workspace_bytes));
     SDPA_TRY(require_device());
     return run_own(a, s, workspace, (hipStream_t)stream);
@@ -291,11 +294,10 @@ int sdpa_dev_attention_scored(const struct sdpa_heads *a, void *workspace, size_
     x.sinks = 0;
     Slots s = {};
     if (!empty(a)) {
-        s = plan_window(&x);
+        s = plan_window(&x, true);
         SDPA_TRY(check_scratch(s.bytes, workspace, workspace_bytes));
     }
     SDPA_TRY(require_device());
-    if (!empty(a)) SDPA_TRY(run_own(&x, s, workspace, (hipStream_t)stream));
     WeightArgs w = {};
     w.q = a->q; w.k = a->k; w.lse = a->lse; w.w_in = a->weights; w.w_out = a->weights_out;
     w.wi_batch = a->weights_batch; w.wi_head = a->weights_head; w.wo_batch = a->weights_out_batch; w.wo_head = a->weights_out_head;
@@ -303,6 +305,19 @@ int sdpa_dev_attention_scored(const struct sdpa_heads *a, void *workspace, size_
     w.B = a->batch; w.Tq = a->q_tokens; w.Tk = a->kv_tokens; w.Hq = a->q_heads; w.Hkv = a->kv_heads; w.Dk = a->dk;
     w.vec = rows_vec(a->q, a->dk, a->dtype) && rows_vec(a->k, a->dk, a->dtype);
     w.scale_log2 = a->scale * 1.44269504088896341f;
+    if (!empty(a) && s.score_ld > 0) {                   // (over few rows) the scores are kept, and the weights come with the join
+        AttendArgs f = attend_args(&x);
+        f.splits = s.own;
+        carve(f, s, workspace);
+        f.scores = (float *)((char *)workspace + s.part);
+        f.score_ld = s.score_ld;
+        HIP_TRY(launch_attend(f, a->dtype, (hipStream_t)stream));
+        w.scores = f.scores; w.score_ld = s.score_ld; w.stat = f.stat; w.slots = s.own;
+        w.scale_log2 = f.scale_log2;                     // (their queries have the scale's sign already)
+        HIP_TRY(launch_combine_scored(f, w, s.own, a->dtype, (hipStream_t)stream));
+        return SDPA_OK;
+    }
+    if (!empty(a)) SDPA_TRY(run_own(&x, s, workspace, (hipStream_t)stream));
     HIP_TRY(launch_weights(w, a->dtype, (hipStream_t)stream));
     return SDPA_OK;
 }

@@ -125,10 +125,17 @@ __device__ inline void weigh(State<DP> &st, f32x16 *s, Probs<T> *p, float ref, f
 
 template <typename T, int DP, int NB, bool MASKED>
 __device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag *q, unsigned lk, unsigned lv, const LaneMap<T, DP> &map,
-                                     int j0, Seen seen, int sinks, float scale, int lane) {
+                                     int j0, Seen seen, int sinks, float scale, int lane, float *keep = nullptr) {
     f32x16 s[NB];
     scores<T, DP, NB>(s, q, lk, map);
     if (MASKED) hide<NB>(s, j0, seen, sinks, true, lane);
+    if (keep) {                                         // the lane's row of kept scores, at this tile
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(keep + n * 32 + 8 * i + 4 * (lane >> 5)) = f32x4{s[n][4 * i], s[n][4 * i + 1], s[n][4 * i + 2], s[n][4 * i + 3]};
+    }
     const float ref = raise<DP>(st, largest<NB>(s), scale);
     Probs<T> p[NB];
     weigh<T, DP, NB>(st, s, p, ref, scale);
@@ -459,6 +466,8 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
     st.clear();
     LaneMap<T, DP> map;
     map.init(lane);
+    // (kept scores: the row of a lane that has one; the list of attention_scored is the cache itself)
+    float *kept = a.scores && (lane & 31) < rows ? a.scores + (((long)b * a.Hkv + h) * rows + (lane & 31)) * a.score_ld : nullptr;
 #pragma unroll 1
     for (int it = it0 + wave, buf = 0; it < it1; it += WAVES) {
         bool exact = false;
@@ -469,8 +478,9 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (a wave reads only what it staged itself)
         const unsigned lk = lds0 + buf * 2 * TILE, lv = lk + TILE;
         const Frame f = list.frame(it * 32, 32);
-        if (sees_all(wg, f, 32)) attend_blocks<T, DP, 1, false>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane);
-        else attend_blocks<T, DP, 1, true>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane);
+        float *keep = kept ? kept + it * 32 : nullptr;
+        if (sees_all(wg, f, 32)) attend_blocks<T, DP, 1, false>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane, keep);
+        else attend_blocks<T, DP, 1, true>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane, keep);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // (its reads are over before the tile is written again)
         if (NBUF == 2) buf ^= 1;
     }
@@ -519,29 +529,35 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
 }
 
 // ---- the join of the slots: the merge of partial triples ------------------------------------------------------------
-// 32 lanes to a row, 8 rows to a workgroup.
+// A workgroup to a row: 32 lanes to its columns, eight groups of lanes to the slots.  (Eight rows to a workgroup, each walking its slots one
+// after the other, took 34 us for 2048 rows of 34 slots; the loads of a row are now eight deep.)
 template <typename T>
-__global__ __launch_bounds__(kHeadsThreads) void combine_kernel(AttendArgs a, int slots) {
-    const long rows = (long)a.B * a.Tq * a.Hq, r = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (r >= rows) return;
-    const int lane = threadIdx.x & 31;
+__device__ inline void combine_row(const AttendArgs &a, int slots, long r) {
+    __shared__ f32x4 sum[8][64];
+    const long rows = (long)a.B * a.Tq * a.Hq;
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
     float m = kNegInf;
-    for (int s = 0; s < slots; ++s) {
-        const float2 ml = a.stat[s * rows + r];
-        if (ml.y != 0.f) m = fmaxf(m, ml.x);
+    for (int s = 0; s < slots; s += 32) {
+        float2 ml = make_float2(kNegInf, 0.f);
+        if (s + lane < slots) ml = a.stat[(s + lane) * rows + r];
+        m = fmaxf(m, ml.y != 0.f ? ml.x : kNegInf);
     }
-    RowId x;
-    const int hq = (int)(r % a.Hq);
-    const long bt = r / a.Hq;
-    x.b = (int)(bt / a.Tq); x.t = (int)(bt - (long)x.b * a.Tq); x.g = 0; x.live = true;
-    float l = 0.f;
-    f32x4 acc[2] = {};
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float ref = m == kNegInf ? 0.f : m;
-    for (int s = 0; s < slots; ++s) {
+    float l = 0.f;
+    for (int s = 0; s < slots; s += 32) {
+        float2 ml = make_float2(kNegInf, 0.f);
+        if (s + lane < slots) ml = a.stat[(s + lane) * rows + r];
+        if (ml.y != 0.f) l += ml.y * __builtin_amdgcn_exp2f(ml.x - ref);
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) l += __shfl_xor(l, d);
+    f32x4 acc[2] = {};
+    for (int s = group; s < slots; s += 8) {
         const float2 ml = a.stat[s * rows + r];
-        if (ml.y == 0.f) continue;
+        if (ml.y == 0.f) continue;                       // (an empty slot was not written)
         const float w = __builtin_amdgcn_exp2f(ml.x - ref);
-        l += ml.y * w;
         const float *src = a.part + (s * rows + r) * a.Dv;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -555,13 +571,69 @@ __global__ __launch_bounds__(kHeadsThreads) void combine_kernel(AttendArgs a, in
             }
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    sum[group][lane] = acc[0];
+    sum[group][32 + lane] = acc[1];
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    f32x4 v = sum[0][threadIdx.x];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int d = k * 128 + lane * 4;
-        if (d < a.Dv) store4<T>(a, x, hq, d, acc[k] * inv);
+    for (int g = 1; g < 8; ++g) v += sum[g][threadIdx.x];
+    RowId x;
+    const int hq = (int)(r % a.Hq), d = threadIdx.x * 4;
+    const long bt = r / a.Hq;
+    x.b = (int)(bt / a.Tq); x.t = (int)(bt - (long)x.b * a.Tq); x.g = 0; x.live = true;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (d < a.Dv) store4<T>(a, x, hq, d, v * inv);
+    if (threadIdx.x == 0) a.lse[((long)x.b * a.Hq + hq) * a.Tq + x.t] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+}
+template <typename T>
+__global__ __launch_bounds__(kHeadsThreads) void combine_kernel(AttendArgs a, int slots) { combine_row<T>(a, slots, blockIdx.x); }
+
+// w_out_j = w_in_j + sum over the rows of exp2(s_j - lse), from the kept scores: 1024 keys of a head to a workgroup
+__device__ inline void add_weights(const WeightArgs &w, int block) {
+    const int blocks = (w.Tk + 1023) / 1024, part = block % blocks, bh = block / blocks, h = bh % w.Hkv, b = bh / w.Hkv, G = w.Hq / w.Hkv;
+    const int nq = clamp_len(w.q_lens, b, w.Tq), nk = clamp_len(w.kv_lens, b, w.Tk), rows = nq * G, all = w.Tq * G;
+    __shared__ float lse2[kFewRows];
+    if ((int)threadIdx.x < rows) {
+        const int t = threadIdx.x / G, hq = h * G + threadIdx.x - t * G;
+        float x;
+        if (w.stat) {
+            const long n = (long)w.B * w.Tq * w.Hq, r = ((long)b * w.Tq + t) * w.Hq + hq;
+            float m = kNegInf, l = 0.f;
+            for (int s = 0; s < w.slots; ++s) {
+                const float2 ml = w.stat[s * n + r];
+                if (ml.y == 0.f) continue;
+                const float top = fmaxf(m, ml.x);
+                l = l * __builtin_amdgcn_exp2f(m - top) + ml.y * __builtin_amdgcn_exp2f(ml.x - top);
+                m = top;
+            }
+            x = l == 0.f ? kNegInf : m + __log2f(l);
+        } else x = w.lse[((long)b * w.Hq + hq) * w.Tq + t] * kLog2e;
+        lse2[threadIdx.x] = x == kNegInf ? __builtin_inff() : x;         // (a row that sees nothing gives nothing)
     }
-    if (lane == 0) a.lse[((long)x.b * a.Hq + hq) * a.Tq + x.t] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+    __syncthreads();
+    const int j = part * 1024 + threadIdx.x * 4;
+    if (j >= w.Tk) return;
+    f32x4 sum = {};
+    if (j < nk) {
+        const float *src = w.scores + (long)bh * all * w.score_ld + j;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+            const f32x4 s = *reinterpret_cast<const f32x4 *>(src + (long)r * w.score_ld);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(s[i] * w.scale_log2 - lse2[r]);
+        }
+    }
+    const float *in = w.w_in + b * w.wi_batch + h * w.wi_head + j;
+    float *out = w.w_out + b * w.wo_batch + h * w.wo_head + j;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (j + i < w.Tk) out[i] = in[i] + (j + i < nk ? sum[i] : 0.f);
+}
+template <typename T>
+__global__ __launch_bounds__(kHeadsThreads) void combine_scored_kernel(AttendArgs a, WeightArgs w, int slots, int rows) {
+    if ((int)blockIdx.x < rows) combine_row<T>(a, slots, blockIdx.x);
+    else add_weights(w, blockIdx.x - rows);
 }
 
 template <typename T, int DP>
@@ -598,10 +670,17 @@ hipError_t launch_attend(const AttendArgs &a, int dtype, hipStream_t s) {
 }
 
 hipError_t launch_combine(const AttendArgs &a, int slots, int dtype, hipStream_t s) {
-    const long rows = (long)a.B * a.Tq * a.Hq;
-    const unsigned grid = (unsigned)((rows + 7) / 8);
+    const unsigned grid = (unsigned)((long)a.B * a.Tq * a.Hq);
     if (dtype == SDPA_BF16) heads::combine_kernel<__bf16><<<grid, heads::kHeadsThreads, 0, s>>>(a, slots);
     else heads::combine_kernel<float><<<grid, heads::kHeadsThreads, 0, s>>>(a, slots);
+    return hipGetLastError();
+}
+
+hipError_t launch_combine_scored(const AttendArgs &a, const WeightArgs &w, int slots, int dtype, hipStream_t s) {
+    const int rows = slots > 1 ? a.B * a.Tq * a.Hq : 0;
+    const unsigned grid = (unsigned)(rows + a.B * a.Hkv * ((a.Tk + 1023) / 1024));
+    if (dtype == SDPA_BF16) heads::combine_scored_kernel<__bf16><<<grid, heads::kHeadsThreads, 0, s>>>(a, w, slots, rows);
+    else heads::combine_scored_kernel<float><<<grid, heads::kHeadsThreads, 0, s>>>(a, w, slots, rows);
     return hipGetLastError();
 }
 
