@@ -80,7 +80,7 @@ struct EvictArgs {
     const int *lens;
     int *lens_out, *kept;
     int B, Tk, H, Dk, Dv, budget, sinks, recent, elem;
-    int vec_k, vec_v;
+    int vec;                          // rows in 16-byte pieces
 };
 
 hipError_t launch_attend(const AttendArgs &a, int dtype, hipStream_t s);

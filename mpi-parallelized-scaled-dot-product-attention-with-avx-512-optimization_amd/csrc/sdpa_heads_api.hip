@@ -185,8 +185,8 @@ int check_evict(const sdpa_heads *a) {
     if (repeats(a->k_out, a->batch, a->budget, a->kv_heads) || repeats(a->v_out, a->batch, a->budget, a->kv_heads))
         return SDPA_EINVAL;
     // (a workgroup moves 1024 pieces of at least one element, and one of 1024 threads selects for a head)
-    const double units = (double)a->budget * (a->dk > a->dv ? a->dk : a->dv), groups = (double)a->batch * a->kv_heads;
-    if (groups * (units / 1024 + 1) > kMaxGroups || groups > kMaxGroups / 4) return SDPA_EUNSUP;
+    const double units = (double)a->budget * (a->dk + a->dv), groups = (double)a->batch * a->kv_heads;
+    if (groups * (units / 1024 + 2) > kMaxGroups || groups > kMaxGroups / 4) return SDPA_EUNSUP;
     return SDPA_OK;
 }
 
@@ -335,8 +335,8 @@ int sdpa_dev_evict_cache(const struct sdpa_heads *a, void *workspace, size_t wor
     x.B = a->batch; x.Tk = a->kv_tokens; x.H = a->kv_heads; x.Dk = a->dk; x.Dv = a->dv;
     x.budget = a->budget; x.sinks = a->sinks; x.recent = a->recent;
     x.elem = elem_bytes(a->dtype);
-    x.vec_k = rows_vec(a->k, a->dk, a->dtype) && rows_vec(a->k_out, a->dk, a->dtype);
-    x.vec_v = rows_vec(a->v, a->dv, a->dtype) && rows_vec(a->v_out, a->dv, a->dtype);
+    x.vec = rows_vec(a->k, a->dk, a->dtype) && rows_vec(a->k_out, a->dk, a->dtype) && rows_vec(a->v, a->dv, a->dtype) &&
+            rows_vec(a->v_out, a->dv, a->dtype);
     HIP_TRY(launch_evict(x, (hipStream_t)stream));
     return SDPA_OK;
 }

@@ -476,58 +476,50 @@ __global__ __launch_bounds__(kHeadsThreads) void backward_join_kernel(BackwardAr
     }
 }
 
-// ---- the weights of every key: 128 keys to a workgroup ------------------------------------------------------------------------
-// w_out_j = w_in_j + sum_i exp(s_ij - lse_i): the first half of the dK / dV walk, with column sums in place of the products.
-template <typename T, int DP>
+// ---- the weights of every key: 32 KW keys to a workgroup --------------------------------------------------------------------------
+// w_out_j = w_in_j + sum_i exp(s_ij - lse_i): the first half of the dK / dV walk, with column sums in place of the products.  KW waves lie
+// along the keys, 4 / KW take the row blocks in turn; fragments come straight from memory (Q stays in the L2), no barriers in the loop.
+template <typename T, int DP, int KW>
 __global__ __launch_bounds__(kHeadsThreads) void weights_kernel(WeightArgs a, int G, int blocks) {
-    using TL = Tile<T, DP>;
-    constexpr int BQ = 32, STEPS = DP / Ops<T>::kStep;
-    __shared__ __attribute__((aligned(1024))) char lq[BQ * TL::kRowBytes];
-    __shared__ float llse[BQ];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int STEPS = DP / Ops<T>::kStep, PHASES = 4 / KW;
+    __shared__ float part[4][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = xcd_place(blockIdx.x, gridDim.x);
-    const int k0 = (id % blocks) * 128, j = k0 + wave * 32 + (lane & 31);
+    const int k0 = (id % blocks) * 32 * KW, j = k0 + wave % KW * 32 + (lane & 31);
     id /= blocks;
     const int h = id % a.Hkv, b = id / a.Hkv;
     const int nq = clamp_len(a.q_lens, b, a.Tq), nk = clamp_len(a.kv_lens, b, a.Tk);
-    const int everything = 1 << 30;
-    const SeenBy tok = seen_by(j, nq, nk, everything, 0), by = {tok.lo * G, tok.hi * G};
+    const SeenBy tok = seen_by(j, nq, nk, 1 << 30, 0), by = {tok.lo * G, tok.hi * G};
     float sum = 0.f;
     if (k0 < nk) {
-        const int first = max(0, k0 - (nk - nq)) * G;
-        const int r_end = nq * G;
         typename Ops<T>::Frag kf[STEPS];
         load_row<T, DP>(kf, row_at(a.k, b, j, h, sizeof(T)), a.Dk, j < nk, a.vec, lane);
-        LaneMap<T, DP> map;
-        map.init(lane);
-        const unsigned aq = lds_address(lq) + map.rows;
-        for (int r0 = first / BQ * BQ; r0 < r_end; r0 += BQ) {
-            __syncthreads();
-            for (int c = tid; c < BQ * TL::kChunks; c += kHeadsThreads) {
-                const int r = r0 + c / TL::kChunks;
-                u32x4 x = {0, 0, 0, 0};
-                if (r < r_end) {
-                    const int t = r / G, hq = h * G + r - t * G;
-                    x = load_chunk((const T *)row_at(a.q, b, t, hq, sizeof(T)), (c % TL::kChunks) * Ops<T>::kVec, a.Dk, a.vec);
-                }
-                *reinterpret_cast<u32x4 *>(lq + TL::chunk(c / TL::kChunks, c % TL::kChunks)) = x;
-            }
-            if (tid < BQ && r0 + tid < r_end) {
-                const int r = r0 + tid, t = r / G, hq = h * G + r - t * G;
-                llse[tid] = a.lse[((long)b * a.Hq + hq) * a.Tq + t] * kLog2e;
-            }
-            __syncthreads();
+        const int r_end = nq * G, first = max(0, k0 - (nk - nq)) * G / 32 + wave / KW;
+        for (int r0 = first * 32; r0 < r_end; r0 += 32 * PHASES) {
+            const int r = r0 + (lane & 31), t = r / G, hq = h * G + r - t * G;
+            typename Ops<T>::Frag qf[STEPS];
+            load_row<T, DP>(qf, row_at(a.q, b, t, hq, sizeof(T)), a.Dk, r < r_end, a.vec, lane);
+            const float lse2 = r < r_end ? a.lse[((long)b * a.Hq + hq) * a.Tq + t] * kLog2e : 0.f;
             f32x16 s = {};
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(aq, 0, i), kf[i], s);
+            for (int i = 0; i < STEPS; ++i)
+                if (sizeof(T) == 2 || i * Ops<T>::kStep < a.Dk) s = Ops<T>::mma(qf[i], kf[i], s);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int rl = row_of(i, lane >> 5), r = r0 + rl;
-                if (r >= by.lo && r < by.hi) sum += __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - llse[rl]);
+                const int at = row_of(i, lane >> 5);
+                const float ref = __shfl(lse2, at);
+                if (r0 + at >= by.lo && r0 + at < by.hi) sum += __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - ref);
             }
         }
     }
     sum = half_sum(sum);
+    if (PHASES > 1) {
+        if (lane < 32) part[wave][lane] = sum;
+        __syncthreads();
+        if (wave >= KW) return;
+#pragma unroll
+        for (int p = 1; p < PHASES; ++p) sum += part[wave + p * KW][lane & 31];
+    }
     if (lane < 32 && j < a.Tk) {
         const float w = a.w_in[b * a.wi_batch + h * a.wi_head + j];
         a.w_out[b * a.wo_batch + h * a.wo_head + j] = w + sum;
@@ -563,8 +555,11 @@ void backward(const BackwardArgs &a, hipStream_t s) {
 
 template <typename T, int DP>
 void weights(const WeightArgs &a, hipStream_t s) {
-    const int blocks = (a.Tk + 127) / 128;
-    if (blocks > 0) weights_kernel<T, DP><<<a.B * a.Hkv * blocks, kHeadsThreads, 0, s>>>(a, a.Hq / a.Hkv, blocks);
+    if (a.Tk == 0) return;
+    // 128 keys to a workgroup read Q a quarter as often; while they do not fill the chip the rows are split instead
+    const int G = a.Hq / a.Hkv, wide = (a.Tk + 127) / 128, narrow = (a.Tk + 31) / 32;
+    if ((long)a.B * a.Hkv * wide >= 512) weights_kernel<T, DP, 4><<<a.B * a.Hkv * wide, kHeadsThreads, 0, s>>>(a, G, wide);
+    else weights_kernel<T, DP, 1><<<a.B * a.Hkv * narrow, kHeadsThreads, 0, s>>>(a, G, narrow);
 }
 
 }  // namespace

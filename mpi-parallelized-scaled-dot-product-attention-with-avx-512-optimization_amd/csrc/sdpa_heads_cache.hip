@@ -14,27 +14,32 @@ __device__ inline uint32_t order_key(float w) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// exclusive prefix count of `flag` over the workgroup's threads; `total` = all of them.  `sums`: one word a wave.
-__device__ inline int block_rank(bool flag, int *sums, int *total) {
+// exclusive prefix sum of `count` over the workgroup's threads.  `sums`: one word a wave.
+__device__ inline int block_before(int count, int *sums) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t mask = __ballot(flag);
-    if (lane == 0) sums[wave] = __popcll(mask);
-    __syncthreads();
-    int before = 0, all = 0;
+    int scan = count;
 #pragma unroll
-    for (int w = 0; w < kSelectThreads / 64; ++w) {
-        const int c = sums[w];
-        before += w < wave ? c : 0;
-        all += c;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(scan, d);
+        if (lane >= d) scan += up;
     }
+    if (lane == 63) sums[wave] = scan;
     __syncthreads();
-    *total = all;
-    return before + __popcll(mask & ((1ull << lane) - 1));
+    int before = scan - count;
+#pragma unroll
+    for (int w = 0; w < kSelectThreads / 64; ++w) before += w < wave ? sums[w] : 0;
+    __syncthreads();
+    return before;
 }
 
 // One workgroup per (sequence, key head).  The c-th greatest weight is found digit by digit (four passes of 8 bits over a
-// histogram in LDS, integer counts only); then one ordered pass numbers what stays.
+// histogram in LDS, integer counts only); then every thread numbers what stays of its own run of keys, behind two prefix sums over
+// the threads.  The weights are read once, into LDS (LOCAL: up to kSelectLocal keys); 8192 keys of 128 heads take 9 us, of which the
+// single reading is 2 -- reading them again in every pass took 26.
+constexpr int kSelectLocal = 32768;
+template <bool LOCAL>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
+    extern __shared__ float local[];
     __shared__ int hist[256];
     __shared__ int sums[kSelectThreads / 64];
     __shared__ uint32_t s_prefix;
@@ -45,19 +50,30 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
     float *wo = a.w_out + b * a.wo_batch + h * a.wo_head;
     int *kept = a.kept + ((long)b * a.H + h) * a.budget;
     if (h == 0 && tid == 0) a.lens_out[b] = live;
-    const int lo = a.sinks, hi = n - a.recent;
-    uint32_t bar = 0;                                 // weights above it stay, and the first `ties` equal to it
-    int ties = 1 << 30;
-    if (n > a.budget) {
-        const int want = a.budget - a.sinks - a.recent;
+    for (int i = live + tid; i < a.budget; i += kSelectThreads) { kept[i] = -1; wo[i] = 0.f; }
+    if (n <= a.budget) {
+        for (int j = tid; j < n; j += kSelectThreads) { kept[j] = j; wo[j] = w[j]; }
+        return;
+    }
+    if (LOCAL) {
+#pragma unroll 8
+        for (int j = tid; j < n; j += kSelectThreads) local[j] = w[j];
+        __syncthreads();
+    }
+    auto weight = [&](int j) { return LOCAL ? local[j] : w[j]; };
+    const int lo = a.sinks, hi = n - a.recent, want = a.budget - a.sinks - a.recent;
+    uint32_t bar = 0xffffffffu;                       // weights above it stay, and the first `ties` equal to it (no weight has that key)
+    int ties = 0;
+    if (want > 0) {
         uint32_t prefix = 0;
         int left = want;                              // how many of the current candidates stay
-        for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
             if (tid < 256) hist[tid] = 0;
             __syncthreads();
+#pragma unroll 4
             for (int j = lo + tid; j < hi; j += kSelectThreads) {
-                const uint32_t key = order_key(w[j]);
-                if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+                const uint32_t key = order_key(weight(j));
+                if (shift == 24 || (key >> ((shift + 8) & 31)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
             }
             __syncthreads();
             if (tid < 64) {                           // the digit in which the left-th greatest candidate lies
@@ -84,76 +100,87 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
             prefix = s_prefix;
             left = s_left;
         }
-        if (want == 0) { bar = 0xffffffffu; ties = 0; }          // (no weight has that key)
-        else { bar = prefix; ties = left; }
+        bar = prefix;
+        ties = left;
     }
-    int out = 0, equal = 0;
-    for (int base = 0; base < n; base += kSelectThreads) {
-        const int j = base + tid;
-        const float x = j < n ? w[j] : 0.f;
-        bool stays = j < n;
-        if (n > a.budget) {
-            const bool fixed = j < lo || j >= hi;
-            const uint32_t key = order_key(x);
-            const bool tie = j < n && !fixed && key == bar;
-            int total;
-            const int rank = block_rank(tie, sums, &total);
-            stays = j < n && (fixed || key > bar || (tie && equal + rank < ties));
-            equal += total;
-        }
-        int total;
-        const int at = out + block_rank(stays, sums, &total);
-        if (stays) { kept[at] = j; wo[at] = x; }
-        out += total;
-    }
-    for (int i = live + tid; i < a.budget; i += kSelectThreads) { kept[i] = -1; wo[i] = 0.f; }
+    // a thread's run of keys (an odd number of them: the threads' reads fall into different banks)
+    const int run = ((n + kSelectThreads - 1) / kSelectThreads) | 1, j0 = min(tid * run, n), j1 = min(j0 + run, n);
+    int equal = 0;
+    for (int j = max(j0, lo); j < min(j1, hi); ++j) equal += order_key(weight(j)) == bar ? 1 : 0;
+    equal = block_before(equal, sums);
+    auto stays = [&](int j, int &rank) {              // `rank`: ties so far
+        if (j < lo || j >= hi) return true;
+        const uint32_t key = order_key(weight(j));
+        return key > bar || (key == bar && rank++ < ties);
+    };
+    int count = 0, rank = equal;
+    for (int j = j0; j < j1; ++j) count += stays(j, rank) ? 1 : 0;
+    int at = block_before(count, sums);
+    rank = equal;
+    for (int j = j0; j < j1; ++j)
+        if (stays(j, rank)) { kept[at] = j; wo[at] = weight(j); ++at; }
 }
 
-// `UNIT`-byte pieces of rows: a thread moves one piece of K or V
+// The rows that stay, in pieces of one U: 4 pieces a thread.  K's workgroups come first, then V's.  At the rate of a copy.
+struct GatherSide { sdpa_tensor in, out; int pieces, blocks; };
 template <typename U>
-__global__ __launch_bounds__(kHeadsThreads) void gather_kernel(EvictArgs a, sdpa_tensor in, sdpa_tensor out, int pieces, int blocks) {
+__global__ __launch_bounds__(kHeadsThreads) void gather_kernel(EvictArgs a, GatherSide k, GatherSide v) {
     int id = blockIdx.x;
-    const int part = id % blocks;
-    id /= blocks;
+    const int k_blocks = a.B * a.H * k.blocks;
+    const bool is_v = id >= k_blocks;
+    const GatherSide &g = is_v ? v : k;
+    if (is_v) id -= k_blocks;
+    const int part = id % g.blocks;
+    id /= g.blocks;
     const int h = id % a.H, b = id / a.H;
     const int *kept = a.kept + ((long)b * a.H + h) * a.budget;
-    const U *src = reinterpret_cast<const U *>((const char *)in.data + (b * in.batch + h * in.head) * a.elem);
-    U *dst = reinterpret_cast<U *>((char *)out.data + (b * out.batch + h * out.head) * a.elem);
-    const long in_row = in.token * a.elem / (long)sizeof(U), out_row = out.token * a.elem / (long)sizeof(U);
-    const int per = kHeadsThreads * 4;
+    const U *src = reinterpret_cast<const U *>((const char *)g.in.data + (b * g.in.batch + h * g.in.head) * a.elem);
+    U *dst = reinterpret_cast<U *>((char *)g.out.data + (b * g.out.batch + h * g.out.head) * a.elem);
+    const long in_row = g.in.token * a.elem / (long)sizeof(U), out_row = g.out.token * a.elem / (long)sizeof(U);
+    U x[4];
+    int slot[4], c[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const long i = (long)part * per + k * kHeadsThreads + threadIdx.x;
-        const int slot = (int)(i / pieces), c = (int)(i - (long)slot * pieces);
-        if (slot >= a.budget) return;
-        const int j = kept[slot];
-        U v = {};
-        if (j >= 0) v = src[j * in_row + c];
-        dst[slot * out_row + c] = v;
+    for (int i = 0; i < 4; ++i) {
+        const long at = (long)part * (kHeadsThreads * 4) + i * kHeadsThreads + threadIdx.x;
+        slot[i] = (int)(at / g.pieces);
+        c[i] = (int)(at - (long)slot[i] * g.pieces);
+        const int j = slot[i] < a.budget ? kept[slot[i]] : -1;
+        x[i] = U{};
+        if (j >= 0) x[i] = src[j * in_row + c[i]];
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (slot[i] < a.budget) dst[slot[i] * out_row + c[i]] = x[i];
 }
 
-template <typename U>
-void gather(const EvictArgs &a, const sdpa_tensor &in, const sdpa_tensor &out, int dim, hipStream_t s) {
-    const int pieces = dim * a.elem / (int)sizeof(U);
-    const int blocks = (int)(((long)a.budget * pieces + kHeadsThreads * 4 - 1) / (kHeadsThreads * 4));
-    gather_kernel<U><<<a.B * a.H * blocks, kHeadsThreads, 0, s>>>(a, in, out, pieces, blocks);
-}
-
-void gather_any(const EvictArgs &a, const sdpa_tensor &in, const sdpa_tensor &out, int dim, int vec, hipStream_t s) {
-    if (vec) gather<u32x4>(a, in, out, dim, s);
-    else if (a.elem == 4) gather<uint32_t>(a, in, out, dim, s);
-    else gather<uint16_t>(a, in, out, dim, s);
+template <typename U> void gather(const EvictArgs &a, hipStream_t s) {
+    auto side = [&](const sdpa_tensor &in, const sdpa_tensor &out, int dim) {
+        GatherSide g = {in, out, dim * a.elem / (int)sizeof(U), 0};
+        g.blocks = (int)(((long)a.budget * g.pieces + kHeadsThreads * 4 - 1) / (kHeadsThreads * 4));
+        return g;
+    };
+    const GatherSide k = side(a.k, a.k_out, a.Dk), v = side(a.v, a.v_out, a.Dv);
+    gather_kernel<U><<<a.B * a.H * (k.blocks + v.blocks), kHeadsThreads, 0, s>>>(a, k, v);
 }
 
 }  // namespace
 }  // namespace heads
 
 hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
-    heads::select_kernel<<<a.B * a.H, heads::kSelectThreads, 0, s>>>(a);
+    const int groups = a.B * a.H;
+    if (a.Tk <= heads::kSelectLocal) {
+        const size_t bytes = (size_t)a.Tk * 4;
+        static const hipError_t wide = hipFuncSetAttribute((const void *)heads::select_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                           heads::kSelectLocal * 4);
+        if (wide != hipSuccess) return wide;
+        heads::select_kernel<true><<<groups, heads::kSelectThreads, bytes, s>>>(a);
+    } else {
+        heads::select_kernel<false><<<groups, heads::kSelectThreads, 0, s>>>(a);
+    }
     if (a.budget == 0) return hipGetLastError();
-    heads::gather_any(a, a.k, a.k_out, a.Dk, a.vec_k, s);
-    heads::gather_any(a, a.v, a.v_out, a.Dv, a.vec_v, s);
+    if (a.vec) heads::gather<heads::u32x4>(a, s);
+    else if (a.elem == 4) heads::gather<uint32_t>(a, s);
+    else heads::gather<uint16_t>(a, s);
     return hipGetLastError();
 }
 

@@ -47,7 +47,8 @@ __device__ inline void scores(f32x16 *s, const typename Ops<T>::Frag *q, unsigne
     for (int n = 0; n < NB; ++n) {
         s[n] = f32x16{};
 #pragma unroll
-        for (int i = 0; i < DP / Ops<T>::kStep; ++i) s[n] = Ops<T>::mma(read_rows<T, DP>(at, n, i), q[i], s[n]);
+        for (int i = 0; i < DP / Ops<T>::kStep; ++i)
+            s[n] = Ops<T>::mma(read_rows<T, DP>(at, n, i), q[i], s[n]);
     }
 }
 
@@ -529,13 +530,15 @@ __global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, in
 }
 
 // ---- the join of the slots: the merge of partial triples ------------------------------------------------------------
-// A workgroup to a row: 32 lanes to its columns, eight groups of lanes to the slots.  (Eight rows to a workgroup, each walking its slots one
-// after the other, took 34 us for 2048 rows of 34 slots; the loads of a row are now eight deep.)
-template <typename T>
-__device__ inline void combine_row(const AttendArgs &a, int slots, long r) {
+// 32 lanes to a row's columns.  GROUPS = 8: a workgroup to a row, its eight groups of lanes to the slots in turn (2048 rows of 34 slots take
+// 12 us, against 34 us with GROUPS = 1).  GROUPS = 1: eight rows to a workgroup (13986 rows of 5 slots: 7 us against 22 us).
+template <typename T, int GROUPS>
+__device__ inline void combine_row(const AttendArgs &a, int slots, long block) {
     __shared__ f32x4 sum[8][64];
     const long rows = (long)a.B * a.Tq * a.Hq;
-    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, group = GROUPS == 8 ? threadIdx.x >> 5 : 0;
+    const long r = GROUPS == 8 ? block : block * 8 + (threadIdx.x >> 5);
+    if (GROUPS == 1 && r >= rows) return;
     float m = kNegInf;
     for (int s = 0; s < slots; s += 32) {
         float2 ml = make_float2(kNegInf, 0.f);
@@ -554,7 +557,7 @@ __device__ inline void combine_row(const AttendArgs &a, int slots, long r) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) l += __shfl_xor(l, d);
     f32x4 acc[2] = {};
-    for (int s = group; s < slots; s += 8) {
+    for (int s = group; s < slots; s += GROUPS) {
         const float2 ml = a.stat[s * rows + r];
         if (ml.y == 0.f) continue;                       // (an empty slot was not written)
         const float w = __builtin_amdgcn_exp2f(ml.x - ref);
@@ -571,23 +574,33 @@ __device__ inline void combine_row(const AttendArgs &a, int slots, long r) {
             }
         }
     }
-    sum[group][lane] = acc[0];
-    sum[group][32 + lane] = acc[1];
-    __syncthreads();
-    if (threadIdx.x >= 64) return;
-    f32x4 v = sum[0][threadIdx.x];
-#pragma unroll
-    for (int g = 1; g < 8; ++g) v += sum[g][threadIdx.x];
     RowId x;
-    const int hq = (int)(r % a.Hq), d = threadIdx.x * 4;
+    const int hq = (int)(r % a.Hq);
     const long bt = r / a.Hq;
     x.b = (int)(bt / a.Tq); x.t = (int)(bt - (long)x.b * a.Tq); x.g = 0; x.live = true;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (d < a.Dv) store4<T>(a, x, hq, d, v * inv);
-    if (threadIdx.x == 0) a.lse[((long)x.b * a.Hq + hq) * a.Tq + x.t] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+    if (lane == 0 && group == 0) a.lse[((long)x.b * a.Hq + hq) * a.Tq + x.t] = l == 0.f ? kNegInf : (m + __log2f(l)) * kLn2;
+    if (GROUPS == 1) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (k * 128 + lane * 4 < a.Dv) store4<T>(a, x, hq, k * 128 + lane * 4, acc[k] * inv);
+        return;
+    }
+    sum[group][lane] = acc[0];
+    sum[group][32 + lane] = acc[1];
+    __syncthreads();
+    const int d = threadIdx.x * 4;
+    if (d >= a.Dv) return;
+    f32x4 v = sum[0][threadIdx.x];
+#pragma unroll
+    for (int g = 1; g < 8; ++g) v += sum[g][threadIdx.x];
+    store4<T>(a, x, hq, d, v * inv);
 }
-template <typename T>
-__global__ __launch_bounds__(kHeadsThreads) void combine_kernel(AttendArgs a, int slots) { combine_row<T>(a, slots, blockIdx.x); }
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(kHeadsThreads) void combine_kernel(AttendArgs a, int slots) { combine_row<T, GROUPS>(a, slots, blockIdx.x); }
+// what the two ways measured above say: a workgroup to a row where its slots are many or the rows few
+inline int combine_groups(long rows, int slots) { return slots > 8 || rows < 2048 ? 8 : 1; }
+inline unsigned combine_blocks(long rows, int groups) { return (unsigned)(groups == 8 ? rows : (rows + 7) / 8); }
 
 // w_out_j = w_in_j + sum over the rows of exp2(s_j - lse), from the kept scores: 1024 keys of a head to a workgroup
 __device__ inline void add_weights(const WeightArgs &w, int block) {
@@ -630,10 +643,10 @@ __device__ inline void add_weights(const WeightArgs &w, int block) {
     for (int i = 0; i < 4; ++i)
         if (j + i < w.Tk) out[i] = in[i] + (j + i < nk ? sum[i] : 0.f);
 }
-template <typename T>
-__global__ __launch_bounds__(kHeadsThreads) void combine_scored_kernel(AttendArgs a, WeightArgs w, int slots, int rows) {
-    if ((int)blockIdx.x < rows) combine_row<T>(a, slots, blockIdx.x);
-    else add_weights(w, blockIdx.x - rows);
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(kHeadsThreads) void combine_scored_kernel(AttendArgs a, WeightArgs w, int slots, int blocks) {
+    if ((int)blockIdx.x < blocks) combine_row<T, GROUPS>(a, slots, blockIdx.x);
+    else add_weights(w, blockIdx.x - blocks);
 }
 
 template <typename T, int DP>
@@ -669,18 +682,34 @@ hipError_t launch_attend(const AttendArgs &a, int dtype, hipStream_t s) {
     return hipGetLastError();
 }
 
+namespace heads {
+namespace {
+template <typename T> void combine(const AttendArgs &a, int slots, hipStream_t s) {
+    const long rows = (long)a.B * a.Tq * a.Hq;
+    const int groups = combine_groups(rows, slots);
+    const unsigned grid = combine_blocks(rows, groups);
+    if (groups == 8) combine_kernel<T, 8><<<grid, kHeadsThreads, 0, s>>>(a, slots);
+    else combine_kernel<T, 1><<<grid, kHeadsThreads, 0, s>>>(a, slots);
+}
+template <typename T> void combine_scored(const AttendArgs &a, const WeightArgs &w, int slots, hipStream_t s) {
+    const long rows = slots > 1 ? (long)a.B * a.Tq * a.Hq : 0;
+    const int groups = combine_groups(rows, slots);
+    const unsigned blocks = combine_blocks(rows, groups), grid = blocks + (unsigned)(a.B * a.Hkv * ((a.Tk + 1023) / 1024));
+    if (groups == 8) combine_scored_kernel<T, 8><<<grid, kHeadsThreads, 0, s>>>(a, w, slots, (int)blocks);
+    else combine_scored_kernel<T, 1><<<grid, kHeadsThreads, 0, s>>>(a, w, slots, (int)blocks);
+}
+}  // namespace
+}  // namespace heads
+
 hipError_t launch_combine(const AttendArgs &a, int slots, int dtype, hipStream_t s) {
-    const unsigned grid = (unsigned)((long)a.B * a.Tq * a.Hq);
-    if (dtype == SDPA_BF16) heads::combine_kernel<__bf16><<<grid, heads::kHeadsThreads, 0, s>>>(a, slots);
-    else heads::combine_kernel<float><<<grid, heads::kHeadsThreads, 0, s>>>(a, slots);
+    if (dtype == SDPA_BF16) heads::combine<__bf16>(a, slots, s);
+    else heads::combine<float>(a, slots, s);
     return hipGetLastError();
 }
 
 hipError_t launch_combine_scored(const AttendArgs &a, const WeightArgs &w, int slots, int dtype, hipStream_t s) {
-    const int rows = slots > 1 ? a.B * a.Tq * a.Hq : 0;
-    const unsigned grid = (unsigned)(rows + a.B * a.Hkv * ((a.Tk + 1023) / 1024));
-    if (dtype == SDPA_BF16) heads::combine_scored_kernel<__bf16><<<grid, heads::kHeadsThreads, 0, s>>>(a, w, slots, rows);
-    else heads::combine_scored_kernel<float><<<grid, heads::kHeadsThreads, 0, s>>>(a, w, slots, rows);
+    if (dtype == SDPA_BF16) heads::combine_scored<__bf16>(a, w, slots, s);
+    else heads::combine_scored<float>(a, w, slots, s);
     return hipGetLastError();
 }
 
