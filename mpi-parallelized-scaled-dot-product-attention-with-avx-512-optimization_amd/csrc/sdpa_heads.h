@@ -25,6 +25,10 @@ inline bool rows_vec(const sdpa_tensor &t, int dim, int dtype) {
     return ((bad | (long)(size_t)t.data) & 15) == 0 && t.token < (1 << 21);
 }
 
+// the few-rows kernel: bytes of a 32-key K and V tile, and the waves of its wide form (128 KiB of LDS)
+constexpr int few_pair_bytes(int pad, int elem) { return 2 * 32 * pad * elem; }
+constexpr int few_wide_waves(int pad, int elem) { return 131072 / few_pair_bytes(pad, elem) < 8 ? 131072 / few_pair_bytes(pad, elem) : 8; }
+
 // One launch over one set of keys: its queries, where its rows go, and what they may see.
 struct AttendArgs {
     sdpa_tensor q, k, v, out;
@@ -37,6 +41,7 @@ struct AttendArgs {
     int slot0, splits;                // this launch's slots
     int B, Tq, Tk, Hq, Hkv, Dk, Dv;
     int window, sinks;
+    int wide;                         // few rows: one workgroup of more waves to a head, no splits
     int shared;                       // 1 = one set of keys for the whole batch, all of them visible (a prefix)
     int vec, vec_out;                 // 16-byte loads of q, k, v / whole 4-element stores of out
     int q_sign;                       // the softmax scale's sign: applied to the queries

@@ -49,10 +49,12 @@ bool empty(const sdpa_heads *a) { return a->batch == 0 || a->q_tokens == 0; }
 // How many workgroups share the keys of a row tile.  A launch wants about two workgroups on each of the 256 CUs; a split costs a
 // partial row (4 * dv + 8 bytes written and read) per query row and needs keys enough to be worth its start: one 32-key tile
 // for each of its waves where they take the keys in turn, a tile of 64 where they share it.
-int pick_splits(long groups, long rows, long keys) {
+int pick_splits(int dtype, long groups, long rows, long keys) {
     const long tiles = rows <= kFewRows ? 1 : ceil_div(rows, 128);
     const long have = groups * tiles;
-    long want = ceil_div(512, have < 1 ? 1 : have);
+    // (few rows: measured flat between 512 and 768 workgroups.  Many rows: never a second, mostly empty round; fp32 workgroups are bound by
+    // their matrix instructions and gain nothing from a neighbour on their CU.)
+    long want = rows <= kFewRows ? ceil_div(512, have < 1 ? 1 : have) : (dtype == SDPA_BF16 ? 512 : 256) / (have < 1 ? 1 : have);
     const long most = ceil_div(keys, rows <= kFewRows ? 128 : 64);
     if (want > most) want = most;
     if (want > kMaxSplits) want = kMaxSplits;
@@ -81,7 +83,14 @@ long keys_seen(const sdpa_heads *a, long rows) {
     return w < a->kv_tokens ? w : a->kv_tokens;
 }
 
+// A call so small that one workgroup a head does it: at most four tiles of 32 keys for each of its waves, and a CU for every head.  (One
+// launch instead of two.)
+bool one_workgroup(const sdpa_heads *a, long groups, long rows, long keys) {
+    return rows <= kFewRows && groups <= 256 && ceil_div(keys, 32) <= 4 * few_wide_waves(heads_pad(a->dk, a->dv), elem_bytes(a->dtype));
+}
+
 struct Slots {
+    bool wide;                    // few rows: the form with one workgroup a head
     int own, prefix;              // slots of the sequences' own keys and of the prefix
     long rows, part, bytes;       // bytes of the slots, and of everything
     long score_ld;                // kept scores (attention_scored over few rows): their row, 0 = none
@@ -97,7 +106,9 @@ struct Slots {
 Slots plan_window(const sdpa_heads *a, bool scored) {
     Slots s = {};
     const long rows = (long)a->q_tokens * (a->q_heads / a->kv_heads);
-    s.own = pick_splits((long)a->batch * a->kv_heads, rows, keys_seen(a, rows));
+    const long groups = (long)a->batch * a->kv_heads, keys = keys_seen(a, rows);
+    if (one_workgroup(a, groups, rows, keys)) { s.wide = true; s.own = 1; }
+    else s.own = pick_splits(a->dtype, groups, rows, keys);
     s.size(a, scored);
     return s;
 }
@@ -105,8 +116,8 @@ Slots plan_window(const sdpa_heads *a, bool scored) {
 Slots plan_prefix(const sdpa_heads *a) {
     Slots s = {};
     const long rows = (long)a->q_tokens * (a->q_heads / a->kv_heads);
-    s.own = pick_splits((long)a->batch * a->kv_heads, rows, a->kv_tokens);
-    s.prefix = a->prefix_tokens > 0 ? pick_splits(a->kv_heads, rows * a->batch, a->prefix_tokens) : 0;
+    s.own = pick_splits(a->dtype, (long)a->batch * a->kv_heads, rows, a->kv_tokens);
+    s.prefix = a->prefix_tokens > 0 ? pick_splits(a->dtype, a->kv_heads, rows * a->batch, a->prefix_tokens) : 0;
     s.size(a, false);
     return s;
 }
@@ -137,6 +148,7 @@ int check_forward(const sdpa_heads *a) {
 int run_own(const sdpa_heads *a, const Slots &s, void *workspace, hipStream_t st) {
     AttendArgs x = attend_args(a);
     x.splits = s.own;
+    x.wide = s.wide;
     carve(x, s, workspace);
     HIP_TRY(launch_attend(x, a->dtype, st));
     if (x.part) HIP_TRY(launch_combine(x, s.own, a->dtype, st));
@@ -308,6 +320,7 @@ int sdpa_dev_attention_scored(const struct sdpa_heads *a, void *workspace, size_
     if (!empty(a) && s.score_ld > 0) {                   // (over few rows) the scores are kept, and the weights come with the join
         AttendArgs f = attend_args(&x);
         f.splits = s.own;
+        f.wide = s.wide;
         carve(f, s, workspace);
         f.scores = (float *)((char *)workspace + s.part);
         f.score_ld = s.score_ld;

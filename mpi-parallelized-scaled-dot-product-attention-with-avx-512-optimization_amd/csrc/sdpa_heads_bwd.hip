@@ -229,7 +229,7 @@ template <typename T, int DP> struct RowStager {
         }
     }
     __device__ void copy(char *tile, int block, int nq, const RowBlocks &rb, bool vec, int wave, int lane) const {
-#pragma unroll 1
+#pragma unroll 4
         for (int k = 0; k < kPieces; ++k) {
             const int ln = opaque(lane), r = row(wave, ln, k), blk = block + (r >> 5), i = r & 31, t = rb.token(blk, i);
             u32x4 x = {0, 0, 0, 0};

@@ -34,8 +34,8 @@ __device__ inline int block_before(int count, int *sums) {
 
 // One workgroup per (sequence, key head).  The c-th greatest weight is found digit by digit (four passes of 8 bits over a
 // histogram in LDS, integer counts only); then every thread numbers what stays of its own run of keys, behind two prefix sums over
-// the threads.  The weights are read once, into LDS (LOCAL: up to kSelectLocal keys); 8192 keys of 128 heads take 9 us, of which the
-// single reading is 2 -- reading them again in every pass took 26.
+// the threads.  The weights are read once, into LDS (LOCAL: up to kSelectLocal keys); 8192 keys of 128 heads take 19 us --
+// reading them again in every pass took 26 us.
 constexpr int kSelectLocal = 32768;
 template <bool LOCAL>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {

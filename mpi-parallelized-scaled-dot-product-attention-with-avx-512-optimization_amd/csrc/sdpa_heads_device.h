@@ -413,6 +413,7 @@ template <typename T, int DP, int ROWS, int WAVES> struct Stager {
     long token;                      // bytes between rows
     int dim;
     unsigned off[kKinds];            // lane offsets inside a tile
+    unsigned has;                    // bit k: off[k] is a chunk of the row, not of its padding
     __device__ static int row(int wave, int lane, int k) { return (((wave + k * WAVES) * 1024 + lane * 16) / TL::kRowBytes); }
     __device__ static int source(int wave, int lane, int k) {                 // the chunk of its row a lane asks for
         return (((wave + k * WAVES) * 64 + lane) % TL::kChunks) ^ TL::swz(row(wave, lane, k));
@@ -423,23 +424,32 @@ template <typename T, int DP, int ROWS, int WAVES> struct Stager {
         dim = d;
 #pragma unroll
         for (int k = 0; k < kKinds; ++k) off[k] = (unsigned)(row(wave, lane, k) * (int)token) + 16u * (unsigned)source(wave, lane, k);
+        has = 0;
+#pragma unroll
+        for (int k = 0; k < kKinds; ++k) has |= source(wave, lane, k) * Ops<T>::kVec < d ? 1u << k : 0u;
     }
     // asynchronous: 16-byte rows (a tile's offsets fit 32 bits).  -> true: exactly kPieces instructions are on their way
     __device__ bool dma(unsigned lds, int v0, const KeyList &l, int wave, int lane) const {
         const char *at = base + (long)l.key(v0) * token;
         lds += (unsigned)wave * 1024u;
-        if (dim == DP && v0 + ROWS <= l.n && (v0 >= l.s || v0 + ROWS <= l.s)) {
+        if (v0 + ROWS <= l.n && (v0 >= l.s || v0 + ROWS <= l.s)) {
             const long step = token * (kKinds * WAVES * 1024 / TL::kRowBytes);
+            if (dim == DP) {
 #pragma unroll
-            for (int k = 0; k < kPieces; ++k) lds_dma(at + k / kKinds * step, off[k % kKinds], lds + k * WAVES * 1024u);
-            return true;
+                for (int k = 0; k < kPieces; ++k) lds_dma(at + k / kKinds * step, off[k % kKinds], lds + k * WAVES * 1024u);
+                return true;
+            }
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k)
+                if ((has >> (k % kKinds)) & 1) lds_dma(at + k / kKinds * step, off[k % kKinds], lds + k * WAVES * 1024u);   // (the padding stays zero)
+            return false;
         } else {
             const int ln = opaque(lane), split = v0 < l.s && l.s < l.n ? l.s : l.n;     // entries of either side: a base each
             const char *above = base + (long)l.key(split < l.n ? split : v0) * token;
 #pragma unroll 1
             for (int k = 0; k < kPieces; ++k) {
                 const int r = row(wave, ln, k), c = source(wave, ln, k), v = v0 + r < l.n ? v0 + r : l.n - 1;
-                if (c * Ops<T>::kVec < dim) {                                            // (the padding stays zero)
+                if (c * Ops<T>::kVec < dim) {
                     if (v < split) lds_dma(at, (unsigned)((v - v0) * (int)token) + 16u * (unsigned)c, lds + k * WAVES * 1024u);
                     else lds_dma(above, (unsigned)((v - split) * (int)token) + 16u * (unsigned)c, lds + k * WAVES * 1024u);
                 }
@@ -449,7 +459,7 @@ template <typename T, int DP, int ROWS, int WAVES> struct Stager {
     }
     // element by element, for rows without 16-byte alignment
     __device__ void copy(char *tile, int v0, const KeyList &l, int wave, int lane) const {
-#pragma unroll 1
+#pragma unroll 4
         for (int k = 0; k < kPieces; ++k) {
             const int ln = opaque(lane), r = row(wave, ln, k), c = source(wave, ln, k), v = v0 + r < l.n ? v0 + r : l.n - 1;
             const T *src = reinterpret_cast<const T *>(base + (long)l.key(v) * token);

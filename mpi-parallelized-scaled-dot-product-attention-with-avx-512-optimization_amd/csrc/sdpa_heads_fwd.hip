@@ -408,15 +408,17 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
 // ---- few rows (single tokens): the waves share 32 rows and take the key tiles in turn ------------------------------------
 // Bound by the reading of the cache.  Every wave stages its own tiles of 32 keys (no barriers), the next one on its way by DMA while this
 // one is multiplied: 64 KiB in flight on a CU.  (fp32 tiles are bound by their matrix instructions and are not double-buffered.)
-template <typename T, int DP> struct FewShape {
-    static constexpr int kPair = 2 * 32 * DP * (int)sizeof(T);                              // a K and a V tile
-    static constexpr int kBufs = sizeof(T) == 2 || DP == 64 ? 2 : 1;
-    static constexpr int kWaves = kPair * kBufs * 4 <= 131072 ? 4 : 2;
+// WIDE: up to eight waves, for calls so small that one workgroup does the keys of a head and no join is launched.
+template <typename T, int DP, bool WIDE> struct FewShape {
+    static constexpr int kPair = few_pair_bytes(DP, sizeof(T));                              // a K and a V tile
+    static constexpr int kWaves = WIDE ? few_wide_waves(DP, sizeof(T)) : kPair * 8 <= 131072 || (sizeof(T) == 4 && DP == 128) ? 4 : 2;
+    static constexpr int kBufs = (sizeof(T) == 2 || DP == 64) && kPair * 2 * kWaves <= 131072 ? 2 : 1;
 };
-template <typename T, int DP, int WAVES, bool VEC>
-__global__ __launch_bounds__(WAVES * 64) void attend_few_kernel(AttendArgs a, int rows, int G) {
+template <typename T, int DP, bool WIDE, bool VEC>
+__global__ __launch_bounds__((FewShape<T, DP, WIDE>::kWaves * 64)) void attend_few_kernel(AttendArgs a, int rows, int G) {
     using TL = Tile<T, DP>;
-    constexpr int TILE = 32 * TL::kRowBytes, NBUF = FewShape<T, DP>::kBufs, WAVE_BYTES = 2 * TILE * NBUF;
+    constexpr int WAVES = FewShape<T, DP, WIDE>::kWaves, NBUF = FewShape<T, DP, WIDE>::kBufs;
+    constexpr int TILE = 32 * TL::kRowBytes, WAVE_BYTES = 2 * TILE * NBUF;
     static_assert(WAVE_BYTES >= 32 * DP * 4, "the waves' rows are joined in the same memory");
     __shared__ __attribute__((aligned(1024))) char lds[WAVES * WAVE_BYTES];
     __shared__ float lm[WAVES][32], ll[WAVES][32];
@@ -653,9 +655,11 @@ template <typename T, int DP>
 void attend(const AttendArgs &a, int rows, int G, int groups, hipStream_t s) {
     constexpr int BN = DP * (int)sizeof(T) <= 256 ? 64 : 32;
     if (rows <= kFewRows) {
-        constexpr int WAVES = FewShape<T, DP>::kWaves;
-        if (a.vec) attend_few_kernel<T, DP, WAVES, true><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
-        else attend_few_kernel<T, DP, WAVES, false><<<groups * a.splits, WAVES * 64, 0, s>>>(a, rows, G);
+        constexpr int threads = FewShape<T, DP, false>::kWaves * 64, wide = FewShape<T, DP, true>::kWaves * 64;
+        const int grid = groups * a.splits;
+        if (a.wide && a.vec) attend_few_kernel<T, DP, true, true><<<grid, wide, 0, s>>>(a, rows, G);
+        else if (a.vec) attend_few_kernel<T, DP, false, true><<<grid, threads, 0, s>>>(a, rows, G);
+        else attend_few_kernel<T, DP, false, false><<<grid, threads, 0, s>>>(a, rows, G);
     } else {
         const int tiles = (rows + 127) / 128, grid = groups * a.splits * tiles;
         if (a.vec) attend_rows_kernel<T, DP, BN, true><<<grid, kHeadsThreads, 0, s>>>(a, rows, G, tiles);

@@ -29,10 +29,15 @@ HEAD_DIM_MAX = 256
 _OP_WINDOW, _OP_WINDOW_BACKWARD, _OP_PREFIX, _OP_SCORED, _OP_EVICT = range(5)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _INT_MAX = (1 << 31) - 1
-# struct sdpa_heads: 60 words (size, 10 tensors, 5 pointers, 4 strides, 2 tensors, 2 pointers), 13 ints, a float
-_PACK = struct.Struct("=60q13if")
-_NO = (0, 0, 0, 0)
-_NO2, _NO4, _NO6 = _NO * 2, _NO * 4, (0,) * 6
+# struct sdpa_heads as bytes, a packer for each call: size, q k v out (16 words), prefix (8), gradients (16), lse and lengths (3),
+# weights (6), k_out v_out (8), lens_out kept (2), then dtype and the seven sizes, window, sinks, prefix_tokens, budget, recent, scale.
+# What a call has no use for is padding, which packs as zeros.
+_SIZE = 8 * 60 + 14 * 4
+_PACK_WINDOW = struct.Struct("=17q64x128x3q48x64x16x10i12xf")
+_PACK_BACKWARD = struct.Struct("=17q64x16q3q48x64x16x10i12xf")
+_PACK_PREFIX = struct.Struct("=17q8q128x3q48x64x16x8i8xi8xf")
+_PACK_SCORED = struct.Struct("=17q64x128x3q6q64x16x8i20xf")
+_PACK_EVICT = struct.Struct("=q32x8q32x64x128x16xq6q8q2q8i4xi4x2if")
 # (the stream's number without a Stream object around it: a microsecond and a half of a call that takes ten)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
@@ -41,12 +46,8 @@ def _at(x):
     return (x.data_ptr(),) + x.stride()[:3]
 
 
-def _pack(q, dims, scale, window=0, sinks=0, prefix_tokens=0, budget=0, recent=0, k=_NO, v=_NO, out=_NO, prefix=_NO2, grads=_NO4, lse=0,
-          q_lens=None, kv_lens=None, weights=_NO6, cache=_NO2, new=(0, 0)):
-    """struct sdpa_heads as bytes"""
-    return _PACK.pack(_PACK.size, *_at(q), *k, *v, *out, *prefix, *grads, lse, 0 if q_lens is None else q_lens.data_ptr(),
-                      0 if kv_lens is None else kv_lens.data_ptr(), *weights, *cache, *new, _DTYPES[q.dtype], *dims, window, sinks,
-                      prefix_tokens, budget, recent, scale)
+def _ptr(x):
+    return 0 if x is None else x.data_ptr()
 
 
 def _call(fn, name, op, x, args):
@@ -174,8 +175,8 @@ def attention_window(q, k, v, window, sinks=0, q_lens=None, kv_lens=None, scale=
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
     out, lse = _outputs(q, Dv, out, lse, (q, k, v), name)
-    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), window, sinks, k=_at(k), v=_at(v), out=_at(out), lse=lse.data_ptr(),
-                 q_lens=q_lens, kv_lens=kv_lens)
+    args = _PACK_WINDOW.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk,
+                             Hq, Hkv, Dk, Dv, window, sinks, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_window, name, _OP_WINDOW, q, args)
     return out, lse
 
@@ -202,8 +203,8 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
     dq = q.new_empty(q.shape) if dq is None else dq
     dk = q.new_empty(k.shape) if dk is None else dk
     dv = q.new_empty(v.shape) if dv is None else dv
-    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), window, sinks, k=_at(k), v=_at(v), out=_at(out),
-                 grads=_at(dout) + _at(dq) + _at(dk) + _at(dv), lse=lse.data_ptr(), q_lens=q_lens, kv_lens=kv_lens)
+    args = _PACK_BACKWARD.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), *_at(dout), *_at(dq), *_at(dk), *_at(dv), lse.data_ptr(), _ptr(q_lens),
+                               _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, window, sinks, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_window_backward, name, _OP_WINDOW_BACKWARD, q, args)
     return dq, dk, dv
 
@@ -222,9 +223,9 @@ def attention_prefix(q, k_prefix, v_prefix, k, v, q_lens=None, kv_lens=None, sca
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, k_prefix, v_prefix), name)
-    prefix = (k_prefix.data_ptr(), 0) + k_prefix.stride()[:2] + (v_prefix.data_ptr(), 0) + v_prefix.stride()[:2]
-    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), prefix_tokens=P, k=_at(k), v=_at(v), out=_at(out), prefix=prefix,
-                 lse=lse.data_ptr(), q_lens=q_lens, kv_lens=kv_lens)
+    args = _PACK_PREFIX.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), k_prefix.data_ptr(), 0, *k_prefix.stride()[:2], v_prefix.data_ptr(), 0,
+                             *v_prefix.stride()[:2], lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv,
+                             P, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_prefix, name, _OP_PREFIX, q, args)
     return out, lse
 
@@ -255,8 +256,8 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
         _weights(weights_out, "weights_out", (B, Hkv, Tk), q, True)
         _apart([weights_out], (q, k, v, weights), name)
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights), name)
-    args = _pack(q, (B, Tq, Tk, Hq, Hkv, Dk, Dv), _scale(scale, Dk), k=_at(k), v=_at(v), out=_at(out), lse=lse.data_ptr(), q_lens=q_lens,
-                 kv_lens=kv_lens, weights=_sums(weights, weights_out))
+    args = _PACK_SCORED.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), *_sums(weights, weights_out),
+                             _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q, args)
     return out, lse, weights_out
 
@@ -298,7 +299,7 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
     weights_out = k.new_empty((B, H, budget), dtype=torch.float32) if weights_out is None else weights_out
     lens_out = k.new_empty((B,), dtype=torch.int32)
     kept = k.new_empty((B, H, budget), dtype=torch.int32)
-    args = _pack(k, (B, 0, T, H, H, Dk, Dv), 1.0, sinks=sinks, budget=budget, recent=recent, k=_at(k), v=_at(v), kv_lens=lens,
-                 weights=_sums(weights, weights_out), cache=_at(k_out) + _at(v_out), new=(lens_out.data_ptr(), kept.data_ptr()))
+    args = _PACK_EVICT.pack(_SIZE, *_at(k), *_at(v), _ptr(lens), *_sums(weights, weights_out), *_at(k_out), *_at(v_out), lens_out.data_ptr(),
+                            kept.data_ptr(), _DTYPES[k.dtype], B, 0, T, H, H, Dk, Dv, sinks, budget, recent, 1.0)
     _call(_lib.load().sdpa_dev_evict_cache, name, _OP_EVICT, k, args)
     return k_out, v_out, weights_out, lens_out, kept
