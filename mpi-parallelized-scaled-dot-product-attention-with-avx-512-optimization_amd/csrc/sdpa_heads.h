@@ -51,13 +51,14 @@ struct AttendArgs {
 struct BackwardArgs {
     sdpa_tensor q, k, v, out, dout, dq, dk, dv;
     const float *lse;
-    float *delta;                     // [B][Hq][Tq] row sums of dO * O
+    float *stats;                     // [2][B * Hkv][stat_rows]: lse (exp2 domain) and -sum dO * O of the rows, in the keys kernel's order
+    long stat_rows, stat_stride;      // (a multiple of 64; the second array's offset)
     float *part;                      // partial dK | dV rows of the key blocks whose queries several workgroups share
     const int *q_lens, *kv_lens;
     int B, Tq, Tk, Hq, Hkv, Dk, Dv;
     int window, sinks;
-    int sink_blocks, sink_chunks;     // key blocks with sink keys, and the workgroups each of them has
-    int rest_chunks;                  // workgroups of every other key block
+    int chunks;                       // workgroups that share a key block's rows
+    int sink_blocks, tail_chunks;     // key blocks with sink keys, and the workgroups for their rows behind the window
     int vec, vec_out, dma;            // 16-byte loads / stores; tiles by DMA
     float scale, scale_log2;
 };

@@ -155,32 +155,32 @@ int run_own(const sdpa_heads *a, const Slots &s, void *workspace, hipStream_t st
     return SDPA_OK;
 }
 
-struct BackwardPlan { int sink_blocks, sink_chunks, rest_chunks; long delta, bytes; double grid; };
+struct BackwardPlan { int chunks, sink_blocks, tail_chunks; long stat_rows, stats, bytes; double grid; };
 
-// The rows a key block walks: about (128 + window) tokens' heads, but every row for a block with sink keys -- those are cut to
-// the length of the others', so that no workgroup walks much longer than the rest; and all are cut further while the launch
-// has fewer than two workgroups a CU.
+// A key block's workgroup walks the rows that see it by the window, about (64 + window) tokens' heads; several share them while the launch
+// has fewer workgroups than the chip has CUs.  A block with sink keys is seen by every row behind: its tail goes to short workgroups
+// of their own, launched last (one walk in a row's length would outlast all others).
 BackwardPlan plan_backward(const sdpa_heads *a) {
     BackwardPlan p = {};
-    const long G = a->q_heads / a->kv_heads, groups = (long)a->batch * a->kv_heads;
-    const long blocks = ceil_div(a->kv_tokens, kBwdKeys);
-    const long sinks = a->sinks < a->kv_tokens ? a->sinks : a->kv_tokens;
-    const long w = (long)a->window + kBwdKeys < a->q_tokens ? (long)a->window + kBwdKeys : a->q_tokens;
-    const long rest_tiles = ceil_div(w * G, 32), sink_tiles = ceil_div((long)a->q_tokens * G, 32);
+    const long G = a->q_heads / a->kv_heads, groups = (long)a->batch * a->kv_heads, blocks = ceil_div(a->kv_tokens, kBwdKeys);
+    const long sinks = a->sinks < a->kv_tokens ? a->sinks : a->kv_tokens, reach = (long)a->window + kBwdKeys;
+    const long walk = (reach < a->q_tokens ? reach : a->q_tokens) * G, tail = reach < a->q_tokens ? (a->q_tokens - reach) * G : 0;
+    long chunks = groups * blocks < 256 ? ceil_div(256, groups * blocks < 1 ? 1 : groups * blocks) : 1;
+    if (chunks > ceil_div(walk, 256)) chunks = ceil_div(walk, 256);
+    if (chunks > kMaxSplits) chunks = kMaxSplits;
+    p.chunks = chunks < 1 ? 1 : (int)chunks;
     p.sink_blocks = (int)ceil_div(sinks, kBwdKeys);
-    long rest = groups * blocks < 512 ? ceil_div(512, groups * blocks < 1 ? 1 : groups * blocks) : 1;
-    if (rest > ceil_div(rest_tiles, 8)) rest = ceil_div(rest_tiles, 8);
-    if (rest > kMaxSplits) rest = kMaxSplits;
-    if (rest < 1) rest = 1;
-    long sink = ceil_div(sink_tiles * rest, rest_tiles < 1 ? 1 : rest_tiles);
-    if (sink > kMaxSplits) sink = kMaxSplits;
-    if (sink < 1) sink = 1;
-    p.rest_chunks = (int)rest;
-    p.sink_chunks = (int)sink;
-    const long items = (sink > 1 ? p.sink_blocks * sink : 0) + (rest > 1 ? (blocks - p.sink_blocks) * rest : 0);
-    p.grid = (double)groups * (p.sink_blocks * sink + (blocks - p.sink_blocks) * rest);
-    p.delta = (groups * G * a->q_tokens * 4 + 15) / 16 * 16;
-    p.bytes = p.delta + groups * items * kBwdKeys * (a->dk + a->dv) * 4 + 16;
+    const long piece = walk / (4 * p.chunks) > 512 ? walk / (4 * p.chunks) : 512;
+    const long tails = ceil_div(tail, piece);
+    p.tail_chunks = p.sink_blocks == 0 ? 0 : (int)(tails < kMaxSplits ? tails : kMaxSplits);
+    p.grid = (double)groups * (blocks * p.chunks + p.sink_blocks * p.tail_chunks);
+    const long slots = p.chunks > 1 ? blocks * p.chunks + p.sink_blocks * p.tail_chunks :
+                       p.tail_chunks > 0 ? p.sink_blocks * (1 + p.tail_chunks) : 0;
+    // rows of a head: blocks of 32, whole tokens to a block (or, of larger groups, blocks to a token), in pairs
+    const long row_blocks = G <= 32 ? ceil_div(a->q_tokens, 32 / G) : a->q_tokens * ceil_div(G, 32);
+    p.stat_rows = ceil_div(row_blocks, 2) * 64;
+    p.stats = 2 * groups * p.stat_rows * 4;
+    p.bytes = p.stats + groups * slots * kBwdKeys * (a->dk + a->dv) * 4 + 16;
     return p;
 }
 
@@ -250,12 +250,14 @@ int sdpa_dev_attention_window_backward(const struct sdpa_heads *a, void *workspa
     BackwardArgs x = {};
     x.q = a->q; x.k = a->k; x.v = a->v; x.out = a->out; x.dout = a->dout; x.dq = a->dq; x.dk = a->dk_out; x.dv = a->dv_out;
     x.lse = a->lse; x.q_lens = a->q_lens; x.kv_lens = a->kv_lens;
-    x.delta = (float *)workspace;
-    x.part = (float *)((char *)workspace + p.delta);
+    x.stats = (float *)workspace;
+    x.stat_rows = p.stat_rows;
+    x.stat_stride = (long)a->batch * a->kv_heads * p.stat_rows;
+    x.part = (float *)((char *)workspace + p.stats);
     x.B = a->batch; x.Tq = a->q_tokens; x.Tk = a->kv_tokens; x.Hq = a->q_heads; x.Hkv = a->kv_heads; x.Dk = a->dk; x.Dv = a->dv;
     x.window = a->window < kMaxTokens ? a->window : kMaxTokens;
     x.sinks = a->sinks;
-    x.sink_blocks = p.sink_blocks; x.sink_chunks = p.sink_chunks; x.rest_chunks = p.rest_chunks;
+    x.chunks = p.chunks; x.sink_blocks = p.sink_blocks; x.tail_chunks = p.tail_chunks;
     x.vec = rows_vec(a->q, a->dk, a->dtype) && rows_vec(a->k, a->dk, a->dtype) && rows_vec(a->v, a->dv, a->dtype) &&
             rows_vec(a->out, a->dv, a->dtype) && rows_vec(a->dout, a->dv, a->dtype);
     // a tile of 64 rows: two blocks of 32 / G tokens' heads, at 32-bit offsets

@@ -46,34 +46,143 @@ __device__ inline void load_row(typename Ops<T>::Frag *f, const void *row, int d
     }
 }
 
-// ---- dQ: 128 rows to a workgroup, 32 to a wave -------------------------------------------------------------------------
-// One 32-key block: S^T and dP^T with the keys as rows, dS^T kept in registers as the operand of dQ^T += K^T dS^T.
-template <typename T, int DP, bool MASKED>
-__device__ inline void grad_rows(f32x16 *dq, const typename Ops<T>::Frag *q, const typename Ops<T>::Frag *g, unsigned tk, unsigned tv,
-                                 const LaneMap<T, DP> &map, int j0, Seen seen, int sinks, float scale, float lse2, float delta, int lane) {
-    constexpr int STEPS = DP / Ops<T>::kStep;
-    f32x16 s = {}, dp = {};
-    const unsigned ak = tk + map.rows, av = tv + map.rows;
+// ---- one 32 x 32 block of pairs -------------------------------------------------------------------------------------------------
+// Tiles X and Y lie in LDS (X = Q, Y = dO against a wave's keys; X = K, Y = V against a wave's queries), their partners x and y in
+// registers, one column to a lane:
+//     S = X x,  dP = Y y,  P = exp(S - lse),  dS = P * (dP - delta),   then   acc_y += Y^T P  (dV)   and   acc_x += X^T dS  (dK or dQ).
+// Written down unit by unit (see Pipe): the exponentials stand beside the units of dP, the rest beside those of dV; dP begins at -delta.
+// What a lane's column sees of the block's rows r: r < hi and (r >= lo or r < sk).
+struct Sees { int hi, lo, sk; };
+
+// lse and -delta: of the lane's column (rows kernel) or of the block's rows, in LDS (keys kernel)
+struct ColumnStats {
+    float lse2, neg_delta;
+    __device__ f32x4 lse_at(int) const { return f32x4{lse2, lse2, lse2, lse2}; }
+    __device__ f32x4 delta_at(int) const { return f32x4{neg_delta, neg_delta, neg_delta, neg_delta}; }
+};
+struct RowStats {
+    unsigned at;                                        // + the lane half's 16 bytes; -delta lies 256 bytes behind lse
+    __device__ f32x4 lse_at(int i) const { return lds_read<f32x4>(at, i * 32); }
+    __device__ f32x4 delta_at(int i) const { return lds_read<f32x4>(at, 256 + i * 32); }
+};
+
+template <typename T, int DP, bool VY, bool VX, bool MASKED, typename Stats> struct GradBlock {
+    using Frag = typename Ops<T>::Frag;
+    static constexpr int KU = DP / Ops<T>::kStep, VK = sizeof(T) == 2 ? 2 : 4, VU = DP / 32 * VK;
+    static constexpr int B0 = KU, C0 = B0 + (VX ? KU : 0), D0 = C0 + (VY ? VU : 0), UNITS = D0 + (VX ? VU : 0), AHEAD = 3;
+    unsigned xr, yr, xc, yc;                            // where the lane reads the tiles' rows and columns
+    Frag ring[AHEAD + 1];
+    f32x16 s, dp;
+    f32x4 lse[4];
+    Probs<T> p, ds;
+    uint32_t vis;
+    __device__ inline __attribute__((always_inline)) Frag fetch(int u) const {
+        if (u < B0) return read_rows<T, DP>(xr, 0, u);
+        if (u < C0) return read_rows<T, DP>(yr, 0, u - B0);
+        if (u < D0) return read_cols_part<DP>(yc, 0, (u - C0) / VK, (u - C0) % VK, T());
+        return read_cols_part<DP>(xc, 0, (u - D0) / VK, (u - D0) % VK, T());
+    }
+    __device__ inline __attribute__((always_inline)) void weight(int i, float scale) {
+        s[i] = __builtin_amdgcn_exp2f(s[i] * scale - lse[i >> 2][i & 3]);
+        if (MASKED) s[i] = (vis >> i) & 1 ? s[i] : 0.f;
+        if (VY && (sizeof(T) == 4 || (i & 1))) put_prob(p, s, i);
+    }
+    __device__ inline __attribute__((always_inline)) void slope(int i) {
+        s[i] = MASKED && !((vis >> i) & 1) ? 0.f : s[i] * dp[i];
+        if (sizeof(T) == 4 || (i & 1)) put_prob(ds, s, i);
+    }
+    template <int U>
+    __device__ inline __attribute__((always_inline)) void unit(f32x16 *ax, f32x16 *ay, const Frag *x, const Frag *y, float scale) {
+        if constexpr (U < UNITS) {
+            if constexpr (U + AHEAD < UNITS) ring[(U + AHEAD) % (AHEAD + 1)] = fetch(U + AHEAD);
+            const Frag f = ring[U % (AHEAD + 1)];
+            if constexpr (U == C0 && !VX) {             // (nothing to stand beside)
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(ak, 0, i), q[i], s);
+                for (int i = 0; i < 16; ++i) weight(i, scale);
+            }
+            if constexpr (U == D0 && VX && !VY) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(av, 0, i), g[i], dp);
-    uint32_t vis = 0;
-    const int half = MASKED ? opaque(lane) >> 5 : 0;
+                for (int i = 0; i < 16; ++i) slope(i);
+            }
+            if constexpr (U < B0) s = Ops<T>::mma(f, x[U], s);
+            else if constexpr (U < C0) dp = Ops<T>::mma(f, y[U - B0], dp);
+            else if constexpr (U < D0) ay[(U - C0) / VK] = mma_part(f, p, (U - C0) % VK, ay[(U - C0) / VK]);
+            else ax[(U - D0) / VK] = mma_part(f, ds, (U - D0) % VK, ax[(U - D0) / VK]);
+            if constexpr (VX && U > B0 && U < C0) {      // (one unit behind the product they read)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(s[i] * scale - lse2);
-        s[i] = p * (dp[i] - delta);
-        if (MASKED) {
-            const int j = j0 + row_of(i, half);
-            const bool ok = j < seen.hi && (j >= seen.lo || j < sinks);
-            vis |= ok ? 1u << i : 0u;
-            s[i] = ok ? s[i] : 0.f;
+                for (int i = 0; i < 16; ++i)
+                    if (B0 + 1 + i * (KU - 1) / 16 == U) weight(i, scale);
+            }
+            if constexpr (VX && VY && U > C0 && U < D0) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (C0 + 1 + i * (VU - 1) / 16 == U) slope(i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            unit<U + 1>(ax, ay, x, y, scale);
         }
     }
-    mma_block<T, DP, DP / 32>(dq, tk, map, 0, to_probs(s, T()), MASKED, vis, 1, lane);
-}
+    __device__ inline __attribute__((always_inline)) void begin(unsigned tx, unsigned ty, const LaneMap<T, DP> &map, const Stats &st, Sees see) {
+        xr = tx + map.rows; yr = ty + map.rows; xc = tx + map.cols; yc = ty + map.cols;
+        s = f32x16{};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lse[i] = st.lse_at(i);
+            if (VX) {
+                const f32x4 d = st.delta_at(i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) dp[4 * i + k] = d[k];
+            }
+        }
+        if (MASKED) {
+            vis = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int r = row_of(i, 0);
+                vis |= r < see.hi && (r >= see.lo || r < see.sk) ? 1u << i : 0u;
+            }
+        }
+    }
+    __device__ inline __attribute__((always_inline)) void run(f32x16 *ax, f32x16 *ay, const Frag *x, const Frag *y, unsigned tx, unsigned ty,
+                                                              const LaneMap<T, DP> &map, const Stats &st, Sees see, float scale) {
+        begin(tx, ty, map, st, see);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) ring[u] = fetch(u);
+        __builtin_amdgcn_sched_barrier(0);
+        unit<0>(ax, ay, x, y, scale);
+    }
+    // the same arithmetic with products that leave out what a masked pair holds (block_not_finite)
+    __device__ inline __attribute__((always_inline)) void run_guarded(f32x16 *ax, f32x16 *ay, const Frag *x, const Frag *y, unsigned tx, unsigned ty,
+                                                                      const LaneMap<T, DP> &map, const Stats &st, Sees see, float scale, int lane) {
+        begin(tx, ty, map, st, see);
+#pragma unroll
+        for (int i = 0; i < KU; ++i) s = Ops<T>::mma(read_rows<T, DP>(xr, 0, i), x[i], s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) weight(i, scale);
+        if constexpr (VY) mma_block<T, DP, DP / 32>(ay, ty, map, 0, p, true, vis, 1, lane);
+        if constexpr (VX) {
+#pragma unroll
+            for (int i = 0; i < KU; ++i) dp = Ops<T>::mma(read_rows<T, DP>(yr, 0, i), y[i], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) slope(i);
+            mma_block<T, DP, DP / 32>(ax, tx, map, 0, ds, true, vis, 1, lane);
+        }
+    }
+};
 
+// The rows a key head's queries are walked in: blocks of 32, whole tokens' grouped heads to a block (the rows a block has left
+// over are zeros), or, for groups of more than 32 heads, blocks of one token.  So a row's place inside its block is the same in
+// every block, and a tile of blocks costs the DMA no vector arithmetic.
+struct RowBlocks {
+    int G, tokens, split;                               // tokens of a block, blocks of a token: one of them is 1
+    __device__ explicit RowBlocks(int g) : G(g), tokens(g <= 32 ? 32 / g : 1), split(g <= 32 ? 1 : (g + 31) / 32) {}
+    __device__ int row(int t) const { return (split > 1 ? t * split : t / tokens) * 32 + (split > 1 ? 0 : t % tokens * G); }
+    __device__ int token(int block, int i) const { return split > 1 ? block / split : block * tokens + i / G; }
+    __device__ int head(int block, int i) const { return split > 1 ? block % split * 32 + i : i % G; }
+    __device__ bool used(int block, int i) const { return split > 1 ? head(block, i) < G : i < tokens * G; }
+};
+
+// ---- dQ: 128 rows to a workgroup, 32 to a wave -------------------------------------------------------------------------
 template <typename T, int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kHeadsThreads, DP * (int)sizeof(T) <= 256 ? 2 : 1)
 void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
@@ -130,8 +239,18 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
         delta = half_sum(delta);
     }
     const long at = ((long)b * a.Hq + hq) * a.Tq + t;
-    const float lse2 = live ? a.lse[at] * kLog2e : 0.f;
-    if (r < rows && lane < 32) a.delta[at] = delta;
+    const float lse2 = live ? a.lse[at] * kLog2e : __builtin_inff();     // (a row that does not exist: weight 2^(0 - inf) = 0)
+    if (r < rows && lane < 32) {                         // for the keys kernel, in the order it walks the rows
+        const RowBlocks rb(G);
+        const int g = r - t * G, place = rb.row(t) + g;
+        float *l = a.stats + ((long)b * a.Hkv + h) * a.stat_rows + place;
+        const int used = rb.split > 1 ? (g == G - 1 ? g & 31 : 31) : rb.tokens * G - 1;
+        const int fill = (place & 31) == used ? 32 - (place & 31) : 1;     // (with the last row of a block, what the block has left over)
+        for (int i = 0; i < fill; ++i) {
+            l[i] = i == 0 ? lse2 : __builtin_inff();
+            l[a.stat_stride + i] = i == 0 ? -delta : 0.f;
+        }
+    }
 
     f32x16 dq[DP / 32];
 #pragma unroll
@@ -140,6 +259,13 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
         for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
     LaneMap<T, DP> map;
     map.init(lane);
+    const ColumnStats stats = {lse2, -delta};
+    auto sees = [&](Frame f) {
+        const int at = f.j0 + 4 * (opaque(lane) >> 5);
+        return Sees{seen.hi - at, seen.lo - at, f.sinks - at};
+    };
+    bool odd = false;                                    // a block with masked pairs holds values that are no numbers
+#pragma unroll 1
     for (int it = 0, buf = 0; it < count; ++it, buf ^= 1) {
         dma_wait();
         __syncthreads();
@@ -149,8 +275,35 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
             const Frame f = list.frame(it * BN + n * 32, 32);
             if (!sees_some(wv, f, 32)) continue;
             const unsigned tk = lds0 + buf * 2 * TILE + n * 32 * TL::kRowBytes, tv = tk + TILE;
-            if (sees_all(wv, f, 32)) grad_rows<T, DP, false>(dq, q, g, tk, tv, map, f.j0, seen, f.sinks, a.scale_log2, lse2, delta, lane);
-            else grad_rows<T, DP, true>(dq, q, g, tk, tv, map, f.j0, seen, f.sinks, a.scale_log2, lse2, delta, lane);
+            if (sees_all(wv, f, 32)) {
+                GradBlock<T, DP, false, true, false, ColumnStats> blk;
+                blk.run(dq, nullptr, q, g, tk, tv, map, stats, Sees{}, a.scale_log2);
+            } else {
+                odd = odd || block_not_finite<T, DP>(tk, 0, lane);
+                GradBlock<T, DP, false, true, true, ColumnStats> blk;
+                blk.run(dq, nullptr, q, g, tk, tv, map, stats, sees(f), a.scale_log2);
+            }
+        }
+    }
+    if (__syncthreads_or(odd)) {                          // then the workgroup does its rows once more, with guarded products
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
+#pragma unroll 1
+        for (int it = 0; it < count; ++it) {
+            __syncthreads();
+            stage(it, 0);
+            dma_wait();
+            __syncthreads();
+#pragma unroll 1
+            for (int n = 0; n < BN / 32; ++n) {
+                const Frame f = list.frame(it * BN + n * 32, 32);
+                if (!sees_some(wv, f, 32)) continue;
+                const unsigned tk = lds0 + n * 32 * TL::kRowBytes, tv = tk + TILE;
+                GradBlock<T, DP, false, true, true, ColumnStats> blk;
+                blk.run_guarded(dq, nullptr, q, g, tk, tv, map, stats, sees(f), a.scale_log2, lane);
+            }
         }
     }
     if (r >= rows) return;
@@ -165,6 +318,14 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
         }
 }
 
+// slots of a key block's partial gradients (1: it writes the gradients itself), and of the blocks before it
+__device__ inline int block_slots(const BackwardArgs &a, int block) { return a.chunks + (block < a.sink_blocks ? a.tail_chunks : 0); }
+__device__ inline long slots_before(const BackwardArgs &a, int block) {
+    const long n = a.chunks > 1 || block < a.sink_blocks ? block : a.sink_blocks;      // (blocks of one slot take no place)
+    const int sinks = block < a.sink_blocks ? block : a.sink_blocks;
+    return a.tail_chunks == 0 && a.chunks == 1 ? 0 : n * a.chunks + (long)sinks * a.tail_chunks;
+}
+
 // which queries see a key: tokens [lo, hi)
 struct SeenBy { int lo, hi; };
 __device__ inline SeenBy seen_by(int j, int nq, int nk, int window, int sinks) {
@@ -177,18 +338,6 @@ __device__ inline SeenBy seen_by(int j, int nq, int nk, int window, int sinks) {
     s.lo = lo; s.hi = hi;
     return s;
 }
-
-// The rows a key head's queries are walked in: blocks of 32, whole tokens' grouped heads to a block (the rows a block has left
-// over are zeros), or, for groups of more than 32 heads, blocks of one token.  So a row's place inside its block is the same in
-// every block, and a tile of blocks costs the DMA no vector arithmetic.
-struct RowBlocks {
-    int G, tokens, split;                               // tokens of a block, blocks of a token: one of them is 1
-    __device__ explicit RowBlocks(int g) : G(g), tokens(g <= 32 ? 32 / g : 1), split(g <= 32 ? 1 : (g + 31) / 32) {}
-    __device__ int row(int t) const { return (split > 1 ? t * split : t / tokens) * 32 + (split > 1 ? 0 : t % tokens * G); }
-    __device__ int token(int block, int i) const { return split > 1 ? block / split : block * tokens + i / G; }
-    __device__ int head(int block, int i) const { return split > 1 ? block % split * 32 + i : i % G; }
-    __device__ bool used(int block, int i) const { return split > 1 ? head(block, i) < G : i < tokens * G; }
-};
 
 // Tiles of two such blocks of one tensor, staged by four waves
 template <typename T, int DP> struct RowStager {
@@ -213,20 +362,25 @@ template <typename T, int DP> struct RowStager {
             off[k] = (unsigned)(((r >> 5) * rb.tokens + i / rb.G) * (int)token + i % rb.G * (int)head) + 16u * (unsigned)source(wave, lane, k);
         }
     }
-    // (groups of at most 32 heads) rows behind the last query are read as the last query's: their weights are masked
-    __device__ void dma(unsigned lds, int block, int nq, const RowBlocks &rb, int wave, int lane) const {
+    // (groups of at most 32 heads) rows behind the last query are read as the last query's: their weights are masked.  -> true: exactly
+    // kPieces instructions are on their way
+    __device__ bool dma(unsigned lds, int block, int nq, const RowBlocks &rb, int wave, int lane) const {
         const int t0 = block * rb.tokens;
         const char *at = base + (long)t0 * token;
-        const bool plain = dim == DP && rb.tokens * rb.G == 32, inside = t0 + 2 * rb.tokens <= nq;
+        lds += (unsigned)(wave * kPieces) * 1024u;
+        if (dim == DP && rb.tokens * rb.G == 32 && t0 + 2 * rb.tokens <= nq) {
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            unsigned o = off[k];
-            const unsigned dst = lds + (unsigned)(wave * kPieces + k) * 1024u;
-            if (plain && inside) { lds_dma(at, o, dst); continue; }
-            const int ln = opaque(lane), r = row(wave, ln, k), i = r & 31, t = t0 + (r >> 5) * rb.tokens + i / rb.G;
-            if (t >= nq) o += (unsigned)((nq - 1 - t) * (int)token);
-            if (i < rb.tokens * rb.G && source(wave, ln, k) * Ops<T>::kVec < dim) lds_dma(at, o, dst);     // (the rest stays zero)
+            for (int k = 0; k < kPieces; ++k) lds_dma(at, off[k], lds + k * 1024u);
+            return true;
         }
+        const int ln = opaque(lane);
+#pragma unroll 1
+        for (int k = 0; k < kPieces; ++k) {
+            const int r = row(wave, ln, k), i = r & 31, x = (r >> 5) * rb.tokens + i / rb.G, c = source(wave, ln, k);
+            const unsigned o = (unsigned)((t0 + x < nq ? x : nq - 1 - t0) * (int)token + i % rb.G * (int)head) + 16u * (unsigned)c;
+            if (i < rb.tokens * rb.G && c * Ops<T>::kVec < dim) lds_dma(at, o, lds + k * 1024u);      // (the rest stays zero)
+        }
+        return false;
     }
     __device__ void copy(char *tile, int block, int nq, const RowBlocks &rb, bool vec, int wave, int lane) const {
 #pragma unroll 4
@@ -240,52 +394,6 @@ template <typename T, int DP> struct RowStager {
     }
 };
 
-// One block of 32 rows against a wave's 32 keys: P, dP, dS have the rows as rows and a key to a lane, and stay in registers as the
-// operands of dV^T += dO^T P and dK^T += Q^T dS.
-template <typename T, int DP, int WHAT, bool MASKED>
-__device__ inline void grad_keys(f32x16 *dk, f32x16 *dv, const typename Ops<T>::Frag *kf, const typename Ops<T>::Frag *vf, unsigned tq,
-                                 unsigned tg, const LaneMap<T, DP> &map, unsigned stats, int r0, SeenBy by, float scale, int lane) {
-    constexpr int STEPS = DP / Ops<T>::kStep;
-    const unsigned aq = tq + map.rows, ag = tg + map.rows, st = stats + (lane >> 5) * 16;
-    f32x16 s = {};
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) s = Ops<T>::mma(read_rows<T, DP>(aq, 0, i), kf[i], s);
-    uint32_t vis = 0;
-    const int half = MASKED ? opaque(lane) >> 5 : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const f32x4 lse2 = lds_read<f32x4>(st, i * 32);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int x = 4 * i + k;
-            s[x] = __builtin_amdgcn_exp2f(s[x] * scale - lse2[k]);
-            if (MASKED) {
-                const int r = r0 + row_of(x, half);
-                const bool ok = r >= by.lo && r < by.hi;
-                vis |= ok ? 1u << x : 0u;
-                s[x] = ok ? s[x] : 0.f;
-            }
-        }
-    }
-    if constexpr ((WHAT & 1) != 0) mma_block<T, DP, DP / 32>(dv, tg, map, 0, to_probs(s, T()), MASKED, vis, 1, lane);
-    if constexpr ((WHAT & 2) != 0) {
-        f32x16 dp = {};
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) dp = Ops<T>::mma(read_rows<T, DP>(ag, 0, i), vf[i], dp);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 delta = lds_read<f32x4>(st, 256 + i * 32);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int x = 4 * i + k;
-                const float ds = s[x] * (dp[x] - delta[k]);
-                s[x] = MASKED && !((vis >> x) & 1) ? 0.f : ds;
-            }
-        }
-        mma_block<T, DP, DP / 32>(dk, tq, map, 0, to_probs(s, T()), MASKED, vis, 1, lane);
-    }
-}
-
 // ---- dK, dV: 64 keys to a workgroup -----------------------------------------------------------------------------------------
 // Waves 0 and 1 take 32 keys each on the even row blocks, waves 2 and 3 the same keys on the odd ones; the two sums are added in LDS
 // at the end.  (Against four waves of 32 keys: twice the workgroups, so that two share a CU and one's exponentials run beside the
@@ -294,21 +402,22 @@ __device__ inline void grad_keys(f32x16 *dk, f32x16 *dv, const typename Ops<T>::
 // no registers for the scores.
 template <typename T, int DP, int WHAT, bool VEC>
 __global__ __launch_bounds__(kHeadsThreads, DP * (int)sizeof(T) <= 128 ? 2 : 1)
-void backward_keys_kernel(BackwardArgs a, int G, int items) {
+void backward_keys_kernel(BackwardArgs a, int G, int blocks) {
     using TL = Tile<T, DP>;
-    constexpr int STEPS = DP / Ops<T>::kStep, TILE = 64 * TL::kRowBytes, NBUF = 4 * TILE <= 131072 ? 2 : 1;
+    constexpr int STEPS = DP / Ops<T>::kStep, TILE = 64 * TL::kRowBytes;
+    constexpr int NBUF = 131072 / (2 * TILE) < 4 ? 131072 / (2 * TILE) : 4, AHEAD = NBUF - 1, PIECES = 2 * RowStager<T, DP>::kPieces;
     constexpr bool DV = (WHAT & 1) != 0, DK = (WHAT & 2) != 0;
     __shared__ __attribute__((aligned(1024))) char lds[2 * TILE * NBUF];     // Q, dO, Q, dO
-    __shared__ __attribute__((aligned(16))) float lstat[2][2][64];            // [buffer][lse, delta][row]
+    __shared__ __attribute__((aligned(16))) float lstat[NBUF][2][64];         // [buffer][lse, -delta][row]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = xcd_place(blockIdx.x, gridDim.x);
-    const int item = id % items;
-    id /= items;
+    // the blocks' walks over the rows that see them by the window first, then the short ones over the rows that see only their sinks
+    const int groups = a.B * a.Hkv, plain = blocks * a.chunks;
+    const bool tail = (int)blockIdx.x >= groups * plain;
+    int id = tail ? (int)blockIdx.x - groups * plain : xcd_place(blockIdx.x, groups * plain);
+    const int per = tail ? a.sink_blocks * a.tail_chunks : plain, chunks = tail ? a.tail_chunks : a.chunks;
+    const int item = id % per, block = item / chunks, chunk = item % chunks;
+    id /= per;
     const int h = id % a.Hkv, b = id / a.Hkv;
-    const int sink_items = a.sink_blocks * a.sink_chunks;
-    const int chunks = item < sink_items ? a.sink_chunks : a.rest_chunks;
-    const int block = item < sink_items ? item / chunks : a.sink_blocks + (item - sink_items) / chunks;
-    const int chunk = item < sink_items ? item % chunks : (item - sink_items) % chunks;
     const int nq = clamp_len(a.q_lens, b, a.Tq), nk = clamp_len(a.kv_lens, b, a.Tk);
     const int k0 = block * kBwdKeys, kw = k0 + (wave & 1) * 32, phase = wave >> 1, j = kw + (lane & 31);
     const RowBlocks rb(G);
@@ -333,7 +442,15 @@ void backward_keys_kernel(BackwardArgs a, int G, int items) {
     }
     const int blk0 = rb.row(all.lo) / 64 * 2;            // row blocks come in pairs
     const int pairs = all.hi > all.lo ? ((rb.row(all.hi) + 31) / 32 - blk0 + 1) / 2 : 0;
-    const int it0 = (int)((long)pairs * chunk / chunks), it1 = (int)((long)pairs * (chunk + 1) / chunks);
+    int begin = 0, end = pairs;                           // a sink block: the pairs its window reaches, and behind them the tail
+    if (block < a.sink_blocks && a.tail_chunks > 0) {
+        const SeenBy w = seen_by(klast, nq, nk, a.window, 0);
+        const int reach = w.hi > w.lo ? min(pairs, max(0, ((rb.row(w.hi) + 31) / 32 - blk0 + 1) / 2)) : 0;
+        begin = tail ? reach : 0;
+        end = tail ? pairs : reach;
+    }
+    const int it0 = begin + (int)((long)(end - begin) * chunk / chunks), it1 = begin + (int)((long)(end - begin) * (chunk + 1) / chunks);
+    const bool idle = tail && kw >= a.sinks;              // (a tail's rows see nothing else)
 
     RowStager<T, DP> sq, sg;
     sq.init(row_at(a.q, b, 0, h * G, sizeof(T)), a.q, a.Dk, rb, wave, lane);
@@ -343,61 +460,90 @@ void backward_keys_kernel(BackwardArgs a, int G, int items) {
         __syncthreads();
     }
     const unsigned lds0 = lds_address(lds), stat0 = lds_address(&lstat[0][0][0]);
-    float rl = 0.f, rd = 0.f;
+    const float *stat = a.stats + ((long)b * a.Hkv + h) * a.stat_rows;
+    // -> true: exactly PIECES instructions are on their way (and one more of waves 0 and 1)
     auto stage = [&](int it, int buf) {
         const int blk = blk0 + 2 * it;
         if (VEC) {
-            sq.dma(lds0 + buf * 2 * TILE, blk, nq, rb, wave, lane);
-            sg.dma(lds0 + buf * 2 * TILE + TILE, blk, nq, rb, wave, lane);
-        } else {
-            sq.copy(lds + buf * 2 * TILE, blk, nq, rb, a.vec, wave, lane);
-            sg.copy(lds + buf * 2 * TILE + TILE, blk, nq, rb, a.vec, wave, lane);
+            if (wave < 2) lds_dma_words(stat + wave * a.stat_stride + blk * 32, lane, stat0 + buf * 512 + wave * 256);
+            const bool p = sq.dma(lds0 + buf * 2 * TILE, blk, nq, rb, wave, lane);
+            return sg.dma(lds0 + buf * 2 * TILE + TILE, blk, nq, rb, wave, lane) && p;
         }
-        if (tid < 64) {                                  // a row that does not exist: weight 2^(0 - inf) = 0
-            const int i = tid & 31, bl = blk + (tid >> 5), t = rb.token(bl, i);
-            const bool live = t < nq && rb.used(bl, i);
-            const long at = ((long)b * a.Hq + h * G + rb.head(bl, i)) * a.Tq + t;
-            rl = live ? a.lse[at] * kLog2e : __builtin_inff();
-            rd = live ? a.delta[at] : 0.f;
-        }
+        if (tid < 128) lstat[buf][wave][lane] = stat[wave * a.stat_stride + blk * 32 + lane];
+        sq.copy(lds + buf * 2 * TILE, blk, nq, rb, a.vec, wave, lane);
+        sg.copy(lds + buf * 2 * TILE + TILE, blk, nq, rb, a.vec, wave, lane);
+        return false;
     };
-    auto put_stat = [&](int buf) {
-        if (tid < 64) { lstat[buf][0][tid] = rl; lstat[buf][1][tid] = rd; }
+    // bit i: the stage issued i stages ago is exactly PIECES instructions
+    unsigned exact = 0;
+    auto issue = [&](int it) {
+        if (it < it1) exact = exact << 1 | (stage(it, (it - it0) % NBUF) ? 1u : 0u);
     };
-    if (NBUF == 2 && it0 < it1) { stage(it0, 0); put_stat(0); }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) issue(it0 + i);
 
     typename Ops<T>::Frag kf[STEPS], vf[DK ? STEPS : 1];
     load_row<T, DP>(kf, row_at(a.k, b, j, h, sizeof(T)), a.Dk, j < nk, a.vec, lane);
     if (DK) load_row<T, DP>(vf, row_at(a.v, b, j, h, sizeof(T)), a.Dv, j < nk, a.vec, lane);
     f32x16 dk[DK ? DP / 32 : 1], dv[DV ? DP / 32 : 1];
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (DK) dk[d][i] = 0.f;
-            if (DV) dv[d][i] = 0.f;
-        }
     LaneMap<T, DP> map;
     map.init(lane);
-    for (int it = it0, buf = 0; it < it1; ++it) {
+    auto zero = [&] {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (DK) dk[d][i] = 0.f;
+                if (DV) dv[d][i] = 0.f;
+            }
+    };
+    auto sees = [&](int r0) {
+        const int at = r0 + 4 * (opaque(lane) >> 5);
+        return Sees{by.hi - at, by.lo - at, -1};
+    };
+    zero();
+    bool odd = false;                                    // a block with masked pairs holds values that are no numbers
+#pragma unroll 1
+    for (int it = it0; it < it1; ++it) {
+        const int buf = (it - it0) % NBUF;
         if (NBUF == 1) {
             __syncthreads();
             stage(it, 0);
-            put_stat(0);
         }
-        dma_wait();
+        // the stages behind this one may still be on their way
+        const int behind = min(AHEAD - 1, it1 - 1 - it);
+        const bool counted = AHEAD > 1 && behind > 0 && (exact & ((1u << behind) - 1)) == (1u << behind) - 1;
+        if (AHEAD > 1 && counted && behind == 1) dma_wait_but<PIECES>();
+        else if (AHEAD > 2 && counted && behind == 2) dma_wait_but<2 * PIECES>();
+        else dma_wait();
         __syncthreads();
-        if (NBUF == 2 && it + 1 < it1) stage(it + 1, buf ^ 1);
+        if (NBUF > 1) issue(it + AHEAD);
         const int r0 = (blk0 + 2 * it + phase) * 32;
         const unsigned tq = lds0 + buf * 2 * TILE + phase * 32 * TL::kRowBytes, tg = tq + TILE;
-        const unsigned stats = stat0 + buf * 512 + phase * 128;
-        if (r0 >= full.lo && r0 + 32 <= full.hi)
-            grad_keys<T, DP, WHAT, false>(dk, dv, kf, vf, tq, tg, map, stats, r0, by, a.scale_log2, lane);
-        else
-            grad_keys<T, DP, WHAT, true>(dk, dv, kf, vf, tq, tg, map, stats, r0, by, a.scale_log2, lane);
-        if (NBUF == 2) {
-            buf ^= 1;
-            if (it + 1 < it1) put_stat(buf);
+        const RowStats stats = {stat0 + buf * 512 + phase * 128 + (lane >> 5) * 16};
+        if (r0 >= full.lo && r0 + 32 <= full.hi) {
+            GradBlock<T, DP, DV, DK, false, RowStats> blk;
+            blk.run(dk, dv, kf, vf, tq, tg, map, stats, Sees{}, a.scale_log2);
+        } else if (!idle) {
+            if (DV) odd = odd || block_not_finite<T, DP>(tg, 0, lane);
+            if (DK) odd = odd || block_not_finite<T, DP>(tq, 0, lane);
+            GradBlock<T, DP, DV, DK, true, RowStats> blk;
+            blk.run(dk, dv, kf, vf, tq, tg, map, stats, sees(r0), a.scale_log2);
+        }
+    }
+    if (__syncthreads_or(odd)) {                          // then the workgroup does its keys once more, with guarded products
+        zero();
+#pragma unroll 1
+        for (int it = it0; it < it1; ++it) {
+            __syncthreads();
+            stage(it, 0);
+            dma_wait();
+            __syncthreads();
+            const int r0 = (blk0 + 2 * it + phase) * 32;
+            const unsigned tq = lds0 + phase * 32 * TL::kRowBytes, tg = tq + TILE;
+            const RowStats stats = {stat0 + phase * 128 + (lane >> 5) * 16};
+            GradBlock<T, DP, DV, DK, true, RowStats> blk;
+            if (!idle) blk.run_guarded(dk, dv, kf, vf, tq, tg, map, stats, sees(r0), a.scale_log2, lane);
         }
     }
     // the odd blocks' sums join the even ones'
@@ -422,11 +568,10 @@ void backward_keys_kernel(BackwardArgs a, int G, int items) {
     if constexpr (DV) join(dv);
     if (phase == 1 || j >= a.Tk) return;
     float *part = nullptr;
-    if (chunks > 1) {
-        // partial rows lie item by item: first the sink blocks' (if they are shared), then the rest's
-        const long base = a.sink_chunks > 1 ? 0 : sink_items;
-        const long per = items - base - (a.rest_chunks > 1 ? 0 : items - sink_items);
-        part = a.part + ((((long)b * a.Hkv + h) * per + (item - base)) * kBwdKeys + (j - k0)) * (a.Dk + a.Dv);
+    const int slots = block_slots(a, block);
+    if (slots > 1) {
+        const long slot = slots_before(a, block) + (tail ? a.chunks + chunk : chunk);
+        part = a.part + ((((long)b * a.Hkv + h) * slots_before(a, blocks) + slot) * kBwdKeys + (j - k0)) * (a.Dk + a.Dv);
     }
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -455,22 +600,21 @@ void backward_keys_kernel(BackwardArgs a, int G, int items) {
         }
 }
 
-// the chunks of key blocks become their gradients, added in their order: four keys to a workgroup
+// the slots of key blocks become their gradients, added in their order: four keys to a workgroup
 template <typename T>
-__global__ __launch_bounds__(kHeadsThreads) void backward_join_kernel(BackwardArgs a, int block0, int blocks, long item0, int chunks,
-                                                                      long per) {
+__global__ __launch_bounds__(kHeadsThreads) void backward_join_kernel(BackwardArgs a, int blocks, int joined) {
     const int w = a.Dk + a.Dv;
     int id = blockIdx.x;
     const int quad = id % (kBwdKeys / 4);
     id /= kBwdKeys / 4;
-    const int blk = id % blocks;
-    id /= blocks;
-    const int h = id % a.Hkv, b = id / a.Hkv, key = quad * 4 + (threadIdx.x >> 6), j = (block0 + blk) * kBwdKeys + key;
+    const int block = id % joined;
+    id /= joined;
+    const int h = id % a.Hkv, b = id / a.Hkv, key = quad * 4 + (threadIdx.x >> 6), j = block * kBwdKeys + key, slots = block_slots(a, block);
     if (j >= a.Tk) return;
-    const float *src = a.part + ((((long)b * a.Hkv + h) * per + item0 + (long)blk * chunks) * kBwdKeys + key) * w;
+    const float *src = a.part + ((((long)b * a.Hkv + h) * slots_before(a, blocks) + slots_before(a, block)) * kBwdKeys + key) * w;
     for (int c = threadIdx.x & 63; c < w; c += 64) {
         float sum = 0.f;
-        for (int x = 0; x < chunks; ++x) sum += src[(long)x * kBwdKeys * w + c];
+        for (int x = 0; x < slots; ++x) sum += src[(long)x * kBwdKeys * w + c];
         T *row = c < a.Dk ? (T *)row_at(a.dk, b, j, h, sizeof(T)) + c : (T *)row_at(a.dv, b, j, h, sizeof(T)) + (c - a.Dk);
         *row = from_f32<T>(sum);
     }
@@ -531,21 +675,16 @@ void backward(const BackwardArgs &a, hipStream_t s) {
     constexpr int BN = DP * (int)sizeof(T) <= 256 ? 64 : 32;
     const int G = a.Hq / a.Hkv, rows = a.Tq * G, groups = a.B * a.Hkv, tiles = (rows + 127) / 128;
     if (tiles > 0) backward_rows_kernel<T, DP, BN, VEC><<<groups * tiles, kHeadsThreads, 0, s>>>(a, rows, G, tiles);
-    const int blocks = (a.Tk + kBwdKeys - 1) / kBwdKeys, rest = blocks - a.sink_blocks;
-    const int sink_items = a.sink_blocks * a.sink_chunks, items = sink_items + rest * a.rest_chunks;
-    if (items == 0) return;
+    const int blocks = (a.Tk + kBwdKeys - 1) / kBwdKeys, grid = groups * (blocks * a.chunks + a.sink_blocks * a.tail_chunks);
+    if (blocks == 0) return;
     if constexpr (DP > 128) {
-        backward_keys_kernel<T, DP, 1, VEC><<<groups * items, kHeadsThreads, 0, s>>>(a, G, items);
-        backward_keys_kernel<T, DP, 2, VEC><<<groups * items, kHeadsThreads, 0, s>>>(a, G, items);
+        backward_keys_kernel<T, DP, 1, VEC><<<grid, kHeadsThreads, 0, s>>>(a, G, blocks);
+        backward_keys_kernel<T, DP, 2, VEC><<<grid, kHeadsThreads, 0, s>>>(a, G, blocks);
     } else {
-        backward_keys_kernel<T, DP, 3, VEC><<<groups * items, kHeadsThreads, 0, s>>>(a, G, items);
+        backward_keys_kernel<T, DP, 3, VEC><<<grid, kHeadsThreads, 0, s>>>(a, G, blocks);
     }
-    const long base = a.sink_chunks > 1 ? 0 : sink_items, per = items - base - (a.rest_chunks > 1 ? 0 : items - sink_items);
-    constexpr int quads = kBwdKeys / 4;
-    if (a.sink_chunks > 1 && a.sink_blocks > 0)
-        backward_join_kernel<T><<<groups * a.sink_blocks * quads, kHeadsThreads, 0, s>>>(a, 0, a.sink_blocks, 0, a.sink_chunks, per);
-    if (a.rest_chunks > 1 && rest > 0)
-        backward_join_kernel<T><<<groups * rest * quads, kHeadsThreads, 0, s>>>(a, a.sink_blocks, rest, sink_items - base, a.rest_chunks, per);
+    const int joined = a.chunks > 1 ? blocks : a.tail_chunks > 0 ? a.sink_blocks : 0;
+    if (joined > 0) backward_join_kernel<T><<<groups * joined * (kBwdKeys / 4), kHeadsThreads, 0, s>>>(a, blocks, joined);
 }
 template <typename T, int DP>
 void backward(const BackwardArgs &a, hipStream_t s) {

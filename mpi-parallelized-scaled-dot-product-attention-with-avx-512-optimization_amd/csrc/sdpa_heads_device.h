@@ -401,6 +401,16 @@ __device__ inline void lds_dma(const char *base, unsigned lane_off, unsigned lds
                  : "memory" SDPA_M0_CLOBBER);
 }
 
+// 4 bytes a lane: 64 consecutive words
+__device__ inline void lds_dma_words(const void *base, int lane, unsigned lds_byte) {
+    asm volatile("s_mov_b32 m0, %1\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dword %0, %2"
+                 :
+                 : "v"(lane * 4), "s"(__builtin_amdgcn_readfirstlane(lds_byte)), "s"(uniform((const char *)base))
+                 : "memory" SDPA_M0_CLOBBER);
+}
+
 // A tile of ROWS rows of a key list, staged by WAVES waves.  Rows behind the list's end are read as its last key (their weights are
 // masked), so that nothing is read that no query of the workgroup sees.
 // The waves take the tile's 1 KiB pieces in turn: with four waves a wave's pieces lie 4 KiB apart, where the swizzle (period 16
