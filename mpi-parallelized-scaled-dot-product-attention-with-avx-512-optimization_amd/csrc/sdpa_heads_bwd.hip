@@ -265,24 +265,36 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
         return Sees{seen.hi - at, seen.lo - at, f.sinks - at};
     };
     bool odd = false;                                    // a block with masked pairs holds values that are no numbers
-#pragma unroll 1
-    for (int it = 0, buf = 0; it < count; ++it, buf ^= 1) {
+    // Blocks in order, those without a masked pair in a loop of their own: with both kinds in one loop the compiler keeps the accumulators in
+    // different registers on the two paths and moves all of them in every turn.
+    constexpr int PER = BN / 32;
+    const int total = count * PER;
+    auto arrive = [&](int e) {
+        if (e % PER != 0) return;
         dma_wait();
         __syncthreads();
-        if (it + 1 < count) stage(it + 1, buf ^ 1);
+        if (e / PER + 1 < count) stage(e / PER + 1, (e / PER + 1) & 1);
+    };
+    auto tile_of = [&](int e) { return lds0 + (e / PER & 1) * 2 * TILE + e % PER * 32 * TL::kRowBytes; };
+    auto whole = [&](int e) { return sees_all(wv, list.frame(e * 32, 32), 32); };
+    int e = 0;
+    while (e < total) {
 #pragma unroll 1
-        for (int n = 0; n < BN / 32; ++n) {
-            const Frame f = list.frame(it * BN + n * 32, 32);
+        for (; e < total && !whole(e); ++e) {
+            arrive(e);
+            const Frame f = list.frame(e * 32, 32);
             if (!sees_some(wv, f, 32)) continue;
-            const unsigned tk = lds0 + buf * 2 * TILE + n * 32 * TL::kRowBytes, tv = tk + TILE;
-            if (sees_all(wv, f, 32)) {
-                GradBlock<T, DP, false, true, false, ColumnStats> blk;
-                blk.run(dq, nullptr, q, g, tk, tv, map, stats, Sees{}, a.scale_log2);
-            } else {
-                odd = odd || block_not_finite<T, DP>(tk, 0, lane);
-                GradBlock<T, DP, false, true, true, ColumnStats> blk;
-                blk.run(dq, nullptr, q, g, tk, tv, map, stats, sees(f), a.scale_log2);
-            }
+            const unsigned tk = tile_of(e), tv = tk + TILE;
+            odd = odd || block_not_finite<T, DP>(tk, 0, lane);
+            GradBlock<T, DP, false, true, true, ColumnStats> blk;
+            blk.run(dq, nullptr, q, g, tk, tv, map, stats, sees(f), a.scale_log2);
+        }
+#pragma unroll 1
+        for (; e < total && whole(e); ++e) {
+            arrive(e);
+            const unsigned tk = tile_of(e), tv = tk + TILE;
+            GradBlock<T, DP, false, true, false, ColumnStats> blk;
+            blk.run(dq, nullptr, q, g, tk, tv, map, stats, Sees{}, a.scale_log2);
         }
     }
     if (__syncthreads_or(odd)) {                          // then the workgroup does its rows once more, with guarded products
@@ -503,9 +515,7 @@ void backward_keys_kernel(BackwardArgs a, int G, int blocks) {
     };
     zero();
     bool odd = false;                                    // a block with masked pairs holds values that are no numbers
-#pragma unroll 1
-    for (int it = it0; it < it1; ++it) {
-        const int buf = (it - it0) % NBUF;
+    auto arrive = [&](int it) {
         if (NBUF == 1) {
             __syncthreads();
             stage(it, 0);
@@ -518,28 +528,40 @@ void backward_keys_kernel(BackwardArgs a, int G, int blocks) {
         else dma_wait();
         __syncthreads();
         if (NBUF > 1) issue(it + AHEAD);
-        const int r0 = (blk0 + 2 * it + phase) * 32;
-        const unsigned tq = lds0 + buf * 2 * TILE + phase * 32 * TL::kRowBytes, tg = tq + TILE;
-        const RowStats stats = {stat0 + buf * 512 + phase * 128 + (lane >> 5) * 16};
-        if (r0 >= full.lo && r0 + 32 <= full.hi) {
-            GradBlock<T, DP, DV, DK, false, RowStats> blk;
-            blk.run(dk, dv, kf, vf, tq, tg, map, stats, Sees{}, a.scale_log2);
-        } else if (!idle) {
+    };
+    auto first_row = [&](int it) { return (blk0 + 2 * it + phase) * 32; };
+    auto whole = [&](int it) { return first_row(it) >= full.lo && first_row(it) + 32 <= full.hi; };
+    auto tile_of = [&](int it) { return lds0 + (it - it0) % NBUF * 2 * TILE + phase * 32 * TL::kRowBytes; };
+    auto stats_of = [&](int it) { return RowStats{stat0 + (it - it0) % NBUF * 512 + phase * 128 + (lane >> 5) * 16}; };
+    int it = it0;
+    while (it < it1) {                                    // (two loops: see the rows kernel)
+#pragma unroll 1
+        for (; it < it1 && !whole(it); ++it) {
+            arrive(it);
+            if (idle) continue;
+            const unsigned tq = tile_of(it), tg = tq + TILE;
             if (DV) odd = odd || block_not_finite<T, DP>(tg, 0, lane);
             if (DK) odd = odd || block_not_finite<T, DP>(tq, 0, lane);
             GradBlock<T, DP, DV, DK, true, RowStats> blk;
-            blk.run(dk, dv, kf, vf, tq, tg, map, stats, sees(r0), a.scale_log2);
+            blk.run(dk, dv, kf, vf, tq, tg, map, stats_of(it), sees(first_row(it)), a.scale_log2);
+        }
+#pragma unroll 1
+        for (; it < it1 && whole(it); ++it) {
+            arrive(it);
+            const unsigned tq = tile_of(it), tg = tq + TILE;
+            GradBlock<T, DP, DV, DK, false, RowStats> blk;
+            blk.run(dk, dv, kf, vf, tq, tg, map, stats_of(it), Sees{}, a.scale_log2);
         }
     }
     if (__syncthreads_or(odd)) {                          // then the workgroup does its keys once more, with guarded products
         zero();
 #pragma unroll 1
-        for (int it = it0; it < it1; ++it) {
+        for (it = it0; it < it1; ++it) {
             __syncthreads();
             stage(it, 0);
             dma_wait();
             __syncthreads();
-            const int r0 = (blk0 + 2 * it + phase) * 32;
+            const int r0 = first_row(it);
             const unsigned tq = lds0 + phase * 32 * TL::kRowBytes, tg = tq + TILE;
             const RowStats stats = {stat0 + phase * 128 + (lane >> 5) * 16};
             GradBlock<T, DP, DV, DK, true, RowStats> blk;
