@@ -166,11 +166,11 @@ BackwardPlan plan_backward(const sdpa_heads *a) {
     const long sinks = a->sinks < a->kv_tokens ? a->sinks : a->kv_tokens, reach = (long)a->window + kBwdKeys;
     const long walk = (reach < a->q_tokens ? reach : a->q_tokens) * G, tail = reach < a->q_tokens ? (a->q_tokens - reach) * G : 0;
     long chunks = groups * blocks < 256 ? ceil_div(256, groups * blocks < 1 ? 1 : groups * blocks) : 1;
-    if (chunks > ceil_div(walk, 256)) chunks = ceil_div(walk, 256);
+    if (chunks > ceil_div(walk, 128)) chunks = ceil_div(walk, 128);
     if (chunks > kMaxSplits) chunks = kMaxSplits;
     p.chunks = chunks < 1 ? 1 : (int)chunks;
     p.sink_blocks = (int)ceil_div(sinks, kBwdKeys);
-    const long piece = walk / (4 * p.chunks) > 512 ? walk / (4 * p.chunks) : 512;
+    const long piece = walk / (4 * p.chunks) > 128 ? walk / (4 * p.chunks) : 128;
     const long tails = ceil_div(tail, piece);
     p.tail_chunks = p.sink_blocks == 0 ? 0 : (int)(tails < kMaxSplits ? tails : kMaxSplits);
     p.grid = (double)groups * (blocks * p.chunks + p.sink_blocks * p.tail_chunks);
