@@ -36,11 +36,14 @@ int check_shape(const sdpa_heads *a) {
 int check_attention(const sdpa_heads *a) {
     SDPA_TRY(check_shape(a));
     if (a->q_heads < 1 || a->q_heads % a->kv_heads != 0) return SDPA_EINVAL;
-    if (a->window < 0 || a->sinks < 0 || a->prefix_tokens < 0 || !(a->scale == a->scale)) return SDPA_EINVAL;
+    if (a->window < 0 || a->sinks < 0 || a->prefix_tokens < 0 || !isfinite(a->scale)) return SDPA_EINVAL;
     if (a->prefix_tokens > kMaxTokens) return SDPA_EUNSUP;
-    // a launch has less than 2^32 threads: 256 for each row of the join (where keys are split), for each 128 keys or rows of a head
-    const double rows = (double)a->batch * a->q_tokens * a->q_heads, groups = (double)a->batch * a->kv_heads;
-    if (rows > kMaxRows || groups * (ceil_div(a->kv_tokens, 128) + 1) > kMaxGroups) return SDPA_EUNSUP;
+    // a launch has less than 2^32 threads: 256 for each 128 keys or rows of a head, and for each row of a join.  Of the forward forms only
+    // few rows are split and joined, and those beside a prefix, whose rows are one tile list for the batch.
+    const double groups = (double)a->batch * a->kv_heads, rows = (double)a->q_tokens * (a->q_heads / a->kv_heads);
+    if (rows > kMaxRows || groups * (ceil_div(a->kv_tokens, 128) + 1) > kMaxGroups || groups * (rows / 128 + 1) > kMaxGroups ||
+        (a->prefix_tokens > 0 && groups * rows > kMaxRows))
+        return SDPA_EUNSUP;
     return SDPA_OK;
 }
 
@@ -155,7 +158,7 @@ int run_own(const sdpa_heads *a, const Slots &s, void *workspace, hipStream_t st
     return SDPA_OK;
 }
 
-struct BackwardPlan { int chunks, sink_blocks, tail_chunks; long stat_rows, stats, bytes; double grid; };
+struct BackwardPlan { int chunks, sink_blocks, tail_chunks; long stat_rows, stats, bytes; double grid; };     // grid: the largest launch
 
 // A key block's workgroup walks the rows that see it by the window, about (64 + window) tokens' heads; several share them while the launch
 // has fewer workgroups than the chip has CUs.  A block with sink keys is seen by every row behind: its tail goes to short workgroups
@@ -173,7 +176,9 @@ BackwardPlan plan_backward(const sdpa_heads *a) {
     const long piece = walk / (4 * p.chunks) > 128 ? walk / (4 * p.chunks) : 128;
     const long tails = ceil_div(tail, piece);
     p.tail_chunks = p.sink_blocks == 0 ? 0 : (int)(tails < kMaxSplits ? tails : kMaxSplits);
+    const long joined = p.chunks > 1 ? blocks : p.tail_chunks > 0 ? p.sink_blocks : 0;
     p.grid = (double)groups * (blocks * p.chunks + p.sink_blocks * p.tail_chunks);
+    if ((double)groups * joined * (kBwdKeys / 4) > p.grid) p.grid = (double)groups * joined * (kBwdKeys / 4);     // (the join's)
     const long slots = p.chunks > 1 ? blocks * p.chunks + p.sink_blocks * p.tail_chunks :
                        p.tail_chunks > 0 ? p.sink_blocks * (1 + p.tail_chunks) : 0;
     // rows of a head: blocks of 32, whole tokens to a block (or, of larger groups, blocks to a token), in pairs

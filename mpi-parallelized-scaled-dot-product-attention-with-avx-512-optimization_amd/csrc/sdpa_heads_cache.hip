@@ -170,9 +170,11 @@ hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
     const int groups = a.B * a.H;
     if (a.Tk <= heads::kSelectLocal) {
         const size_t bytes = (size_t)a.Tk * 4;
-        static const hipError_t wide = hipFuncSetAttribute((const void *)heads::select_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                           heads::kSelectLocal * 4);
-        if (wide != hipSuccess) return wide;
+        if (bytes > 32768) {                             // (an attribute of the device's function: not kept for the process)
+            const hipError_t e = hipFuncSetAttribute((const void *)heads::select_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                     heads::kSelectLocal * 4);
+            if (e != hipSuccess) return e;
+        }
         heads::select_kernel<true><<<groups, heads::kSelectThreads, bytes, s>>>(a);
     } else {
         heads::select_kernel<false><<<groups, heads::kSelectThreads, 0, s>>>(a);

@@ -93,6 +93,12 @@ def _apart(outs, ins, name):
             _need(a1 <= b0 or b1 <= a0, "%s: an output overlaps an input" % name)
 
 
+def _distinct(outs, name):
+    """... nor begin where another output does (parts of one packed tensor may lie between each other)"""
+    at = [x.data_ptr() for x in outs if x is not None and x.numel() > 0]
+    _need(len(set(at)) == len(at), "%s: two outputs are the same memory" % name)
+
+
 def _lens(x, name, batch, like):
     """lengths (None = all); accepted at once where all is well, as in the other checks a small call meets"""
     if x is None or (type(x) is torch.Tensor and x.dtype is torch.int32 and x.shape == (batch,) and x.device == like.device and
@@ -158,6 +164,7 @@ def _outputs(q, Dv, out, lse, ins, name):
         _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
         _need(lse.is_contiguous(), "lse: must be contiguous")
         _apart([lse], ins, name)
+        _distinct((out, lse), name)
     _on_gpu(q, name)
     if out is None:
         out = q.new_empty((B, Tq, Hq, Dv))
@@ -199,6 +206,7 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
         if x is not None:
             _rows(x, n, like.shape, q.dtype, q.device)
             _apart([x], ins, name)
+            _distinct((dq, dk, dv), name)
     _on_gpu(q, name)
     dq = q.new_empty(q.shape) if dq is None else dq
     dk = q.new_empty(k.shape) if dk is None else dk
@@ -255,7 +263,7 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
     elif weights_out is not weights:
         _weights(weights_out, "weights_out", (B, Hkv, Tk), q, True)
         _apart([weights_out], (q, k, v, weights), name)
-    out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights), name)
+    out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights, weights_out), name)
     args = _PACK_SCORED.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), *_sums(weights, weights_out),
                              _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q, args)
@@ -293,6 +301,10 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
               "weights_out: needs %d tokens" % budget)
         _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k, True)
         _apart([weights_out], ins, name)
+    if k_out is not None:
+        _distinct((k_out, v_out, weights_out), name)
+    elif v_out is not None:
+        _distinct((v_out, weights_out), name)
     _on_gpu(k, name)
     k_out = k.new_empty((B, budget, H, Dk)) if k_out is None else k_out
     v_out = k.new_empty((B, budget, H, Dv)) if v_out is None else v_out

@@ -29,7 +29,7 @@ def attention(q, k, v, see, scale, dtype):
     """one head: q [nq, dk], k [nk, dk], v [nk, dv] -> out, lse, weights P, and the bounds of out, lse, P's relative error"""
     s = scale * (q @ k.T)
     nq, nk = s.shape
-    ds = (q.shape[1] + 4) * F32 * scale * (np.abs(q) @ np.abs(k).T)
+    ds = (q.shape[1] + 4) * F32 * abs(scale) * (np.abs(q) @ np.abs(k).T)
     p = np.zeros_like(s)
     lse = np.full(nq, -np.inf)
     err = np.zeros(nq)                                     # a row's relative error of any weight
@@ -64,8 +64,8 @@ def gradients(q, k, v, dout, p, out, err, scale, dtype):
                                                w * (p @ np.abs(v) * np.abs(dout)).sum(1, keepdims=True))
     dq, dk, dv = scale * ds @ k, scale * ds.T @ q, p.T @ dout
     a = np.abs
-    tq = u * a(dq) + scale * (e + n * F32 * a(ds)) @ a(k) + 1e-30
-    tk = scale * (e + n * F32 * a(ds)).T @ a(q) + 1e-30          # (the group's sum is rounded once: the caller adds u |dk|)
+    tq = u * a(dq) + abs(scale) * (e + n * F32 * a(ds)) @ a(k) + 1e-30
+    tk = abs(scale) * (e + n * F32 * a(ds)).T @ a(q) + 1e-30          # (the group's sum is rounded once: the caller adds u |dk|)
     tv = (p * (w + err[:, None] + n * F32)).T @ a(dout) + 1e-30
     return dq, dk, dv, tq, tk, tv
 

@@ -122,10 +122,11 @@ def test_window_backward(c, pkg):
     check_gradients(q, k, v, dout, dq, dk, dv, ql, kl, window, sinks, dtype)
 
 
-def check_gradients(q, k, v, dout, dq, dk, dv, ql, kl, window, sinks, dtype):
+def check_gradients(q, k, v, dout, dq, dk, dv, ql, kl, window, sinks, dtype, scale=None):
     B, Tq, Hq, Dk = q.shape
     Hkv = k.shape[2]
-    G, scale, u = Hq // Hkv, Dk ** -0.5, ref.half_step(dtype)
+    G, u = Hq // Hkv, ref.half_step(dtype)
+    scale = Dk ** -0.5 if scale is None else scale
     _, _, _, _, heads = reference(q, k, v, ql, kl, window, sinks, scale, dtype)
     Q, K, V, D = f64(q), f64(k), f64(v), f64(dout)
     wq, wk, wv = np.zeros(Q.shape), np.zeros(K.shape), np.zeros(V.shape)

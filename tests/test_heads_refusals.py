@@ -43,6 +43,24 @@ def test_outputs_over_inputs_are_refused(pkg):
         pkg.evict_cache(k, v, w, None, 4, weights_out=w)
 
 
+def test_one_tensor_for_two_outputs_is_refused(pkg):
+    q, kv = torch.zeros(2, 3, 2, 8), torch.zeros(2, 3, 2, 8)
+    o, lse, g = torch.zeros(2, 3, 2, 8), torch.zeros(2, 2, 3), torch.zeros(2, 3, 2, 8)
+    w = torch.zeros(2, 2, 3)
+    for kw in (dict(dq=g, dk=g), dict(dk=g, dv=g), dict(dq=g, dv=g)):
+        with pytest.raises(ValueError, match="two outputs"):
+            pkg.attention_window_backward(g.clone(), q, kv, kv, o, lse, 4, **kw)
+    flat = torch.zeros(200)
+    with pytest.raises(ValueError, match="two outputs"):
+        pkg.attention_window(q, kv, kv, 4, out=flat[:96].view(2, 3, 2, 8), lse=flat[:12].view(2, 2, 3))
+    with pytest.raises(ValueError, match="overlap"):
+        pkg.attention_scored(q, kv, kv, w, weights_out=flat[:12].view(2, 2, 3), lse=flat[:12].view(2, 2, 3))
+    with pytest.raises(ValueError, match="two outputs"):
+        pkg.evict_cache(kv, kv, w, None, 2, k_out=g, v_out=g)
+    with pytest.raises(ValueError, match="two outputs"):
+        pkg.evict_cache(kv, kv, w, None, 2, v_out=flat[:96].view(2, 3, 2, 8), weights_out=flat[:12].view(2, 2, 3))
+
+
 @pytest.mark.parametrize("kw", [dict(dout=torch.zeros(2, 3, 4, 8)), dict(out=torch.zeros(2, 3, 4, 6, dtype=torch.bfloat16)),
                                 dict(lse=torch.zeros(2, 3, 4)), dict(dq=torch.zeros(2, 3, 4, 6)), dict(dv=torch.zeros(2, 5, 2, 8))],
                          ids=lambda kw: "-".join(kw))
@@ -130,7 +148,8 @@ def test_c_entries_refuse(op, kw, code, pkg):
 
 @pytest.mark.parametrize("op,kw,code", [
     (0, dict(q_heads=3), -1), (0, dict(window=-1), -1), (0, dict(lse=0), -1), (0, dict(out=(4096, 0, 24, 6)), -1), (0, dict(scale=float("nan")), -1),
-    (1, dict(dq=(0, 96, 32, 8)), -1), (1, dict(dv_out=(4096, 60, 0, 6)), -1), (1, dict(dout=(0, 1, 1, 1)), -1), (2, dict(prefix=4), -1),
+    (0, dict(scale=float("inf")), -1), (3, dict(scale=float("-inf")), -1), (2, dict(prefix=4, kp=(4096, 0, 8, 8), vp=(4096, 0, 8, 6), q_tokens=1 << 22), -6),
+    (0, dict(q_tokens=1 << 24), -6), (1, dict(batch=1 << 20, kv_tokens=64, sinks=4, q_tokens=200), -6), (1, dict(dq=(0, 96, 32, 8)), -1), (1, dict(dv_out=(4096, 60, 0, 6)), -1), (1, dict(dout=(0, 1, 1, 1)), -1), (2, dict(prefix=4), -1),
     (2, dict(prefix=-1), -1), (3, dict(weights=0), -1), (3, dict(ws=(10, 5, -1, 5)), -1), (4, dict(budget=1), -1), (4, dict(kept=0), -1),
     (4, dict(lens_out=0), -1), (4, dict(k_out=(4096, 64, 0, 8)), -1), (0, dict(batch=1 << 20, q_tokens=1 << 20), -6)], ids=str)
 def test_c_entries_refuse_their_own(op, kw, code, pkg):
