@@ -1,6 +1,6 @@
 // sdpa_heads_bwd.hip -- gradients of attention_window, and the weights every key was given (attention_scored).
 //
-//     P = exp(s - lse) on visible pairs, dP = dO V^T, delta_i = sum_d dO_id O_id, dS = P * (dP - delta)
+//     P = exp(s - lse) on visible pairs, dP = dO V^T, delta_i = sum_d dO_id O_id = sum_j P_ij dP_ij, dS = P * (dP - delta)
 //     dV = P^T dO      dK = scale dS^T Q (both summed over the G heads that share them)      dQ = scale dS K
 //
 // Two kernels, no atomics: one whose workgroups own query rows (dQ, and delta on the way), one whose workgroups own keys (dK, dV)
@@ -182,6 +182,28 @@ struct RowBlocks {
     __device__ bool used(int block, int i) const { return split > 1 ? head(block, i) < G : i < tokens * G; }
 };
 
+// delta of rows that see few keys, as the sum of P dP it stands for: sum dO * O takes O as it was rounded, which a mean over many keys
+// hides and one over few does not (bf16, 15 to 40 keys a row: dQ and dK off by 0.0027 to 0.0034 of their norms, 0.0024 with the sum, which
+// is what rounding dS leaves; 150 keys: 0.0026).  One walk more over tiles that lie in the L2.
+constexpr int kDeltaKeys = 512;
+template <typename T, int DP>
+__device__ inline float weighted_sum(const typename Ops<T>::Frag *q, const typename Ops<T>::Frag *g, unsigned tk, unsigned tv,
+                                     const LaneMap<T, DP> &map, float lse2, Sees see, float scale) {
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int i = 0; i < DP / Ops<T>::kStep; ++i) s = Ops<T>::mma(read_rows<T, DP>(tk + map.rows, 0, i), q[i], s);
+#pragma unroll
+    for (int i = 0; i < DP / Ops<T>::kStep; ++i) dp = Ops<T>::mma(read_rows<T, DP>(tv + map.rows, 0, i), g[i], dp);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = row_of(i, 0);
+        const bool seen = r < see.hi && (r >= see.lo || r < see.sk);
+        sum += seen ? __builtin_amdgcn_exp2f(s[i] * scale - lse2) * dp[i] : 0.f;
+    }
+    return sum;
+}
+
 // ---- dQ: 128 rows to a workgroup, 32 to a wave -------------------------------------------------------------------------
 template <typename T, int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kHeadsThreads, DP * (int)sizeof(T) <= 256 ? 2 : 1)
@@ -225,8 +247,36 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
     typename Ops<T>::Frag q[STEPS], g[STEPS];
     load_row<T, DP>(q, row_at(a.q, b, t, hq, sizeof(T)), a.Dk, live, a.vec, lane);
     load_row<T, DP>(g, row_at(a.dout, b, t, hq, sizeof(T)), a.Dv, live, a.vec, lane);
+    const long at = ((long)b * a.Hq + hq) * a.Tq + t;
+    const float lse2 = live ? a.lse[at] * kLog2e : __builtin_inff();     // (a row that does not exist: weight 2^(0 - inf) = 0)
+    LaneMap<T, DP> map;
+    map.init(lane);
+    auto sees = [&](Frame f) {
+        const int at = f.j0 + 4 * (opaque(lane) >> 5);
+        return Sees{seen.hi - at, seen.lo - at, f.sinks - at};
+    };
     float delta = 0.f;
-    {
+    if (sizeof(T) == 2 && list.n <= kDeltaKeys) {        // (the first tile is on its way)
+#pragma unroll 1
+        for (int it = 0; it < count; ++it) {
+            if (it > 0) {
+                __syncthreads();
+                stage(it, 0);
+            }
+            dma_wait();
+            __syncthreads();
+#pragma unroll 1
+            for (int n = 0; n < BN / 32; ++n) {
+                const Frame f = list.frame(it * BN + n * 32, 32);
+                if (!sees_some(wv, f, 32)) continue;
+                const unsigned tk = lds0 + n * 32 * TL::kRowBytes;
+                delta += weighted_sum<T, DP>(q, g, tk, tk + TILE, map, lse2, sees(f), a.scale_log2);
+            }
+        }
+        delta = half_sum(delta);
+        __syncthreads();
+        if (count > 1) stage(0, 0);
+    } else {
         const T *row = (const T *)row_at(a.out, b, t, hq, sizeof(T));
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -238,8 +288,6 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
         }
         delta = half_sum(delta);
     }
-    const long at = ((long)b * a.Hq + hq) * a.Tq + t;
-    const float lse2 = live ? a.lse[at] * kLog2e : __builtin_inff();     // (a row that does not exist: weight 2^(0 - inf) = 0)
     if (r < rows && lane < 32) {                         // for the keys kernel, in the order it walks the rows
         const RowBlocks rb(G);
         const int g = r - t * G, place = rb.row(t) + g;
@@ -257,13 +305,7 @@ void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-    LaneMap<T, DP> map;
-    map.init(lane);
     const ColumnStats stats = {lse2, -delta};
-    auto sees = [&](Frame f) {
-        const int at = f.j0 + 4 * (opaque(lane) >> 5);
-        return Sees{seen.hi - at, seen.lo - at, f.sinks - at};
-    };
     bool odd = false;                                    // a block with masked pairs holds values that are no numbers
     // Blocks in order, those without a masked pair in a loop of their own: with both kinds in one loop the compiler keeps the accumulators in
     // different registers on the two paths and moves all of them in every turn.
