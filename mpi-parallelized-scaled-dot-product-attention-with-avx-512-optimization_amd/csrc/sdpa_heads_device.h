@@ -78,18 +78,31 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// 16 bytes of a row: elements [d0, d0 + kVec), zero from `dim` on
+// 16 bytes of a row: elements [d0, d0 + kVec), zero from `dim` on.  `vec`: the row is 16-byte aligned and whole.  Others, in
+// bf16, are read in one load too (at their elements' alignment, which global loads allow), but for the row's last piece, whose elements are
+// read at once: two sequences of 1024 tokens, 8 heads of 100 columns, window 300, backward 207 us (element by element throughout: 331).  For
+// fp32's four elements that gains 5 % and costs the widest heads registers.
 template <typename T> __device__ inline u32x4 load_chunk(const T *row, int d0, int dim, bool vec) {
     constexpr int N = Ops<T>::kVec;
     u32x4 r = {0, 0, 0, 0};
     if (vec) {
         if (d0 < dim) r = *reinterpret_cast<const u32x4 *>(row + d0);
-    } else {
+    } else if (sizeof(T) == 4) {
         union { T e[N]; u32x4 u; } x;
         x.u = r;
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (d0 + i < dim) x.e[i] = row[d0 + i];
+        r = x.u;
+    } else if (d0 + N <= dim) {
+        __builtin_memcpy(&r, row + d0, 16);
+    } else if (d0 < dim) {
+        union { T e[N]; u32x4 u; } x;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x.e[i] = row[min(d0 + i, dim - 1)];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (d0 + i >= dim) x.e[i] = T(0.f);
         r = x.u;
     }
     return r;
