@@ -124,25 +124,28 @@ __device__ inline void weigh(State<DP> &st, f32x16 *s, Probs<T> *p, float ref, f
     st.l += sum;
 }
 
-template <typename T, int DP, int NB, bool MASKED>
+// the lane's row of kept scores, at this tile
+template <int NB> __device__ inline void keep_scores(float *keep, const f32x16 *s, int lane) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f32x4 *>(keep + n * 32 + 8 * i + 4 * (lane >> 5)) = f32x4{s[n][4 * i], s[n][4 * i + 1], s[n][4 * i + 2], s[n][4 * i + 3]};
+}
+
+// a tile with masked pairs, guarded
+template <typename T, int DP, int NB>
 __device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag *q, unsigned lk, unsigned lv, const LaneMap<T, DP> &map,
-                                     int j0, Seen seen, int sinks, float scale, int lane, float *keep = nullptr) {
+                                     int j0, Seen seen, int sinks, float scale, int lane) {
     f32x16 s[NB];
     scores<T, DP, NB>(s, q, lk, map);
-    if (MASKED) hide<NB>(s, j0, seen, sinks, true, lane);
-    if (keep) {                                         // the lane's row of kept scores, at this tile
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f32x4 *>(keep + n * 32 + 8 * i + 4 * (lane >> 5)) = f32x4{s[n][4 * i], s[n][4 * i + 1], s[n][4 * i + 2], s[n][4 * i + 3]};
-    }
+    hide<NB>(s, j0, seen, sinks, true, lane);
     const float ref = raise<DP>(st, largest<NB>(s), scale);
     Probs<T> p[NB];
     weigh<T, DP, NB>(st, s, p, ref, scale);
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-        if (MASKED && __builtin_expect(block_not_finite<T, DP>(lv, n, lane), 0))
+        if (__builtin_expect(block_not_finite<T, DP>(lv, n, lane), 0))
             mma_block_guarded<T, DP, DP / 32>(st.o, lv, map, n, p[n], seen_bits(j0 + n * 32, seen, sinks, lane), 3);
         else
             mma_block<T, DP, DP / 32>(st.o, lv, map, n, p[n], false, 0u, 3, lane);
@@ -380,7 +383,7 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
             __syncthreads();
             const Frame f = list.frame(it * BN, BN);
             if (sees_some(wv, f, BN))
-                attend_blocks<T, DP, NB, true>(st, q, lds0, lds0 + 2 * TILE, map, f.j0, seen, f.sinks, a.scale_log2, lane);
+                attend_blocks<T, DP, NB>(st, q, lds0, lds0 + 2 * TILE, map, f.j0, seen, f.sinks, a.scale_log2, lane);
         }
     }
     st.l = half_sum(st.l);
@@ -475,6 +478,9 @@ __global__ __launch_bounds__((FewShape<T, DP, WIDE>::kWaves * 64)) void attend_f
     map.init(lane);
     // (kept scores: the row of a lane that has one; the list of attention_scored is the cache itself)
     float *kept = a.scores && (lane & 31) < rows ? a.scores + (((long)b * a.Hkv + h) * rows + (lane & 31)) * a.score_ld : nullptr;
+    // One way through the products for masked tiles and others: a second one would have the accumulators in other registers, and heads of
+    // 256 columns in scratch memory (16 tokens, 8 heads on 2 of 256 columns, XXFEW256).
+    bool odd = false;                                    // a tile with masked pairs holds values that are no numbers
 #pragma unroll 1
     for (int it = it0 + wave, buf = 0; it < it1; it += WAVES) {
         bool exact = false;
@@ -485,11 +491,32 @@ __global__ __launch_bounds__((FewShape<T, DP, WIDE>::kWaves * 64)) void attend_f
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (a wave reads only what it staged itself)
         const unsigned lk = lds0 + buf * 2 * TILE, lv = lk + TILE;
         const Frame f = list.frame(it * 32, 32);
-        float *keep = kept ? kept + it * 32 : nullptr;
-        if (sees_all(wg, f, 32)) attend_blocks<T, DP, 1, false>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane, keep);
-        else attend_blocks<T, DP, 1, true>(st, q, lk, lv, map, f.j0, seen, f.sinks, a.scale_log2, lane, keep);
+        const bool masked = !sees_all(wg, f, 32);
+        f32x16 s[1];
+        scores<T, DP, 1>(s, q, lk, map);
+        if (masked) {
+            hide<1>(s, f.j0, seen, f.sinks, true, lane);
+            odd = odd || block_not_finite<T, DP>(lv, 0, lane);
+        }
+        if (kept) keep_scores<1>(kept + it * 32, s, lane);
+        const float ref = raise<DP>(st, largest<1>(s), a.scale_log2);
+        Probs<T> p[1];
+        weigh<T, DP, 1>(st, s, p, ref, a.scale_log2);
+        mma_block<T, DP, DP / 32>(st.o, lv, map, 0, p[0], false, 0u, 3, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // (its reads are over before the tile is written again)
         if (NBUF == 2) buf ^= 1;
+    }
+    if (odd) {                                           // then the wave does its tiles once more, with guarded products
+        st.clear();
+#pragma unroll 1
+        for (int it = it0 + wave; it < it1; it += WAVES) {
+            stage(it, 0);
+            dma_wait();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const Frame f = list.frame(it * 32, 32);
+            attend_blocks<T, DP, 1>(st, q, lds0, lds0 + TILE, map, f.j0, seen, f.sinks, a.scale_log2, lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
     }
     st.l = half_sum(st.l);
     if (!x.live) { st.m = kNegInf; st.l = 0.f; }         // (blocks that need no mask gave weights to rows that do not exist)
