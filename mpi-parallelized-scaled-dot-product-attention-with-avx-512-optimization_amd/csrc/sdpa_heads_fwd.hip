@@ -479,7 +479,7 @@ __global__ __launch_bounds__((FewShape<T, DP, WIDE>::kWaves * 64)) void attend_f
     // (kept scores: the row of a lane that has one; the list of attention_scored is the cache itself)
     float *kept = a.scores && (lane & 31) < rows ? a.scores + (((long)b * a.Hkv + h) * rows + (lane & 31)) * a.score_ld : nullptr;
     // One way through the products for masked tiles and others: a second one would have the accumulators in other registers, and heads of
-    // 256 columns in scratch memory (16 tokens, 8 heads on 2 of 256 columns, XXFEW256).
+    // 256 columns in scratch memory (8 tokens against 2048 keys, 8 heads on 2 of 256 columns, the call: bf16 27 us against 37, fp32 91 against 101).
     bool odd = false;                                    // a tile with masked pairs holds values that are no numbers
 #pragma unroll 1
     for (int it = it0 + wave, buf = 0; it < it1; it += WAVES) {
