@@ -22,6 +22,10 @@ bool repeats(const sdpa_tensor &t, int batch, int tokens, int heads) {
     return (batch > 1 && t.batch == 0) || (tokens > 1 && t.token == 0) || (heads > 1 && t.head == 0);
 }
 
+bool repeats_weights(const sdpa_heads *a) {
+    return (a->batch > 1 && a->weights_out_batch == 0) || (a->kv_heads > 1 && a->weights_out_head == 0);
+}
+
 long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 int check_shape(const sdpa_heads *a) {
@@ -199,6 +203,7 @@ int check_evict(const sdpa_heads *a) {
         return SDPA_EINVAL;
     if ((in && !a->weights) || (out && (!a->weights_out || !a->kept)) || !a->lens_out) return SDPA_EINVAL;
     if (a->weights_batch < 0 || a->weights_head < 0 || a->weights_out_batch < 0 || a->weights_out_head < 0) return SDPA_EINVAL;
+    if (out && repeats_weights(a)) return SDPA_EINVAL;
     if (repeats(a->k_out, a->batch, a->budget, a->kv_heads) || repeats(a->v_out, a->batch, a->budget, a->kv_heads))
         return SDPA_EINVAL;
     // (a workgroup moves 1024 pieces of at least one element, and one of 1024 threads selects for a head)
@@ -308,6 +313,7 @@ int sdpa_dev_attention_scored(const struct sdpa_heads *a, void *workspace, size_
     if (a->batch == 0) return SDPA_OK;
     if (a->kv_tokens > 0 && (!a->weights || !a->weights_out)) return SDPA_EINVAL;
     if (a->weights_batch < 0 || a->weights_head < 0 || a->weights_out_batch < 0 || a->weights_out_head < 0) return SDPA_EINVAL;
+    if (a->kv_tokens > 0 && repeats_weights(a)) return SDPA_EINVAL;
     sdpa_heads x = *a;
     x.window = kMaxTokens;
     x.sinks = 0;

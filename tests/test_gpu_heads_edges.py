@@ -232,3 +232,43 @@ def test_more_rows_than_a_launch_has_workgroups_for_a_row_each(pkg):
     close(out[-1:], want, to, "out")
     close(lse[-1:], wl, tl, "lse")
     check_gradients(q, k, v, dout, *(x[-1:] for x in grads), None, None, 40, 2, "bf16")
+
+
+@pytest.mark.parametrize("B,Tq,Tk", [(0, 3, 5), (2, 0, 5), (2, 3, 0), (2, 90, 0), (2, 0, 0)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_nothing_to_do(dtype, B, Tq, Tk, pkg):
+    """no sequences, no queries, no keys: zeros, log sums of -inf, weights and caches as they were"""
+    q, k, v = make((B, Tq, 4, 64), dtype, 1), make((B, Tk, 2, 64), dtype, 2), make((B, Tk, 2, 64), dtype, 3)
+    kp, vp = make((1, 6, 2, 64), dtype, 4)[0], make((1, 6, 2, 64), dtype, 5)[0]
+    w = torch.rand((B, 2, Tk), device="cuda")
+    out, lse = pkg.attention_window(q, k, v, 4, sinks=1)
+    grads = pkg.attention_window_backward(q.clone(), q, k, v, out, lse, 4, sinks=1)
+    o2, l2, w2 = pkg.attention_scored(q, k, v, w, weights_out=torch.empty_like(w))
+    if Tq == 0 or Tk == 0:
+        assert torch.equal(w2, w) and not any(x.any() for x in (out, o2, *grads)) and lse.eq(-float("inf")).all() and l2.eq(-float("inf")).all()
+    assert [tuple(x.shape) for x in grads] == [tuple(x.shape) for x in (q, k, v)]
+    assert pkg.attention_prefix(q, kp, vp, k, v)[0].shape == q.shape
+    nk, nv, nw, nl, kept = pkg.evict_cache(k, v, w, None, 3, sinks=1)
+    assert nk.shape == (B, 3, 2, 64) and nl.eq(min(Tk, 3)).all() and (Tk or kept.eq(-1).all())
+
+
+@pytest.mark.parametrize("Tq", [1, 100])
+def test_sinks_beyond_the_cache_are_plain_causal_attention(Tq, pkg):
+    q, k, v = make((2, Tq, 4, 64), "bf16", 1), make((2, 150, 2, 64), "bf16", 2), make((2, 150, 2, 64), "bf16", 3)
+    run_both(pkg, q, k, v, 0, 1 << 40, None, [150, 60], None, "bf16")
+    run_both(pkg, q, k, v, 1, 151, None, [150, 60], None, "bf16")
+
+
+def test_a_long_selection_in_a_graph(pkg):
+    k, v = make((2, 20001, 1, 8), "bf16", 1), make((2, 20001, 1, 8), "bf16", 2)
+    w = torch.zeros((2, 1, 20001), device="cuda")
+    pkg.evict_cache(k, v, w, None, 900)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = pkg.evict_cache(k, v, w, None, 900, sinks=3, recent=20)
+    for turn in range(3):
+        w.copy_(torch.rand(w.shape, generator=torch.Generator().manual_seed(turn)))
+        g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, pkg.evict_cache(k, v, w, None, 900, sinks=3, recent=20)):
+            assert torch.equal(x, y)

@@ -150,7 +150,7 @@ def test_c_entries_refuse(op, kw, code, pkg):
     (0, dict(q_heads=3), -1), (0, dict(window=-1), -1), (0, dict(lse=0), -1), (0, dict(out=(4096, 0, 24, 6)), -1), (0, dict(scale=float("nan")), -1),
     (0, dict(scale=float("inf")), -1), (3, dict(scale=float("-inf")), -1), (2, dict(prefix=4, kp=(4096, 0, 8, 8), vp=(4096, 0, 8, 6), q_tokens=1 << 22), -6),
     (0, dict(q_tokens=1 << 24), -6), (1, dict(batch=1 << 20, kv_tokens=64, sinks=4, q_tokens=200), -6), (1, dict(dq=(0, 96, 32, 8)), -1), (1, dict(dv_out=(4096, 60, 0, 6)), -1), (1, dict(dout=(0, 1, 1, 1)), -1), (2, dict(prefix=4), -1),
-    (2, dict(prefix=-1), -1), (3, dict(weights=0), -1), (3, dict(ws=(10, 5, -1, 5)), -1), (4, dict(budget=1), -1), (4, dict(kept=0), -1),
+    (2, dict(prefix=-1), -1), (3, dict(weights=0), -1), (3, dict(ws=(10, 5, -1, 5)), -1), (3, dict(ws=(10, 5, 0, 5)), -1), (4, dict(ws=(10, 5, 10, 0)), -1), (4, dict(budget=1), -1), (4, dict(kept=0), -1),
     (4, dict(lens_out=0), -1), (4, dict(k_out=(4096, 64, 0, 8)), -1), (0, dict(batch=1 << 20, q_tokens=1 << 20), -6)], ids=str)
 def test_c_entries_refuse_their_own(op, kw, code, pkg):
     assert getattr(pkg.load(), ENTRIES[op])(pack(**kw), 4096, 1 << 20, None) == code
