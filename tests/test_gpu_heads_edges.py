@@ -272,3 +272,27 @@ def test_a_long_selection_in_a_graph(pkg):
         torch.cuda.synchronize()
         for x, y in zip(got, pkg.evict_cache(k, v, w, None, 900, sinks=3, recent=20)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 100, 128, 256])
+@pytest.mark.parametrize("Tk,window", [(200, 60), (6000, 5000)])
+def test_a_token_does_not_see_what_holds_no_numbers(Tk, window, D, dtype, pkg):
+    """single tokens, one of whose tiles is masked and holds NaN or Inf in rows they do not see (the form of one workgroup, and the split one)"""
+    q, k, v = make((2, 3, 4, D), dtype, 1), make((2, Tk, 2, D), dtype, 2), make((2, Tk, 2, D), dtype, 3)
+    n = [Tk - 3, Tk - 40]
+    kw = dict(sinks=2, kv_lens=lens(n))
+    want = pkg.attention_window(q, k, v, window, **kw)
+    ws = pkg.attention_scored(q, k, v, torch.zeros((2, 2, Tk), device="cuda"), kv_lens=lens(n))
+    for value in (float("nan"), float("inf"), -float("inf")):
+        K, V = k.clone(), v.clone()
+        for b in range(2):
+            for x in (K, V):
+                x[b, n[b]:] = value
+        got = pkg.attention_scored(q, K, V, torch.zeros((2, 2, Tk), device="cuda"), kv_lens=lens(n))
+        assert all(torch.equal(x, y) for x, y in zip(got, ws))
+        for b in range(2):                                # right before the window, behind the sinks
+            for x in (K, V):
+                x[b, 2:n[b] - 2 - window] = value
+        got = pkg.attention_window(q, K, V, window, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
