@@ -86,7 +86,9 @@ template <int NB> __device__ inline void hide(f32x16 *s, int j0, Seen seen, int 
 
 // The reference exponent follows the maximum only when that rose by more than 2^8: a weight is then at most 2^8 instead of 1,
 // which costs no precision (fp32 sums, and operand roundings are relative), and the 16 * DP / 32 multiplications of a rescale are
-// rare.  Scores are compared unscaled (the scale is positive: load_query) and scaled inside the exponential's argument.
+// rare.  The branch is the wave's, the decision each column's own: a row's bits must not depend on the rows beside it (a column
+// without a row among them).  Scores are compared unscaled (the scale is positive: load_query) and scaled inside the exponential's
+// argument.
 // -> the exponent the tile's weights refer to
 template <int NB> __device__ inline float largest(const f32x16 *s) {
     float mx = s[0][0];
@@ -98,10 +100,10 @@ template <int NB> __device__ inline float largest(const f32x16 *s) {
 }
 template <int DP> __device__ inline float raise(State<DP> &st, float mx, float scale) {
     const float top = half_max(mx) * scale;
-    if (__any(top > st.m + 8.f)) {
-        const float m = fmaxf(st.m, top);
-        const float alpha = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
-        st.m = m;
+    const bool rises = top > st.m + 8.f;
+    if (__any(rises)) {
+        const float alpha = rises ? __builtin_amdgcn_exp2f(st.m - top) : 1.f;
+        st.m = rises ? top : st.m;
         st.l *= alpha;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)

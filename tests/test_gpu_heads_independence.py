@@ -1,0 +1,70 @@
+"""GPU: a row of the batched attention operators is a function of its own query and of the keys it sees -- bit for bit, whatever its neighbours
+in the call hold."""
+import pytest
+import torch
+
+from test_gpu_heads import lens, make
+
+pytestmark = pytest.mark.gpu
+DTYPES = ["bf16", "f32"]
+
+
+def rising(k, top=3.0):
+    """keys that grow along the cache: a row's softmax maximum rises a little in tile after tile"""
+    T = k.shape[-3]
+    return k * torch.linspace(0.3, top, T, device=k.device).view(-1, 1, 1).to(k.dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,Tq,Tk", [(2, 3, 200), (2, 5, 5000), (200, 3, 1000), (2, 300, 300), (2, 700, 900), (40, 100, 600)])
+def test_a_large_key_that_a_row_does_not_see(B, Tq, Tk, dtype, pkg):
+    """finite keys of a later token, large enough to move the softmax maximum of the rows that do see them"""
+    q, k, v = make((B, Tq, 4, 64), dtype, 1), rising(make((B, Tk, 2, 64), dtype, 2)), make((B, Tk, 2, 64), dtype, 3)
+    want, wl = pkg.attention_window(q, k, v, Tk)
+    ws = pkg.attention_scored(q, k, v, torch.zeros((B, 2, Tk), device="cuda"))
+    for hit in sorted({1, Tq // 3, Tq // 2, Tq - 1} - {0}):      # the first row that sees the changed key
+        for factor in (8.0, 50.0):
+            K = k.clone()
+            K[:, Tk - Tq + hit] = k[:, Tk - Tq + hit] * factor
+            out, lse = pkg.attention_window(q, K, v, Tk)
+            assert torch.equal(out[:, :hit], want[:, :hit]) and torch.equal(lse[..., :hit], wl[..., :hit]), (hit, factor)
+            assert not torch.equal(out[:, hit:], want[:, hit:])
+            so, sl, _ = pkg.attention_scored(q, K, v, torch.zeros((B, 2, Tk), device="cuda"))
+            assert torch.equal(so[:, :hit], ws[0][:, :hit]) and torch.equal(sl[..., :hit], ws[1][..., :hit]), (hit, factor)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,Tq,P", [(3, 1, 700), (3, 1, 9000), (20, 2, 700), (20, 2, 9000)])
+def test_another_sequence_behind_the_same_prefix(B, Tq, P, dtype, pkg):
+    """the queries of a batch share the prefix's tiles, and nothing else"""
+    Tk = 40
+    q, k, v = make((B, Tq, 4, 64), dtype, 1), make((B, Tk, 2, 64), dtype, 2), make((B, Tk, 2, 64), dtype, 3)
+    kp, vp = rising(make((1, P, 2, 64), dtype, 4)[0]), make((1, P, 2, 64), dtype, 5)[0]
+    want, wl = pkg.attention_prefix(q, kp, vp, k, v)
+    for factor in (3.0, 10.0, 40.0):
+        Q = q.clone()
+        Q[1] = q[1] * factor
+        out, lse = pkg.attention_prefix(Q, kp, vp, k, v)
+        for b in [b for b in range(B) if b != 1]:
+            assert torch.equal(out[b], want[b]) and torch.equal(lse[b], wl[b]), (b, factor)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tq,nq", [(4, 2), (6, 5), (100, 40), (260, 131)])
+def test_padded_rows_beside_values_that_are_no_numbers(Tq, nq, dtype, pkg):
+    """a ragged call whose last live rows share a wave with rows that do not exist: a hidden cache row without numbers changes nothing"""
+    Tk, nk, window, sinks = 1500, 1401, 1100, 3
+    q, k, v = make((1, Tq, 4, 64), dtype, 1), make((1, Tk, 2, 64), dtype, 2), make((1, Tk, 2, 64), dtype, 3)
+    q, k = q.abs(), -rising(k.abs().flip(1), 4.0).flip(1)        # scores below those of an empty query, and rising
+    B = 130                                               # (so many that a workgroup walks many tiles)
+    q, k, v = (x.expand(B, -1, -1, -1) for x in (q, k, v))
+    kw = dict(sinks=sinks, q_lens=lens([nq] * B), kv_lens=lens([nk] * B))
+    want = pkg.attention_window(q, k, v, window, **kw)
+    V = v.clone()
+    V[:, nk:] = V[:, sinks:nk - nq - window + 2] = float("nan")       # (the last of them is the first row's first key)
+    got = pkg.attention_window(q, k, V, window, **kw)
+    assert got[0][:, 0].isnan().all() and torch.equal(got[0][:, 1:], want[0][:, 1:]) and torch.equal(got[1], want[1])
+    Q = q.clone()
+    Q[:, nq:] = 1e4                                       # what rows behind the length hold
+    got = pkg.attention_window(Q, k, v, window, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
