@@ -642,6 +642,7 @@ __device__ inline void add_weights(const WeightArgs &w, int block) {
     const int blocks = (w.Tk + 1023) / 1024, part = block % blocks, bh = block / blocks, h = bh % w.Hkv, b = bh / w.Hkv, G = w.Hq / w.Hkv;
     const int nq = clamp_len(w.q_lens, b, w.Tq), nk = clamp_len(w.kv_lens, b, w.Tk), rows = nq * G, all = w.Tq * G;
     __shared__ float lse2[kFewRows];
+    __shared__ int last[kFewRows];                       // the last key a row sees
     if ((int)threadIdx.x < rows) {
         const int t = threadIdx.x / G, hq = h * G + threadIdx.x - t * G;
         float x;
@@ -657,6 +658,7 @@ __device__ inline void add_weights(const WeightArgs &w, int block) {
             }
             x = l == 0.f ? kNegInf : m + __log2f(l);
         } else x = w.lse[((long)b * w.Hq + hq) * w.Tq + t] * kLog2e;
+        last[threadIdx.x] = nk - nq + t;
         lse2[threadIdx.x] = x == kNegInf ? __builtin_inff() : x;         // (a row that sees nothing gives nothing)
     }
     __syncthreads();
@@ -669,7 +671,8 @@ __device__ inline void add_weights(const WeightArgs &w, int block) {
         for (int r = 0; r < rows; ++r) {
             const f32x4 s = *reinterpret_cast<const f32x4 *>(src + (long)r * w.score_ld);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(s[i] * w.scale_log2 - lse2[r]);
+            for (int i = 0; i < 4; ++i)                  // (by the key's place: a row whose lse is no number gives nothing to what it does not see)
+                sum[i] += j + i <= last[r] ? __builtin_amdgcn_exp2f(s[i] * w.scale_log2 - lse2[r]) : 0.f;
         }
     }
     const float *in = w.w_in + b * w.wi_batch + h * w.wi_head + j;

@@ -68,3 +68,20 @@ def test_padded_rows_beside_values_that_are_no_numbers(Tq, nq, dtype, pkg):
     Q[:, nq:] = 1e4                                       # what rows behind the length hold
     got = pkg.attention_window(Q, k, v, window, **kw)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tk", [60, 700, 6000])
+@pytest.mark.parametrize("Tq", [5, 40])
+def test_a_row_without_numbers_gives_its_weights_only_to_keys_it_sees(Tq, Tk, dtype, pkg):
+    """attention_scored: the weights of the keys behind a row whose query holds NaN are those of the other rows"""
+    q, k, v = make((2, Tq, 4, 64), dtype, 1), make((2, Tk, 2, 64), dtype, 2), make((2, Tk, 2, 64), dtype, 3)
+    w = torch.rand((2, 2, Tk), generator=torch.Generator().manual_seed(4)).cuda()
+    _, _, want = pkg.attention_scored(q, k, v, w, weights_out=torch.empty_like(w))
+    Q = q.clone()
+    Q[1, 1, 2] = float("nan")                             # one head of the second token, of the second key head's group
+    out, lse, got = pkg.attention_scored(Q, k, v, w, weights_out=torch.empty_like(w))
+    first = Tk - Tq + 2                                   # keys from here on are not seen by it
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1, 0], want[1, 0])
+    assert torch.equal(got[1, 1, first:], want[1, 1, first:]) and got[1, 1, :first].isnan().all()
+    assert out[1, 1, 2].isnan().all() and lse[1, 2, 1].isnan() and out.isnan().sum() == out.shape[-1]
