@@ -709,7 +709,7 @@ __global__ __launch_bounds__(kHeadsThreads) void weights_kernel(WeightArgs a, in
     const int nq = clamp_len(a.q_lens, b, a.Tq), nk = clamp_len(a.kv_lens, b, a.Tk);
     const SeenBy tok = seen_by(j, nq, nk, 1 << 30, 0), by = {tok.lo * G, tok.hi * G};
     float sum = 0.f;
-    if (k0 < nk) {
+    if (k0 < nk && nq > 0) {                             // (a call without queries may come without keys: nothing is read)
         typename Ops<T>::Frag kf[STEPS];
         load_row<T, DP>(kf, row_at(a.k, b, j, h, sizeof(T)), a.Dk, j < nk, a.vec, lane);
         const int r_end = nq * G, first = max(0, k0 - (nk - nq)) * G / 32 + wave / KW;
