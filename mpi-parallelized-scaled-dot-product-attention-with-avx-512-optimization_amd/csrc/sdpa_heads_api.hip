@@ -162,7 +162,7 @@ int run_own(const sdpa_heads *a, const Slots &s, void *workspace, hipStream_t st
     return SDPA_OK;
 }
 
-struct BackwardPlan { int chunks, sink_blocks, tail_chunks; long stat_rows, stats, bytes; double grid; };     // grid: the largest launch
+struct BackwardPlan { int chunks, sink_blocks, tail_chunks; long stat_rows, stats, bytes; double grid; };
 
 // A key block's workgroup walks the rows that see it by the window, about (64 + window) tokens' heads; several share them while the launch
 // has fewer workgroups than the chip has CUs.  A block with sink keys is seen by every row behind: its tail goes to short workgroups
@@ -179,10 +179,16 @@ BackwardPlan plan_backward(const sdpa_heads *a) {
     p.sink_blocks = (int)ceil_div(sinks, kBwdKeys);
     const long piece = walk / (4 * p.chunks) > 128 ? walk / (4 * p.chunks) : 128;
     const long tails = ceil_div(tail, piece);
-    p.tail_chunks = p.sink_blocks == 0 ? 0 : (int)(tails < kMaxSplits ? tails : kMaxSplits);
-    const long joined = p.chunks > 1 ? blocks : p.tail_chunks > 0 ? p.sink_blocks : 0;
+    // Each of them has a slot in the scratch, so there are as many as fill the chip twice, or an eighth of the key blocks (a quarter of the
+    // bytes of bf16 gradients), and where that leaves less than two to a block there is no need for them: so many long walks fill the chip
+    // by themselves.
+    const long busy = groups * blocks / 8 > 512 ? groups * blocks / 8 : 512, most = groups * p.sink_blocks < 1 ? 0 : busy / (groups * p.sink_blocks);
+    p.tail_chunks = most < 2 ? 0 : (int)(tails < most ? tails < kMaxSplits ? tails : kMaxSplits : most < kMaxSplits ? most : kMaxSplits);
+    // the largest launch, the join's 16 workgroups of a block among them (counted for every sink block with a tail, so that what is refused goes
+    // by the sizes alone and not by the plan)
+    const long joined = p.chunks > 1 ? blocks : tail > 0 ? p.sink_blocks : 0;
     p.grid = (double)groups * (blocks * p.chunks + p.sink_blocks * p.tail_chunks);
-    if ((double)groups * joined * (kBwdKeys / 4) > p.grid) p.grid = (double)groups * joined * (kBwdKeys / 4);     // (the join's)
+    if ((double)groups * joined * (kBwdKeys / 4) > p.grid) p.grid = (double)groups * joined * (kBwdKeys / 4);
     const long slots = p.chunks > 1 ? blocks * p.chunks + p.sink_blocks * p.tail_chunks :
                        p.tail_chunks > 0 ? p.sink_blocks * (1 + p.tail_chunks) : 0;
     // rows of a head: blocks of 32, whole tokens to a block (or, of larger groups, blocks to a token), in pairs

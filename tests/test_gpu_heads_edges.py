@@ -296,3 +296,17 @@ def test_a_token_does_not_see_what_holds_no_numbers(Tk, window, D, dtype, pkg):
                 x[b, 2:n[b] - 2 - window] = value
         got = pkg.attention_window(q, K, V, window, **kw)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("c", [
+    # dtype, B, T, Hq, Hkv, D, window, sinks: several blocks of sinks, and so many groups that their tails have few or no workgroups of their own
+    ("bf16", 20, 450, 8, 4, 64, 40, 300),
+    ("f32", 17, 500, 4, 4, 64, 70, 200),
+    ("bf16", 3, 900, 2, 2, 64, 30, 700),
+    ("bf16", 70, 330, 8, 8, 64, 9, 4),
+], ids=str)
+def test_many_sinks_of_many_sequences(c, pkg):
+    dtype, B, T, Hq, Hkv, D, window, sinks = c
+    q, k, v = make((B, T, Hq, D), dtype, 1, 1.5), make((B, T, Hkv, D), dtype, 2), make((B, T, Hkv, D), dtype, 3)
+    n = [T - (37 * b) % (T // 2) for b in range(B)]
+    run_both(pkg, q, k, v, window, sinks, n, n, None, dtype)

@@ -184,3 +184,16 @@ def test_the_reference_gradient_is_the_derivative():
         up, down = [q, k, v], [q, k, v]
         up[i], down[i] = x + h * d, x - h * d
         assert abs((loss(*up) - loss(*down)) / (2 * h) - (grads[i] * d).sum()) < 1e-7
+
+
+@pytest.mark.parametrize("batch,tokens,window,sinks,heads,dk", [
+    (1, 8192, 0, 8192, (32, 8), 128), (4, 32768, 0, 1 << 30, (32, 8), 128), (2, 8192, 128, 1024, (32, 8), 128), (64, 4096, 128, 4, (32, 8), 128),
+    (2, 4096, 1024, 4, (16, 4), 128), (1, 500, 20, 500, (4, 1), 64), (1, 1 << 20, 512, 100, (8, 8), 256), (512, 300, 10, 70, (2, 2), 64)])
+def test_the_backward_scratch_is_bounded_by_the_chip_and_the_gradients(batch, tokens, window, sinks, heads, dk, pkg):
+    """two row statistics for every row, and slots of 64 keys: at most 1024 of them and 3/16 of the key blocks, however many keys are sinks"""
+    hq, hkv = heads
+    args = pack(batch=batch, q_tokens=tokens, kv_tokens=tokens, q_heads=hq, kv_heads=hkv, dk=dk, dv=dk, window=window, sinks=sinks, dtype=1)
+    need = pkg.load().sdpa_dev_heads_workspace(1, args)
+    stats = 2 * 4 * batch * hkv * (tokens * (hq // hkv) + 64)
+    blocks = batch * hkv * ((tokens + 63) // 64)
+    assert 0 < need <= stats + (1024 + 3 * blocks / 16) * 64 * 2 * dk * 4 + 16
