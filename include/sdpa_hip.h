@@ -509,8 +509,13 @@ struct sdpa_heads {
     float scale;                  /* scores are scale * q.k; any finite number                      */
 };
 
-/* Sizes: at most 2^30 tokens, 2^24 - 1 query rows of a key head and (kv_tokens / 128 + 1) * batch * kv_heads below 2^24 (beside a prefix:
- * query rows of all heads below 2^24); beyond them a call returns SDPA_EUNSUP.                                                      */
+/* Sizes, with groups = batch * kv_heads; a call beyond them returns SDPA_EUNSUP, and so does the question of its scratch:
+ *   all calls   at most 2^30 tokens
+ *   attention   query rows of a key head (q_tokens * q_heads / kv_heads), groups * (kv_tokens / 128 + 1) and groups * (those rows / 128 + 1)
+ *               below 2^24 each; beside a prefix groups * rows too
+ *   backward    besides, blocks of 64 keys of all groups (with sinks an eighth more) below 2^24; those with sinks below 2^20 where
+ *               q_tokens > window + 64
+ *   eviction    groups * (budget * (dk + dv) / 1024 + 2) below 2^24 and groups below 2^22                                        */
 
 /* Scratch a call needs (0 = none; negative: the SDPA_E* code the call would return).  The scratch belongs to one call at a time:
  * calls on different streams, and captured graphs that may replay side by side, take one each.  `op` names the call.              */

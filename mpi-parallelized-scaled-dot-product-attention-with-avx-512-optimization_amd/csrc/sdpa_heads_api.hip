@@ -199,6 +199,12 @@ BackwardPlan plan_backward(const sdpa_heads *a) {
     return p;
 }
 
+// the plan of a call, or why there is none (for the call and for the question of its scratch)
+int plan_backward(const sdpa_heads *a, BackwardPlan &p) {
+    p = plan_backward(a);
+    return p.grid > kMaxGroups ? SDPA_EUNSUP : SDPA_OK;
+}
+
 int check_evict(const sdpa_heads *a) {
     SDPA_TRY(check_shape(a));
     if (a->budget < 0 || a->sinks < 0 || a->recent < 0 || (long)a->sinks + a->recent > a->budget) return SDPA_EINVAL;
@@ -223,21 +229,22 @@ int check_evict(const sdpa_heads *a) {
 extern "C" {
 
 long sdpa_dev_heads_workspace(int op, const struct sdpa_heads *a) {
+    if (op < SDPA_OP_WINDOW || op > SDPA_OP_EVICT) return SDPA_EINVAL;
     if (op == SDPA_OP_EVICT) {
         const int c = check_evict(a);
         return c != SDPA_OK ? c : 0;
     }
-    const int c = check_attention(a);
+    int c = check_attention(a);
     if (c != SDPA_OK) return c;
-    if (op == SDPA_OP_WINDOW_BACKWARD) return plan_backward(a).bytes;
+    if (op == SDPA_OP_WINDOW_BACKWARD) {
+        BackwardPlan p;
+        c = plan_backward(a, p);
+        return c != SDPA_OK ? c : p.bytes;
+    }
     if (empty(a)) return 0;
     sdpa_heads x = *a;
     if (op == SDPA_OP_PREFIX || op == SDPA_OP_SCORED) { x.window = kMaxTokens; x.sinks = 0; }
-    switch (op) {
-        case SDPA_OP_WINDOW: case SDPA_OP_SCORED: return plan_window(&x, op == SDPA_OP_SCORED).bytes;
-        case SDPA_OP_PREFIX: return plan_prefix(&x).bytes;
-        default: return SDPA_EINVAL;
-    }
+    return op == SDPA_OP_PREFIX ? plan_prefix(&x).bytes : plan_window(&x, op == SDPA_OP_SCORED).bytes;
 }
 
 int sdpa_dev_attention_window(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream) {
@@ -259,8 +266,8 @@ int sdpa_dev_attention_window_backward(const struct sdpa_heads *a, void *workspa
     if (repeats(a->dq, a->batch, a->q_tokens, a->q_heads) || repeats(a->dk_out, a->batch, a->kv_tokens, a->kv_heads) ||
         repeats(a->dv_out, a->batch, a->kv_tokens, a->kv_heads))
         return SDPA_EINVAL;
-    const BackwardPlan p = plan_backward(a);
-    if (p.grid > kMaxGroups) return SDPA_EUNSUP;
+    BackwardPlan p;
+    SDPA_TRY(plan_backward(a, p));
     SDPA_TRY(check_scratch(p.bytes, workspace, workspace_bytes));
     SDPA_TRY(require_device());
     BackwardArgs x = {};

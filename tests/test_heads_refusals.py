@@ -197,3 +197,12 @@ def test_the_backward_scratch_is_bounded_by_the_chip_and_the_gradients(batch, to
     stats = 2 * 4 * batch * hkv * (tokens * (hq // hkv) + 64)
     blocks = batch * hkv * ((tokens + 63) // 64)
     assert 0 < need <= stats + (1024 + 3 * blocks / 16) * 64 * 2 * dk * 4 + 16
+
+
+def test_the_question_of_the_scratch_is_refused_as_the_call_is(pkg):
+    """sizes beyond a launch are refused before anybody allocates the scratch for them; so is a call that there is none of"""
+    lib = pkg.load()
+    for kw in (dict(batch=1 << 20, kv_tokens=64, sinks=4, q_tokens=200), dict(batch=1 << 21, kv_tokens=256, sinks=0, q_tokens=1)):
+        assert lib.sdpa_dev_heads_workspace(1, pack(**kw)) == lib.sdpa_dev_attention_window_backward(pack(**kw), 4096, 1 << 20, None) == -6
+    for op in (-1, 5, 9):
+        assert lib.sdpa_dev_heads_workspace(op, pack(batch=0)) == -1
