@@ -14,13 +14,15 @@ that see no key (and rows behind q_lens) get out 0, lse -inf and gradient 0; key
 
 All work is enqueued on torch's current stream of the tensors' device; scratch comes from torch's allocator, a piece of its own for
 every call.  Nothing waits for the device, so every call can be captured into a graph.  The operators are not
-recorded by autograd: a tensor that requires a gradient is refused while gradients are enabled (use `detach()` and
-`attention_window_backward`).
+recorded by autograd: a tensor that requires a gradient is refused while gradients are enabled, read or written (use `detach()` and
+`attention_window_backward`), and so is one that carries a forward-mode tangent.  Tensors of the caller's that are written count as
+modified in place: a graph that saved one notices.
 """
 import math
 import struct
 
 import torch
+from torch.autograd import forward_ad, graph
 
 from . import _lib
 from ._lib import SdpaError, check
@@ -114,17 +116,33 @@ def _count(x, name):
     return x if x < _INT_MAX else _INT_MAX
 
 
+def _recorded(x):
+    """would autograd record what is done with x?  (the level: no forward-mode derivative is being taken anywhere)"""
+    return (x.requires_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None)
+
+
+def _unrecorded(x, name, call):
+    if x is not None and _recorded(x):
+        raise ValueError("%s requires a gradient: %s is not recorded by autograd, pass %s.detach()" % (name, call, name))
+
+
+def _written(*given):
+    """the caller's own tensors that a call wrote"""
+    given = [x for x in given if x is not None]
+    if given:
+        graph.increment_version(given)
+
+
 def _fits(x, shape, like):
-    """an operand as it should be: shape, type, device, contiguous rows, no gradient to record"""
+    """an operand as it should be: shape, type, device, contiguous rows"""
     return (type(x) is torch.Tensor and x.shape == shape and x.dtype is like.dtype and x.device == like.device and
-            (x.stride(-1) == 1 or shape[-1] == 1) and not (x.requires_grad and torch.is_grad_enabled()))
+            (x.stride(-1) == 1 or shape[-1] == 1))
 
 
 def _operand(x, name, shape, like, call):
     if not _fits(x, shape, like):
         _rows(x, name, shape, like.dtype, like.device)
-        _need(not (x.requires_grad and torch.is_grad_enabled()),
-              "%s requires a gradient: %s is not recorded by autograd, pass %s.detach()" % (name, call, name))
+    _unrecorded(x, name, call)
 
 
 def _qkv(q, k, v, name):
@@ -159,9 +177,11 @@ def _outputs(q, Dv, out, lse, ins, name):
     B, Tq, Hq = q.shape[:3]
     if out is not None:
         _rows(out, "out", (B, Tq, Hq, Dv), q.dtype, q.device)
+        _unrecorded(out, "out", name)
         _apart([out], ins, name)
     if lse is not None:
         _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
+        _unrecorded(lse, "lse", name)
         _need(lse.is_contiguous(), "lse: must be contiguous")
         _apart([lse], ins, name)
         _distinct((out, lse), name)
@@ -181,10 +201,12 @@ def attention_window(q, k, v, window, sinks=0, q_lens=None, kv_lens=None, scale=
     window, sinks = _count(window, "window"), _count(sinks, "sinks")
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
+    given = out, lse
     out, lse = _outputs(q, Dv, out, lse, (q, k, v), name)
     args = _PACK_WINDOW.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk,
                              Hq, Hkv, Dk, Dv, window, sinks, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_window, name, _OP_WINDOW, q, args)
+    _written(*given)
     return out, lse
 
 
@@ -201,19 +223,23 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
     _operand(out, "out", (B, Tq, Hq, Dv), q, name)
     _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
     _need(lse.is_contiguous(), "lse: must be contiguous")
+    _unrecorded(lse, "lse", name)
     ins = (dout, q, k, v, out, lse)
     for x, n, like in ((dq, "dq", q), (dk, "dk", k), (dv, "dv", v)):
         if x is not None:
             _rows(x, n, like.shape, q.dtype, q.device)
+            _unrecorded(x, n, name)
             _apart([x], ins, name)
             _distinct((dq, dk, dv), name)
     _on_gpu(q, name)
+    given = dq, dk, dv
     dq = q.new_empty(q.shape) if dq is None else dq
     dk = q.new_empty(k.shape) if dk is None else dk
     dv = q.new_empty(v.shape) if dv is None else dv
     args = _PACK_BACKWARD.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), *_at(dout), *_at(dq), *_at(dk), *_at(dv), lse.data_ptr(), _ptr(q_lens),
                                _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, window, sinks, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_window_backward, name, _OP_WINDOW_BACKWARD, q, args)
+    _written(*given)
     return dq, dk, dv
 
 
@@ -230,19 +256,22 @@ def attention_prefix(q, k_prefix, v_prefix, k, v, q_lens=None, kv_lens=None, sca
     _operand(v_prefix, "v_prefix", (P, Hkv, Dv), q, name)
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
+    given = out, lse
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, k_prefix, v_prefix), name)
     args = _PACK_PREFIX.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), k_prefix.data_ptr(), 0, *k_prefix.stride()[:2], v_prefix.data_ptr(), 0,
                              *v_prefix.stride()[:2], lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv,
                              P, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_prefix, name, _OP_PREFIX, q, args)
+    _written(*given)
     return out, lse
 
 
-def _weights(x, name, shape, like, written=False):
+def _weights(x, name, shape, like, call, written=False):
     """[batch, heads, tokens] float32; one that is written must not repeat elements"""
     if not (type(x) is torch.Tensor and x.shape == shape and x.dtype is torch.float32 and x.device == like.device and x.is_contiguous()):
         _rows(x, name, shape, torch.float32, like.device)
         _need(not written or all(n == 1 or s > 0 for n, s in zip(x.shape, x.stride())), "%s: repeats elements" % name)
+    _unrecorded(x, name, call)
 
 
 def _sums(weights, weights_out):
@@ -255,18 +284,20 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
     -> (out, lse, the increased weights).  evict_cache() goes by these sums."""
     name = "attention_scored"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
-    _weights(weights, "weights", (B, Hkv, Tk), q, weights_out is None)
+    _weights(weights, "weights", (B, Hkv, Tk), q, name, weights_out is None)
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
     if weights_out is None:
         weights_out = weights
     elif weights_out is not weights:
-        _weights(weights_out, "weights_out", (B, Hkv, Tk), q, True)
+        _weights(weights_out, "weights_out", (B, Hkv, Tk), q, name, True)
         _apart([weights_out], (q, k, v, weights), name)
+    given = out, lse, weights_out
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights, weights_out), name)
     args = _PACK_SCORED.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), *_sums(weights, weights_out),
                              _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, _scale(scale, Dk))
     _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q, args)
+    _written(*given)
     return out, lse, weights_out
 
 
@@ -286,7 +317,7 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
     _need(1 <= Dk <= HEAD_DIM_MAX and 1 <= Dv <= HEAD_DIM_MAX and H > 0, "head dims must be 1 to %d" % HEAD_DIM_MAX)
     _operand(k, "k", (B, T, H, Dk), k, name)
     _operand(v, "v", (B, T, H, Dv), k, name)
-    _weights(weights, "weights", (B, H, T), k)
+    _weights(weights, "weights", (B, H, T), k, name)
     _lens(lens, "lens", B, k)
     budget, sinks, recent = _count(budget, "budget"), _count(sinks, "sinks"), _count(recent, "recent")
     _need(sinks + recent <= budget, "sinks + recent must not exceed the budget")
@@ -295,17 +326,19 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
         if x is not None:
             _need(isinstance(x, torch.Tensor) and x.dim() == 4 and x.shape[1] >= budget, "%s: needs %d tokens" % (n, budget))
             _rows(x, n, (B, x.shape[1], H, dim), k.dtype, k.device)
+            _unrecorded(x, n, name)
             _apart([x], ins, name)
     if weights_out is not None:
         _need(isinstance(weights_out, torch.Tensor) and weights_out.dim() == 3 and weights_out.shape[2] >= budget,
               "weights_out: needs %d tokens" % budget)
-        _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k, True)
+        _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k, name, True)
         _apart([weights_out], ins, name)
     if k_out is not None:
         _distinct((k_out, v_out, weights_out), name)
     elif v_out is not None:
         _distinct((v_out, weights_out), name)
     _on_gpu(k, name)
+    given = k_out, v_out, weights_out
     k_out = k.new_empty((B, budget, H, Dk)) if k_out is None else k_out
     v_out = k.new_empty((B, budget, H, Dv)) if v_out is None else v_out
     weights_out = k.new_empty((B, H, budget), dtype=torch.float32) if weights_out is None else weights_out
@@ -314,4 +347,5 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
     args = _PACK_EVICT.pack(_SIZE, *_at(k), *_at(v), _ptr(lens), *_sums(weights, weights_out), *_at(k_out), *_at(v_out), lens_out.data_ptr(),
                             kept.data_ptr(), _DTYPES[k.dtype], B, 0, T, H, H, Dk, Dv, sinks, budget, recent, 1.0)
     _call(_lib.load().sdpa_dev_evict_cache, name, _OP_EVICT, k, args)
+    _written(*given)
     return k_out, v_out, weights_out, lens_out, kept

@@ -206,3 +206,41 @@ def test_the_question_of_the_scratch_is_refused_as_the_call_is(pkg):
         assert lib.sdpa_dev_heads_workspace(1, pack(**kw)) == lib.sdpa_dev_attention_window_backward(pack(**kw), 4096, 1 << 20, None) == -6
     for op in (-1, 5, 9):
         assert lib.sdpa_dev_heads_workspace(op, pack(batch=0)) == -1
+
+
+def calls(pkg):
+    """every tensor of every operator, read or written: (call, name, shape)"""
+    q, k, v = qkv()
+    o, lse, w, kp, vp = torch.zeros(2, 3, 4, 6), torch.zeros(2, 4, 3), torch.zeros(2, 2, 5), torch.zeros(7, 2, 8), torch.zeros(7, 2, 6)
+    out = dict(out=torch.zeros(2, 3, 4, 6), lse=torch.zeros(2, 4, 3))
+    sets = [
+        (pkg.attention_window, dict(q=q, k=k, v=v, **out), dict(window=4)),
+        (pkg.attention_window_backward, dict(dout=o, q=q, k=k, v=v, out=o.clone(), lse=lse, dq=q.clone(), dk=k.clone(), dv=v.clone()), dict(window=4)),
+        (pkg.attention_prefix, dict(q=q, k_prefix=kp, v_prefix=vp, k=k, v=v, **out), {}),
+        (pkg.attention_scored, dict(q=q, k=k, v=v, weights=w, weights_out=w.clone(), **out), {}),
+        (pkg.evict_cache, dict(k=k, v=v, weights=w, k_out=k.clone(), v_out=v.clone(), weights_out=w.clone()), dict(lens=None, budget=4)),
+    ]
+    return [(f, tensors, other, name) for f, tensors, other in sets for name in tensors]
+
+
+def test_no_tensor_that_requires_a_gradient_is_read_or_written(pkg):
+    for f, tensors, other, name in calls(pkg):
+        args = dict(tensors, **{name: tensors[name].clone().requires_grad_()})
+        with pytest.raises(ValueError, match="%s requires a gradient" % name):
+            f(**args, **other)
+        with torch.no_grad(), pytest.raises(pkg.SdpaError):      # (allowed here: the call gets as far as the device)
+            f(**args, **other)
+    q, k, v = qkv()
+    with pytest.raises(ValueError, match="weights requires"):     # (written in place)
+        pkg.attention_scored(q, k, v, torch.zeros(2, 2, 5).requires_grad_())
+
+
+def test_no_tensor_with_a_forward_mode_tangent(pkg):
+    with torch.autograd.forward_ad.dual_level():
+        for f, tensors, other, name in calls(pkg):
+            dual = torch.autograd.forward_ad.make_dual(tensors[name], torch.ones_like(tensors[name]))
+            with pytest.raises(ValueError, match="%s requires a gradient" % name):
+                f(**dict(tensors, **{name: dual}), **other)
+        f, tensors, other, _ = calls(pkg)[0]
+        with pytest.raises(pkg.SdpaError):                        # (others are not refused)
+            f(**tensors, **other)
