@@ -478,6 +478,8 @@ SDPA_API int  sdpa_dev_shard_partial_bf16(const void *Qb, int ldq, const void *K
  * LAST tokens of the cache.  Lengths are int32 on the device, clamped there to [0, q_tokens] / [0, kv_tokens]; null = all of them.
  * A row that sees no key: out 0, lse -inf.  Rows i >= q_lens[b] likewise, and their gradients are 0; gradients of keys
  * j >= kv_lens[b] are 0.  A key that a row does not see has no influence on it, whatever its cache row holds (NaN included).
+ * Outputs lie over no input and no other output, and hold no element twice (their parts may lie between each other); the one exception is
+ * weights_out, which may be `weights`.
  * Everything is deterministic: no result depends on the order of atomics.                                                        */
 #define SDPA_F32  0
 #define SDPA_BF16 1
@@ -541,8 +543,7 @@ SDPA_API int sdpa_dev_attention_scored(const struct sdpa_heads *a, void *workspa
 /* Cuts every (sequence, key head) of a cache to `budget` keys.  n = kv_lens[b] <= budget: all stay.  Else the first `sinks`, the
  * last `recent` and the budget - sinks - recent of greatest weight between them stay (ties: the lower index; NaN counts below
  * everything), in their order.  They move to the front of k_out / v_out / weights_out; kept[b,h,:] are their old indices, lens_out[b] =
- * min(n, budget); [lens_out, budget) is filled with zeros (kept: -1), what lies behind `budget` is left as it was.  The outputs
- * must not overlap the inputs.                                                                                                  */
+ * min(n, budget); [lens_out, budget) is filled with zeros (kept: -1), what lies behind `budget` is left as it was.               */
 SDPA_API int sdpa_dev_evict_cache(const struct sdpa_heads *a, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus

@@ -80,25 +80,86 @@ def _rows(x, name, shape, dtype, device=None):
 
 
 def _span(x):
-    if x.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return 0, 0
     a = x.data_ptr()
-    return a, a + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+    if not x.is_contiguous():
+        n = sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1
+    return a, a + n * x.element_size()
 
 
-def _apart(outs, ins, name):
-    """a caller's own output tensor must not lie over an input"""
-    for o in outs:
-        a0, a1 = _span(o)
-        for i in ins:
-            b0, b1 = _span(i)
-            _need(a1 <= b0 or b1 <= a0, "%s: an output overlaps an input" % name)
+def _box(x):
+    """a tensor's bytes: (stride, count) of its dims from the largest stride on, the bytes of an element the last of them"""
+    e = x.element_size()
+    dims = sorted(((s * e, n) for s, n in zip(x.stride(), x.shape) if n > 1 and s > 0), reverse=True)
+    if dims and dims[-1][0] == e:
+        dims[-1] = (1, dims[-1][1] * e)                   # (a contiguous row)
+    else:
+        dims.append((1, e))
+    return dims
 
 
-def _distinct(outs, name):
-    """... nor begin where another output does (parts of one packed tensor may lie between each other)"""
-    at = [x.data_ptr() for x in outs if x is not None and x.numel() > 0]
-    _need(len(set(at)) == len(at), "%s: two outputs are the same memory" % name)
+def _reach(dims):
+    return sum(s * (n - 1) for s, n in dims)
+
+
+def _meet(d, a, b, left):
+    """do two boxes share a byte, the second one `d` bytes behind the first?  Stride by stride, from the largest on: of its steps only those matter
+    that bring what remains of the two within each other's reach, which are one or two where strides nest.  `left`: steps until
+    the answer is "perhaps"."""
+    left[0] -= 1
+    if left[0] < 0:
+        return True
+    ra, rb = _reach(a), _reach(b)
+    if d > ra or -d > rb:
+        return False
+    if not a and not b:
+        return True
+    s = max(a[0][0] if a else 0, b[0][0] if b else 0)
+    lo = hi = 0                                           # steps of the first box less those of the second
+    if a and a[0][0] == s:
+        hi = a[0][1] - 1
+        a = a[1:]
+    if b and b[0][0] == s:
+        lo = 1 - b[0][1]
+        b = b[1:]
+    ra, rb = _reach(a), _reach(b)
+    return any(_meet(d - s * m, a, b, left) for m in range(max(lo, -((ra - d) // s)), min(hi, (rb + d) // s) + 1))
+
+
+def _overlap(x, y, xs, ys):
+    """(xs, ys: their spans)"""
+    return xs[0] < ys[1] and ys[0] < xs[1] and _meet(ys[0] - xs[0], _box(x), _box(y), [4096])
+
+
+def _repeats(x):
+    """does a tensor hold an element twice?"""
+    if x.numel() == 0 or x.is_contiguous():
+        return False
+    if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+        return True
+    dims = _box(x)
+    while len(dims) > 1:
+        (s, n), dims = dims[0], dims[1:]
+        if any(_meet(s * m, dims, dims, [4096]) for m in range(1, min(n - 1, _reach(dims) // s) + 1)):
+            return True
+    return False
+
+
+def _clear(outs, ins, name):
+    """a caller's own output tensors hold no element twice and lie over no input and no other output (parts of one packed tensor may lie
+    between each other)"""
+    outs = [(x, _span(x)) for x in outs if x is not None]
+    if not outs:
+        return
+    ins = [(x, _span(x)) for x in ins]
+    for i, (x, xs) in enumerate(outs):
+        _need(not _repeats(x), "%s: an output repeats elements" % name)
+        for y, ys in ins:
+            _need(not _overlap(x, y, xs, ys), "%s: an output overlaps an input" % name)
+        for y, ys in outs[:i]:
+            _need(not _overlap(x, y, xs, ys), "%s: two outputs overlap" % name)
 
 
 def _lens(x, name, batch, like):
@@ -178,13 +239,11 @@ def _outputs(q, Dv, out, lse, ins, name):
     if out is not None:
         _rows(out, "out", (B, Tq, Hq, Dv), q.dtype, q.device)
         _unrecorded(out, "out", name)
-        _apart([out], ins, name)
     if lse is not None:
         _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
         _unrecorded(lse, "lse", name)
         _need(lse.is_contiguous(), "lse: must be contiguous")
-        _apart([lse], ins, name)
-        _distinct((out, lse), name)
+    _clear((out, lse), ins, name)
     _on_gpu(q, name)
     if out is None:
         out = q.new_empty((B, Tq, Hq, Dv))
@@ -229,10 +288,9 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
         if x is not None:
             _rows(x, n, like.shape, q.dtype, q.device)
             _unrecorded(x, n, name)
-            _apart([x], ins, name)
-            _distinct((dq, dk, dv), name)
-    _on_gpu(q, name)
     given = dq, dk, dv
+    _clear(given, ins, name)
+    _on_gpu(q, name)
     dq = q.new_empty(q.shape) if dq is None else dq
     dk = q.new_empty(k.shape) if dk is None else dk
     dv = q.new_empty(v.shape) if dv is None else dv
@@ -270,7 +328,7 @@ def _weights(x, name, shape, like, call, written=False):
     """[batch, heads, tokens] float32; one that is written must not repeat elements"""
     if not (type(x) is torch.Tensor and x.shape == shape and x.dtype is torch.float32 and x.device == like.device and x.is_contiguous()):
         _rows(x, name, shape, torch.float32, like.device)
-        _need(not written or all(n == 1 or s > 0 for n, s in zip(x.shape, x.stride())), "%s: repeats elements" % name)
+        _need(not written or not _repeats(x), "%s: repeats elements" % name)
     _unrecorded(x, name, call)
 
 
@@ -291,7 +349,7 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
         weights_out = weights
     elif weights_out is not weights:
         _weights(weights_out, "weights_out", (B, Hkv, Tk), q, name, True)
-        _apart([weights_out], (q, k, v, weights), name)
+        _clear((weights_out,), (q, k, v, weights), name)
     given = out, lse, weights_out
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights, weights_out), name)
     args = _PACK_SCORED.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), *_sums(weights, weights_out),
@@ -321,24 +379,18 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
     _lens(lens, "lens", B, k)
     budget, sinks, recent = _count(budget, "budget"), _count(sinks, "sinks"), _count(recent, "recent")
     _need(sinks + recent <= budget, "sinks + recent must not exceed the budget")
-    ins = (k, v, weights)
     for x, n, dim in ((k_out, "k_out", Dk), (v_out, "v_out", Dv)):
         if x is not None:
             _need(isinstance(x, torch.Tensor) and x.dim() == 4 and x.shape[1] >= budget, "%s: needs %d tokens" % (n, budget))
             _rows(x, n, (B, x.shape[1], H, dim), k.dtype, k.device)
             _unrecorded(x, n, name)
-            _apart([x], ins, name)
     if weights_out is not None:
         _need(isinstance(weights_out, torch.Tensor) and weights_out.dim() == 3 and weights_out.shape[2] >= budget,
               "weights_out: needs %d tokens" % budget)
         _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k, name, True)
-        _apart([weights_out], ins, name)
-    if k_out is not None:
-        _distinct((k_out, v_out, weights_out), name)
-    elif v_out is not None:
-        _distinct((v_out, weights_out), name)
-    _on_gpu(k, name)
     given = k_out, v_out, weights_out
+    _clear([x if x is None else x.narrow(d, 0, budget) for x, d in zip(given, (1, 1, 2))], (k, v, weights), name)     # (what is written of them)
+    _on_gpu(k, name)
     k_out = k.new_empty((B, budget, H, Dk)) if k_out is None else k_out
     v_out = k.new_empty((B, budget, H, Dv)) if v_out is None else v_out
     weights_out = k.new_empty((B, H, budget), dtype=torch.float32) if weights_out is None else weights_out

@@ -244,3 +244,63 @@ def test_no_tensor_with_a_forward_mode_tangent(pkg):
         f, tensors, other, _ = calls(pkg)[0]
         with pytest.raises(pkg.SdpaError):                        # (others are not refused)
             f(**tensors, **other)
+
+
+def test_outputs_that_overlap_in_part_are_refused(pkg):
+    q, kv = torch.zeros(2, 3, 2, 8), torch.zeros(2, 3, 2, 8)
+    o, lse, w = torch.zeros(2, 3, 2, 8), torch.zeros(2, 2, 3), torch.zeros(2, 2, 3)
+    packed = torch.zeros(2, 3, 6, 8)
+    back = lambda **kw: pkg.attention_window_backward(o, q, kv, kv, o.clone(), lse, 4, **kw)
+    for dk, dv in ((packed[:, :, 0:2], packed[:, :, 1:3]), (packed[:, :, 2:4], packed[:, :, 0:6:2][:, :, 1:]), (packed[:, :, 4:], packed[:, :, 3:5])):
+        with pytest.raises(ValueError, match="two outputs overlap"):
+            back(dk=dk, dv=dv)
+    with pytest.raises(pkg.SdpaError):                    # (side by side, and every second head: they lie between each other)
+        back(dq=packed[:, :, 4:], dk=packed[:, :, 0:4:2], dv=packed[:, :, 1:4:2])
+    flat = torch.zeros(400)
+    with pytest.raises(ValueError, match="repeats elements"):
+        back(dk=flat.as_strided((2, 3, 2, 8), (48, 16, 4, 1)))
+    with pytest.raises(ValueError, match="repeats elements"):
+        pkg.attention_window(q, kv, kv, 4, out=flat.as_strided((2, 3, 2, 8), (40, 16, 8, 1)))
+    with pytest.raises(ValueError, match="repeats elements"):
+        pkg.attention_scored(q, kv, kv, flat.as_strided((2, 2, 3), (5, 2, 1)))
+    with pytest.raises(ValueError, match="two outputs overlap"):
+        pkg.evict_cache(kv, kv, w, None, 2, k_out=packed[:, :, :2], v_out=packed[:, 1:, 0:2])
+    with pytest.raises(pkg.SdpaError):                    # (what lies behind the budget is not written)
+        pkg.evict_cache(kv, kv, w, None, 1, k_out=packed[:, :, :2], v_out=packed[:, 1:, 0:2])
+    with pytest.raises(pkg.SdpaError):                    # (an output between the parts of an input)
+        pkg.attention_window(packed[:, :, 0:6:3], packed[:, :, 1:6:3], kv, 4, out=packed[:, :, 2:6:3])
+    with pytest.raises(ValueError, match="overlaps an input"):
+        pkg.attention_window(packed[:, :, 0:2], kv, kv, 4, out=packed[:, :, 1:3])
+
+
+def test_the_overlap_of_strided_tensors_is_what_their_elements_say(pkg):
+    """against the sets of their bytes"""
+    from importlib import import_module
+    heads = import_module(pkg.__name__ + ".heads")
+    rng = np.random.default_rng(7)
+    met = repeated = 0
+    for turn in range(3000):
+        room = torch.zeros(4000, dtype=torch.float32)
+        views, bytes_of = [], []
+        for _ in range(2):
+            dtype = (torch.float32, torch.bfloat16)[rng.integers(2)]
+            flat = room.view(dtype)
+            shape = tuple(int(n) for n in rng.integers(1, 5, 4))
+            if rng.random() < 0.5:                        # as a user's: a part of something larger, in some order
+                base = flat[int(rng.integers(0, 40)):][:6 ** 4].view(6, 6, 6, 6).permute(*rng.permutation(4).tolist())
+                x = base[tuple(slice(int(o), int(o) + n, int(rng.integers(1, 3))) for o, n in zip(rng.integers(0, 3, 4), shape))]
+            else:
+                x = flat.as_strided(shape, tuple(int(s) for s in rng.integers(0, 30, 4)), int(rng.integers(0, 60)))
+            views.append(x)
+            at = sum(np.arange(n).reshape([-1 if i == d else 1 for i in range(4)]) * s for d, (n, s) in enumerate(zip(x.shape, x.stride())))
+            at = np.asarray(x.storage_offset() + at).ravel()
+            bytes_of.append((at[:, None] * x.element_size() + np.arange(x.element_size())).ravel())
+        x, y = views
+        want = len(np.intersect1d(*bytes_of)) > 0
+        xs, ys = heads._span(x), heads._span(y)
+        assert heads._overlap(x, y, xs, ys) == want == heads._overlap(y, x, ys, xs)
+        for z, b in zip(views, bytes_of):
+            assert heads._repeats(z) == (len(np.unique(b)) < len(b))
+            repeated += heads._repeats(z)
+        met += want
+    assert 300 < met < 2700 and 300 < repeated < 5000
