@@ -310,3 +310,26 @@ def test_many_sinks_of_many_sequences(c, pkg):
     q, k, v = make((B, T, Hq, D), dtype, 1, 1.5), make((B, T, Hkv, D), dtype, 2), make((B, T, Hkv, D), dtype, 3)
     n = [T - (37 * b) % (T // 2) for b in range(B)]
     run_both(pkg, q, k, v, window, sinks, n, n, None, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 100, 128, 256])
+@pytest.mark.parametrize("B,Tq,Tk,G", [(8, 40, 1200, 2), (9, 130, 1000, 1)])
+def test_weights_of_chunks_of_many_sequences(B, Tq, Tk, G, D, dtype, pkg):
+    """so many key heads that a workgroup of the weights' kernel takes 128 keys; lengths that end inside its tiles, one of no tokens"""
+    H = 8
+    q, k, v = make((B, Tq, H * G, D), dtype, 1, 1.5), make((B, Tk, H, D), dtype, 2), make((B, Tk, H, D), dtype, 3)
+    ql, kl = [Tq - (11 * b) % Tq for b in range(B)], [Tk - (157 * b) % Tk for b in range(B)]
+    ql[2] = kl[3] = 0
+    w = torch.rand((B, H, Tk), generator=torch.Generator().manual_seed(4)).cuda()
+    out, lse, got = pkg.attention_scored(q, k, v, w, q_lens=lens(ql), kv_lens=lens(kl), weights_out=torch.empty_like(w))
+    want, wl, to, tl, heads = reference(q, k, v, ql, kl, 1 << 40, 0, D ** -0.5, dtype)
+    close(out, want, to, "out")
+    close(lse, wl, tl, "lse")
+    sums, tol = f64(w), np.zeros(w.shape)
+    for (b, h), (nq, nk, p, o, err) in heads.items():
+        sums[b, h // G, :nk] += p.sum(0)
+        tol[b, h // G, :nk] += (p * (err[:, None] + 2 * nq * ref.F32)).sum(0)
+    close(got, sums, tol + 2 * H * G * ref.F32 * np.abs(sums) + 1e-30, "weights")
+    again = pkg.attention_scored(q, k, v, w, q_lens=lens(ql), kv_lens=lens(kl))[2]
+    assert again is w and torch.equal(w, got)
