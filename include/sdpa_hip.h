@@ -508,7 +508,7 @@ struct sdpa_heads {
     int window, sinks;            /* key j is seen iff j <= p and (p - j < window or j < sinks)       */
     int prefix_tokens;
     int budget, recent;
-    float scale;                  /* scores are scale * q.k; any finite number                      */
+    float scale;                  /* scores are scale * q.k; at most 2^127 in size                   */
 };
 
 /* Sizes, with groups = batch * kv_heads; a call beyond them returns SDPA_EUNSUP, and so does the question of its scratch:

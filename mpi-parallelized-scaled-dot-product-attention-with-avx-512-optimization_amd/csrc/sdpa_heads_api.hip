@@ -12,6 +12,7 @@ using namespace sdpa;
 
 constexpr int kMaxTokens = 1 << 30;
 constexpr int kMaxSplits = 64;
+constexpr float kMaxScale = 0x1p127f;     // times log2(e) it is finite still: a larger one would make NaN of scores of 0
 constexpr double kMaxRows = (1 << 24) - 1, kMaxGroups = (1 << 24) - 1;
 
 bool bad_tensor(const sdpa_tensor &t, bool needed) {
@@ -40,7 +41,8 @@ int check_shape(const sdpa_heads *a) {
 int check_attention(const sdpa_heads *a) {
     SDPA_TRY(check_shape(a));
     if (a->q_heads < 1 || a->q_heads % a->kv_heads != 0) return SDPA_EINVAL;
-    if (a->window < 0 || a->sinks < 0 || a->prefix_tokens < 0 || !isfinite(a->scale)) return SDPA_EINVAL;
+    if (a->window < 0 || a->sinks < 0 || a->prefix_tokens < 0) return SDPA_EINVAL;
+    if (!(fabsf(a->scale) <= kMaxScale)) return SDPA_EINVAL;
     if (a->prefix_tokens > kMaxTokens) return SDPA_EUNSUP;
     // a launch has less than 2^32 threads: 256 for each 128 keys or rows of a head, and for each row of a join.  Of the forward forms only
     // few rows are split and joined, and those beside a prefix, whose rows are one tile list for the batch.

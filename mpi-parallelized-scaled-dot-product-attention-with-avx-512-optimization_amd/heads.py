@@ -31,6 +31,7 @@ HEAD_DIM_MAX = 256
 _OP_WINDOW, _OP_WINDOW_BACKWARD, _OP_PREFIX, _OP_SCORED, _OP_EVICT = range(5)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _INT_MAX = (1 << 31) - 1
+_SCALE_MAX = 2.0 ** 127                    # (times log2(e) it is a 32-bit number still)
 # struct sdpa_heads as bytes, a packer for each call: size, q k v out (16 words), prefix (8), gradients (16), lse and lengths (3),
 # weights (6), k_out v_out (8), lens_out kept (2), then dtype and the seven sizes, window, sinks, prefix_tokens, budget, recent, scale.
 # What a call has no use for is padding, which packs as zeros.
@@ -226,7 +227,11 @@ def _qkv(q, k, v, name):
 
 
 def _scale(scale, dk):
-    return 1.0 / math.sqrt(dk) if scale is None else float(scale)
+    if scale is None:
+        return 1.0 / math.sqrt(dk)
+    scale = float(scale)
+    _need(abs(scale) <= _SCALE_MAX, "scale: expected a number of at most %.4g in size, got %r" % (_SCALE_MAX, scale))
+    return scale
 
 
 def _on_gpu(x, name):
@@ -257,13 +262,14 @@ def attention_window(q, k, v, window, sinks=0, q_lens=None, kv_lens=None, scale=
     -> (out [B, Tq, Hq, Dv], lse [B, Hq, Tq]); window >= Tk is plain causal attention.  `out`, `lse`: tensors to write into."""
     name = "attention_window"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    scale = _scale(scale, Dk)
     window, sinks = _count(window, "window"), _count(sinks, "sinks")
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
     given = out, lse
     out, lse = _outputs(q, Dv, out, lse, (q, k, v), name)
     args = _PACK_WINDOW.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk,
-                             Hq, Hkv, Dk, Dv, window, sinks, _scale(scale, Dk))
+                             Hq, Hkv, Dk, Dv, window, sinks, scale)
     _call(_lib.load().sdpa_dev_attention_window, name, _OP_WINDOW, q, args)
     _written(*given)
     return out, lse
@@ -275,6 +281,7 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
     -> (dq, dk, dv), shaped and typed like q, k, v.  Deterministic.  `dq`, `dk`, `dv`: tensors to write into."""
     name = "attention_window_backward"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    scale = _scale(scale, Dk)
     window, sinks = _count(window, "window"), _count(sinks, "sinks")
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
@@ -295,7 +302,7 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
     dk = q.new_empty(k.shape) if dk is None else dk
     dv = q.new_empty(v.shape) if dv is None else dv
     args = _PACK_BACKWARD.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), *_at(dout), *_at(dq), *_at(dk), *_at(dv), lse.data_ptr(), _ptr(q_lens),
-                               _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, window, sinks, _scale(scale, Dk))
+                               _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, window, sinks, scale)
     _call(_lib.load().sdpa_dev_attention_window_backward, name, _OP_WINDOW_BACKWARD, q, args)
     _written(*given)
     return dq, dk, dv
@@ -307,6 +314,7 @@ def attention_prefix(q, k_prefix, v_prefix, k, v, q_lens=None, kv_lens=None, sca
     the batch.  -> (out, lse) over both parts."""
     name = "attention_prefix"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    scale = _scale(scale, Dk)
     for x, n in ((k_prefix, "k_prefix"), (v_prefix, "v_prefix")):
         _need(isinstance(x, torch.Tensor) and x.dim() == 3, "%s: expected [tokens, heads, dim]" % n)
     P = k_prefix.shape[0]
@@ -318,7 +326,7 @@ def attention_prefix(q, k_prefix, v_prefix, k, v, q_lens=None, kv_lens=None, sca
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, k_prefix, v_prefix), name)
     args = _PACK_PREFIX.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), k_prefix.data_ptr(), 0, *k_prefix.stride()[:2], v_prefix.data_ptr(), 0,
                              *v_prefix.stride()[:2], lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv,
-                             P, _scale(scale, Dk))
+                             P, scale)
     _call(_lib.load().sdpa_dev_attention_prefix, name, _OP_PREFIX, q, args)
     _written(*given)
     return out, lse
@@ -342,6 +350,7 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
     -> (out, lse, the increased weights).  evict_cache() goes by these sums."""
     name = "attention_scored"
     B, Tq, Tk, Hq, Hkv, Dk, Dv = _qkv(q, k, v, name)
+    scale = _scale(scale, Dk)
     _weights(weights, "weights", (B, Hkv, Tk), q, name, weights_out is None)
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
@@ -353,7 +362,7 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
     given = out, lse, weights_out
     out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights, weights_out), name)
     args = _PACK_SCORED.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), *_sums(weights, weights_out),
-                             _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, _scale(scale, Dk))
+                             _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, scale)
     _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q, args)
     _written(*given)
     return out, lse, weights_out

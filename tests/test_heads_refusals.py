@@ -304,3 +304,18 @@ def test_the_overlap_of_strided_tensors_is_what_their_elements_say(pkg):
             repeated += heads._repeats(z)
         met += want
     assert 300 < met < 2700 and 300 < repeated < 5000
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38, -3e38, 1e39])
+def test_scales_beyond_32_bits_are_refused(scale, pkg):
+    q, k, v = qkv()
+    for f in (lambda **kw: pkg.attention_window(q, k, v, 4, **kw), lambda **kw: pkg.attention_scored(q, k, v, torch.zeros(2, 2, 5), **kw),
+              lambda **kw: pkg.attention_prefix(q, k[0], v[0], k, v, **kw),
+              lambda **kw: pkg.attention_window_backward(torch.zeros(2, 3, 4, 6), q, k, v, torch.zeros(2, 3, 4, 6), torch.zeros(2, 4, 3), 4, **kw)):
+        with pytest.raises(ValueError, match="scale"):
+            f(scale=scale)
+        with pytest.raises(pkg.SdpaError):
+            f(scale=2.0 ** 127)
+    if abs(scale) < 1e39 or scale != scale or scale in (float("inf"), -float("inf")):
+        for op in range(4):
+            assert getattr(pkg.load(), ENTRIES[op])(pack(scale=scale), 4096, 1 << 20, None) == -1
