@@ -479,7 +479,7 @@ SDPA_API int  sdpa_dev_shard_partial_bf16(const void *Qb, int ldq, const void *K
  * A row that sees no key: out 0, lse -inf.  Rows i >= q_lens[b] likewise, and their gradients are 0; gradients of keys
  * j >= kv_lens[b] are 0.  A key that a row does not see has no influence on it, whatever its cache row holds (NaN included).
  * Outputs lie over no input and no other output, and hold no element twice (their parts may lie between each other); the one exception is
- * weights_out, which may be `weights`.
+ * attention_scored's weights_out, which may be `weights`.
  * Everything is deterministic: no result depends on the order of atomics.                                                        */
 #define SDPA_F32  0
 #define SDPA_BF16 1
@@ -499,7 +499,7 @@ struct sdpa_heads {
     float *lse;                   /* [B, q_heads, q_tokens] contiguous: log of the row's softmax sum (written forward, read backward) */
     const int *q_lens, *kv_lens;  /* [B] device int32, or null                                       */
     const float *weights;         /* [B, kv_heads, kv_tokens], tokens contiguous                     */
-    float *weights_out;           /* the same shape; may be `weights` itself                         */
+    float *weights_out;           /* attention_scored: the same shape, may be `weights` itself; eviction: [B, kv_heads, >= budget] */
     long weights_batch, weights_head, weights_out_batch, weights_out_head;   /* element strides      */
     struct sdpa_tensor k_out, v_out;         /* eviction: [B, >= budget tokens, kv_heads, dk / dv]    */
     int *lens_out, *kept;         /* eviction: [B] and [B, kv_heads, budget] contiguous              */

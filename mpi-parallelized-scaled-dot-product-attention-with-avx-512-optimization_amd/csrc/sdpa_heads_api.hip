@@ -218,6 +218,9 @@ int check_evict(const sdpa_heads *a) {
     if ((in && !a->weights) || (out && (!a->weights_out || !a->kept)) || !a->lens_out) return SDPA_EINVAL;
     if (a->weights_batch < 0 || a->weights_head < 0 || a->weights_out_batch < 0 || a->weights_out_head < 0) return SDPA_EINVAL;
     if (out && repeats_weights(a)) return SDPA_EINVAL;
+    // lengths and weights are read by workgroups that others' results of these would overtake
+    const uintptr_t n_in = (uintptr_t)a->kv_lens, n_out = (uintptr_t)a->lens_out, n_bytes = (uintptr_t)a->batch * sizeof(int);
+    if ((n_in && n_out < n_in + n_bytes && n_in < n_out + n_bytes) || (in && out && a->weights_out == a->weights)) return SDPA_EINVAL;
     if (repeats(a->k_out, a->batch, a->budget, a->kv_heads) || repeats(a->v_out, a->batch, a->budget, a->kv_heads))
         return SDPA_EINVAL;
     // (a workgroup moves 1024 pieces of at least one element, and one of 1024 threads selects for a head)

@@ -319,3 +319,12 @@ def test_scales_beyond_32_bits_are_refused(scale, pkg):
     if abs(scale) < 1e39 or scale != scale or scale in (float("inf"), -float("inf")):
         for op in range(4):
             assert getattr(pkg.load(), ENTRIES[op])(pack(scale=scale), 4096, 1 << 20, None) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(kv_lens=1 << 20, lens_out=1 << 20), dict(kv_lens=1 << 20, lens_out=(1 << 20) + 4), dict(kv_lens=(1 << 20) + 4, lens_out=1 << 20),
+                                dict(weights=1 << 20, weights_out=1 << 20)], ids=str)
+def test_an_eviction_over_its_own_lengths_or_weights_is_refused(kw, pkg):
+    lib = pkg.load()
+    far = dict(weights=1 << 16, weights_out=1 << 17)
+    assert lib.sdpa_dev_heads_workspace(4, pack(**far, kv_lens=1 << 20, lens_out=(1 << 20) + 8)) == 0
+    assert lib.sdpa_dev_heads_workspace(4, pack(**dict(far, **kw))) == -1 == lib.sdpa_dev_evict_cache(pack(**dict(far, **kw)), None, 0, None)
