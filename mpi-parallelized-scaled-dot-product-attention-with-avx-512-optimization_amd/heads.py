@@ -154,7 +154,7 @@ def _clear(outs, ins, name):
     outs = [(x, _span(x)) for x in outs if x is not None]
     if not outs:
         return
-    ins = [(x, _span(x)) for x in ins]
+    ins = [(x, _span(x)) for x in ins if x is not None]
     for i, (x, xs) in enumerate(outs):
         _need(not _repeats(x), "%s: an output repeats elements" % name)
         for y, ys in ins:
@@ -267,7 +267,7 @@ def attention_window(q, k, v, window, sinks=0, q_lens=None, kv_lens=None, scale=
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
     given = out, lse
-    out, lse = _outputs(q, Dv, out, lse, (q, k, v), name)
+    out, lse = _outputs(q, Dv, out, lse, (q, k, v, q_lens, kv_lens), name)
     args = _PACK_WINDOW.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk,
                              Hq, Hkv, Dk, Dv, window, sinks, scale)
     _call(_lib.load().sdpa_dev_attention_window, name, _OP_WINDOW, q, args)
@@ -290,7 +290,7 @@ def attention_window_backward(dout, q, k, v, out, lse, window, sinks=0, q_lens=N
     _rows(lse, "lse", (B, Hq, Tq), torch.float32, q.device)
     _need(lse.is_contiguous(), "lse: must be contiguous")
     _unrecorded(lse, "lse", name)
-    ins = (dout, q, k, v, out, lse)
+    ins = (dout, q, k, v, out, lse, q_lens, kv_lens)
     for x, n, like in ((dq, "dq", q), (dk, "dk", k), (dv, "dv", v)):
         if x is not None:
             _rows(x, n, like.shape, q.dtype, q.device)
@@ -323,7 +323,7 @@ def attention_prefix(q, k_prefix, v_prefix, k, v, q_lens=None, kv_lens=None, sca
     _lens(q_lens, "q_lens", B, q)
     _lens(kv_lens, "kv_lens", B, q)
     given = out, lse
-    out, lse = _outputs(q, Dv, out, lse, (q, k, v, k_prefix, v_prefix), name)
+    out, lse = _outputs(q, Dv, out, lse, (q, k, v, k_prefix, v_prefix, q_lens, kv_lens), name)
     args = _PACK_PREFIX.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), k_prefix.data_ptr(), 0, *k_prefix.stride()[:2], v_prefix.data_ptr(), 0,
                              *v_prefix.stride()[:2], lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv,
                              P, scale)
@@ -358,9 +358,9 @@ def attention_scored(q, k, v, weights, q_lens=None, kv_lens=None, scale=None, we
         weights_out = weights
     elif weights_out is not weights:
         _weights(weights_out, "weights_out", (B, Hkv, Tk), q, name, True)
-        _clear((weights_out,), (q, k, v, weights), name)
+        _clear((weights_out,), (q, k, v, weights, q_lens, kv_lens), name)
     given = out, lse, weights_out
-    out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights, weights_out), name)
+    out, lse = _outputs(q, Dv, out, lse, (q, k, v, weights, weights_out, q_lens, kv_lens), name)
     args = _PACK_SCORED.pack(_SIZE, *_at(q), *_at(k), *_at(v), *_at(out), lse.data_ptr(), _ptr(q_lens), _ptr(kv_lens), *_sums(weights, weights_out),
                              _DTYPES[q.dtype], B, Tq, Tk, Hq, Hkv, Dk, Dv, scale)
     _call(_lib.load().sdpa_dev_attention_scored, name, _OP_SCORED, q, args)
@@ -398,7 +398,7 @@ def evict_cache(k, v, weights, lens, budget, sinks=0, recent=0, k_out=None, v_ou
               "weights_out: needs %d tokens" % budget)
         _weights(weights_out, "weights_out", (B, H, weights_out.shape[2]), k, name, True)
     given = k_out, v_out, weights_out
-    _clear([x if x is None else x.narrow(d, 0, budget) for x, d in zip(given, (1, 1, 2))], (k, v, weights), name)     # (what is written of them)
+    _clear([x if x is None else x.narrow(d, 0, budget) for x, d in zip(given, (1, 1, 2))], (k, v, weights, lens), name)     # (what is written of them)
     _on_gpu(k, name)
     k_out = k.new_empty((B, budget, H, Dk)) if k_out is None else k_out
     v_out = k.new_empty((B, budget, H, Dv)) if v_out is None else v_out

@@ -328,3 +328,16 @@ def test_an_eviction_over_its_own_lengths_or_weights_is_refused(kw, pkg):
     far = dict(weights=1 << 16, weights_out=1 << 17)
     assert lib.sdpa_dev_heads_workspace(4, pack(**far, kv_lens=1 << 20, lens_out=(1 << 20) + 8)) == 0
     assert lib.sdpa_dev_heads_workspace(4, pack(**dict(far, **kw))) == -1 == lib.sdpa_dev_evict_cache(pack(**dict(far, **kw)), None, 0, None)
+
+
+def test_outputs_over_the_lengths_are_refused(pkg):
+    q, k, v = qkv(Dv=8)
+    room = torch.zeros(96)
+    n = room.view(torch.int32)[94:]
+    for f in (lambda: pkg.attention_window(q[:, :1], k, v, 4, kv_lens=n, out=room[32:].view(2, 1, 4, 8)),
+              lambda: pkg.attention_window(q, k, v, 4, q_lens=n, lse=room[72:].view(2, 4, 3)),
+              lambda: pkg.attention_prefix(q, k[0], v[0], k, v, kv_lens=n, lse=room[72:].view(2, 4, 3)),
+              lambda: pkg.attention_scored(q, k, v, torch.zeros(2, 2, 5), kv_lens=n, weights_out=room[76:].view(2, 2, 5)),
+              lambda: pkg.evict_cache(k, v, torch.zeros(2, 2, 5), n, 4, weights_out=room[80:].view(2, 2, 4))):
+        with pytest.raises(ValueError, match="overlaps an input"):
+            f()
