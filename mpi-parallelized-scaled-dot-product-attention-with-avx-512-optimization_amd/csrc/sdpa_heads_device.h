@@ -63,6 +63,7 @@ __device__ inline float to_f32(float x) { return x; }
 template <typename T> __device__ inline T from_f32(float x) { return (T)x; }   // (to nearest even)
 
 // ---- LDS tiles: rows of DP elements, 16-byte chunks XOR-swizzled by the row ----------------------------------------------
+// Chunk c of a row lies at row * kRowBytes + ((c ^ swz(row)) << 4): LaneMap reads by this, the stagers write by it.
 // Both readers are conflict-free: 16 consecutive rows at one chunk (the row-wise fragments) land in 16 different chunk
 // classes of the 64 banks, and 4 consecutive rows at 4 consecutive chunks (the transposing load) do too.
 template <typename T, int DP> struct Tile {
@@ -70,11 +71,6 @@ template <typename T, int DP> struct Tile {
     static constexpr int kRowBytes = DP * (int)sizeof(T);
     __device__ static int swz(int row) {
         return kChunks == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
-    }
-    __device__ static int chunk(int row, int c) { return row * kRowBytes + ((c ^ swz(row)) << 4); }
-    __device__ static int elem(int row, int col) {
-        const int b = col * (int)sizeof(T);
-        return chunk(row, b >> 4) + (b & 15);
     }
 };
 

@@ -691,9 +691,12 @@ template <typename T, int DP>
 void attend(const AttendArgs &a, int rows, int G, int groups, hipStream_t s) {
     constexpr int BN = DP * (int)sizeof(T) <= 256 ? 64 : 32;
     if (rows <= kFewRows) {
-        constexpr int threads = FewShape<T, DP, false>::kWaves * 64, wide = FewShape<T, DP, true>::kWaves * 64;
+        using Plain = FewShape<T, DP, false>;
+        using Wide = FewShape<T, DP, true>;              // (fp32 above 64 columns: 128 KiB are the plain form's waves)
+        constexpr int threads = Plain::kWaves * 64;
+        constexpr bool WIDE = Wide::kWaves != Plain::kWaves || Wide::kBufs != Plain::kBufs;
         const int grid = groups * a.splits;
-        if (a.wide && a.vec) attend_few_kernel<T, DP, true, true><<<grid, wide, 0, s>>>(a, rows, G);
+        if (WIDE && a.wide && a.vec) attend_few_kernel<T, DP, WIDE, true><<<grid, Wide::kWaves * 64, 0, s>>>(a, rows, G);
         else if (a.vec) attend_few_kernel<T, DP, false, true><<<grid, threads, 0, s>>>(a, rows, G);
         else attend_few_kernel<T, DP, false, false><<<grid, threads, 0, s>>>(a, rows, G);
     } else {
