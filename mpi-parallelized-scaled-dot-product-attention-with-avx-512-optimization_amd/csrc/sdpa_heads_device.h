@@ -234,8 +234,9 @@ template <typename T, int DP> __device__ inline bool block_not_finite(unsigned t
         const u32x4 w = lds_read<u32x4>(at + (unsigned)(k * 1024), block * 32 * Tile<T, DP>::kRowBytes);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (sizeof(T) == 2) bad = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[i]), bf16x2{0, 0}, bad, false);
-            else bad = __builtin_fmaf(__uint_as_float(w[i]), 0.f, bad);
+            const uint32_t x = w[i];                     // (a variable of its own: a bit cast of a vector's element takes element 0)
+            if constexpr (sizeof(T) == 2) bad = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), bf16x2{0, 0}, bad, false);
+            else bad = __builtin_fmaf(__uint_as_float(x), 0.f, bad);
         }
     }
     return __any(bad != bad);

@@ -85,3 +85,47 @@ def test_a_row_without_numbers_gives_its_weights_only_to_keys_it_sees(Tq, Tk, dt
     assert torch.equal(got[0], want[0]) and torch.equal(got[1, 0], want[1, 0])
     assert torch.equal(got[1, 1, first:], want[1, 1, first:]) and got[1, 1, :first].isnan().all()
     assert out[1, 1, 2].isnan().all() and lse[1, 2, 1].isnan() and out.isnan().sum() == out.shape[-1]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("Tq,Tk,D", [(3, 70, 64), (2, 3000, 128), (4, 60, 256), (64, 64, 64), (90, 200, 128), (40, 60, 256), (70, 90, 33)])
+def test_a_single_element_that_is_no_number(Tq, Tk, D, value, dtype, pkg):
+    """one element of one hidden row, at every place inside a 16-byte piece: neither outputs nor gradients of rows that do not see it change"""
+    q, k, v = make((1, Tq, 4, D), dtype, 1), make((1, Tk, 2, D), dtype, 2), make((1, Tk, 2, D), dtype, 3)
+    dout = make((1, Tq, 4, D), dtype, 4)
+    want = pkg.attention_window(q, k, v, Tk)
+    grads = pkg.attention_window_backward(dout, q, k, v, *want, Tk)
+    ws = pkg.attention_scored(q, k, v, torch.zeros((1, 2, Tk), device="cuda"))
+    key = Tk - max(1, Tq // 2)                            # seen from this row on
+    hit = key - (Tk - Tq)
+    for col in list(range(8)) + [D // 2 + 3, D - 2, D - 1]:
+        K, V = k.clone(), v.clone()
+        K[0, key, 0, col] = V[0, key, 1, col] = value
+        out, lse = pkg.attention_window(q, K, V, Tk)
+        assert torch.equal(out[:, :hit], want[0][:, :hit]) and torch.equal(lse[..., :hit], want[1][..., :hit]), col
+        so, sl, _ = pkg.attention_scored(q, K, V, torch.zeros((1, 2, Tk), device="cuda"))
+        assert torch.equal(so[:, :hit], ws[0][:, :hit]) and torch.equal(sl[..., :hit], ws[1][..., :hit]), col
+        # (values: dQ of the rows before; queries and output gradients: dK, dV of the keys behind them)
+        dq, _, _ = pkg.attention_window_backward(dout, q, K, V, *want, Tk)
+        assert torch.equal(dq[:, :hit], grads[0][:, :hit]), col
+        Q, DO = q.clone(), dout.clone()
+        Q[0, 0, 0, col] = DO[0, 0, 2, col] = value
+        _, dk, dv = pkg.attention_window_backward(DO, Q, k, v, *want, Tk)
+        first = Tk - Tq + 1                               # keys the first row does not see
+        assert torch.equal(dk[:, first:], grads[1][:, first:]) and torch.equal(dv[:, first:], grads[2][:, first:]), col
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_element_of_a_masked_tile_is_looked_at(dtype, pkg):
+    T = 40
+    for D in (64, 128):
+        q, k, v = make((1, T, 1, D), dtype, 1), make((1, T, 1, D), dtype, 2), make((1, T, 1, D), dtype, 3)
+        want, _ = pkg.attention_window(q, k, v, T)
+        for col in range(D):
+            V = v.clone()
+            for row in (1, 17, 38):
+                V[0, row:, 0, col] = float("inf")
+                out, _ = pkg.attention_window(q, k, V, T)
+                assert torch.equal(out[:, :row], want[:, :row]), (D, row, col)
+                V[0, row:, 0, col] = v[0, row:, 0, col]
