@@ -472,7 +472,8 @@ SDPA_API int  sdpa_dev_shard_partial_bf16(const void *Qb, int ldq, const void *K
  * G = Hq / Hkv share a key/value head, causal, over a cache.  Tensors are [batch, tokens, heads, dim] with any element strides
  * (a head-major tensor is the same with other strides); the dim elements of a row are contiguous.  Rows whose bases and strides are
  * multiples of 16 bytes take 16-byte accesses; all others are right as well, and slower.  fp32 tensors are multiplied on the f32
- * matrix instructions; bf16 tensors on the bf16 ones, accumulated in fp32, softmax weights rounded to bf16 as operands.
+ * matrix instructions; bf16 tensors on the bf16 ones, accumulated in fp32, softmax weights and their slopes as operands in two terms (2^-16
+ * of a value): bf16 results are off by their own rounding and little else.
  *
  * Query i of sequence b (i < q_lens[b]) is at position p = kv_lens[b] - q_lens[b] + i of its sequence: the queries are the
  * LAST tokens of the cache.  Lengths are int32 on the device, clamped there to [0, q_tokens] / [0, kv_tokens]; null = all of them.

@@ -154,6 +154,17 @@ __device__ inline void attend_blocks(State<DP> &st, const typename Ops<T>::Frag 
     }
 }
 
+// An infinity that a row sees, times what is left of its weight (0, or of the other sign), has become NaN: then the guarded way, too.
+template <typename T, int DP> __device__ inline bool lost_infinity(const State<DP> &st) {
+    if (sizeof(T) == 4) return false;
+    float bad = 0.f;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bad = __builtin_fmaf(st.o[d][i], 0.f, bad);
+    return __any(bad != bad);
+}
+
 // a finished row (or its partial triple): 4 consecutive values of row `x`, columns d .. d + 3
 template <typename T>
 __device__ inline void store4(const AttendArgs &a, const RowId &x, int hq, int d, f32x4 v) {
@@ -372,6 +383,7 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[n] = s2[n];
     }
+    odd = odd || lost_infinity<T, DP>(st);
     // Such a tile gave NaN to rows that do not see it: the workgroup does its rows once more, with a guarded product and
     // otherwise the same arithmetic.
     if (__syncthreads_or(odd)) {
@@ -508,6 +520,7 @@ __global__ __launch_bounds__((FewShape<T, DP, WIDE>::kWaves * 64)) void attend_f
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // (its reads are over before the tile is written again)
         if (NBUF == 2) buf ^= 1;
     }
+    odd = odd || lost_infinity<T, DP>(st);
     if (odd) {                                           // then the wave does its tiles once more, with guarded products
         st.clear();
 #pragma unroll 1
