@@ -206,8 +206,8 @@ __device__ inline float weighted_sum(const typename Ops<T>::Frag *q, const typen
 }
 
 // ---- dQ: 128 rows to a workgroup, 32 to a wave -------------------------------------------------------------------------
-// Bound by its matrix and vector instructions, which a SIMD issues one after the other.  Two sequences of 4096 tokens, 16 heads on 4 of 128
-// columns, window 1024, bf16: 122 us, 91 GFLOP in three products = 740 TFLOP/s.
+// Two sequences of 4096 tokens, 16 heads on 4 of 128 columns, window 1024, bf16: 149 us, 91 GFLOP in three products = 610 TFLOP/s.  Counters:
+// matrix instructions (dS is two operands) 0.39 of a SIMD's cycles, vector ones 0.28, a wave waits 0.29 of its time and has no turn for 0.32.
 template <typename T, int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kHeadsThreads, DP * (int)sizeof(T) <= 256 ? 2 : 1)
 void backward_rows_kernel(BackwardArgs a, int rows, int G, int tiles) {
@@ -453,9 +453,11 @@ template <typename T, int DP> struct RowStager {
 
 // ---- dK, dV: 64 keys to a workgroup -----------------------------------------------------------------------------------------
 // Waves 0 and 1 take 32 keys each on the even row blocks, waves 2 and 3 the same keys on the odd ones; the two sums are added in LDS
-// at the end.  Bound by LDS reads (every 32 x 32 block reads Q and dO twice, 32 KiB a wave at 128 columns) beside the matrix instructions, and
-// by the last round of workgroups; the shape above: 237 us, 121 GFLOP in four products = 510 TFLOP/s.  128 keys to a workgroup of eight waves,
-// V in LDS in place of registers, took 286 us; -lse / scale and -delta as the products' start, for fewer vector instructions, 245.
+// at the end.  The shape above: 290 us, 121 GFLOP in four products = 420 TFLOP/s.  Counters: matrix instructions (P and dS are two operands)
+// 0.30 of a SIMD's cycles, vector ones 0.20, LDS 0.14 of a CU's, 0.18 idle behind the last round of workgroups, and the one wave of
+// a SIMD (accumulators and operands fill the registers) waits 0.32 of its time: every block starts with reads and a chain of products that
+// nothing stands beside.  With P and dS in one term, 237 us then: 128 keys to a workgroup of eight waves, V in LDS in place of
+// registers, took 286; -lse / scale and -delta as the products' start, for fewer vector instructions, 245.
 // WHAT: 3 = both; heads of 256 do them one after the other (1 = dV, 2 = dK): two accumulators and two operands of 256 columns leave
 // no registers for the scores.
 template <typename T, int DP, int WHAT, bool VEC>

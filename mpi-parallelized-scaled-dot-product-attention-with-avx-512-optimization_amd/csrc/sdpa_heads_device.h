@@ -77,7 +77,7 @@ template <typename T, int DP> struct Tile {
 
 // 16 bytes of a row: elements [d0, d0 + kVec), zero from `dim` on.  `vec`: the row is 16-byte aligned and whole.  Others, in
 // bf16, are read in one load too (at their elements' alignment, which global loads allow), but for the row's last piece, whose elements are
-// read at once: two sequences of 1024 tokens, 8 heads of 100 columns, window 300, backward 207 us (element by element throughout: 331).  For
+// read at once: two sequences of 1024 tokens, 8 heads of 100 columns, window 300, backward 169 us (element by element throughout: 284).  For
 // fp32's four elements that gains 5 % and costs the widest heads registers.
 template <typename T> __device__ inline u32x4 load_chunk(const T *row, int d0, int dim, bool vec) {
     constexpr int N = Ops<T>::kVec;

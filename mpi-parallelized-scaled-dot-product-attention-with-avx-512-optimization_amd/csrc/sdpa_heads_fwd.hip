@@ -220,7 +220,8 @@ __device__ inline void load_query(typename Ops<T>::Frag *q, const AttendArgs &a,
 // The tile's products are a list of units -- for each 32-key block the K units (a step of the next tile's scores), then the V units
 // (a piece of O += V^T P) -- and a unit is written down as it is to be issued: the LDS read of the unit three ahead, this unit's
 // matrix instructions, and a few of the vector instructions that are due.  hipcc left alone puts all exponentials first and every
-// read right in front of its use (5000 cycles a tile and wave of 64 keys and 128 columns, against 1024 of its matrix instructions).
+// read right in front of its use (5000 cycles a tile and wave of 64 keys and 128 columns, against 1024 of its matrix instructions with
+// weights in one term, 1536 in two).
 template <typename T, int DP, int NB> struct Pipe {
     static constexpr int KU = DP / Ops<T>::kStep, VK = sizeof(T) == 2 ? 2 : 4, VU = DP / 32 * VK, PER = KU + VU, UNITS = NB * PER, AHEAD = 3;
     using Frag = typename Ops<T>::Frag;
@@ -282,8 +283,9 @@ template <typename T, int DP, int NB> struct Pipe {
 
 // ---- many rows: a workgroup's four waves share every key tile, each owns 32 rows -------------------------------------------------
 // The loop is a pipeline over the tiles.  LDS holds two K tiles and two V tiles; K runs one tile ahead of V, the DMA one ahead of both,
-// one barrier a tile.  Bound by its matrix and vector instructions, which a SIMD issues one after the other: a prompt of 8192 tokens,
-// 32 heads on 8 of 128 columns, window 1024, bf16: 202 us, 129 GFLOP = 640 TFLOP/s.
+// one barrier a tile.  A prompt of 8192 tokens, 32 heads on 8 of 128 columns, window 1024, bf16: 240 us, 129 GFLOP = 540 TFLOP/s.  Counters: a
+// SIMD's matrix instructions (the weights are two operands) take 0.39 of its cycles, its vector instructions 0.40, and a wave waits 0.31 of
+// its time: the two waves of a SIMD fill each other's pauses in part only.
 template <typename T, int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kHeadsThreads, DP <= 128 ? 2 : 1)
 void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
@@ -427,9 +429,10 @@ void attend_rows_kernel(AttendArgs a, int rows, int G, int tiles) {
 // Bound by the reading of the cache.  Every wave stages its own tiles of 32 keys (no barriers), the next one on its way by DMA while this
 // one is multiplied: 64 KiB in flight on a CU.  (fp32 tiles are bound by their matrix instructions and are not double-buffered.)
 // WIDE: up to eight waves, for calls so small that one workgroup does the keys of a head and no join is launched (one token of 16
-// heads on 4 of 64 columns, a window of 512: 17 us with the call around it, 21 in two launches).
-// Measured, 32 heads on 8 of 128 columns, bf16: 48 tokens over windows of 4096 158 us, 806 MB = 5.1 TB/s; 16 tokens over up to 8192 keys
-// with their scores kept 87 us, 377 MB = 4.3 TB/s.
+// heads on 4 of 64 columns, a window of 512: 17.5 us with the call around it, 10.8 of them the kernel's four workgroups, which take their
+// tiles one after the other; 21 us in two launches).
+// Measured, 32 heads on 8 of 128 columns, bf16: 48 tokens over windows of 4096 160 us, 806 MB = 5.0 TB/s; 16 tokens over up to 8192 keys
+// with their scores kept 89 us, 377 MB = 4.2 TB/s.
 template <typename T, int DP, bool WIDE> struct FewShape {
     static constexpr int kPair = few_pair_bytes(DP, sizeof(T));                              // a K and a V tile
     static constexpr int kWaves = WIDE ? few_wide_waves(DP, sizeof(T)) : kPair * 8 <= 131072 || (sizeof(T) == 4 && DP == 128) ? 4 : 2;
@@ -492,8 +495,9 @@ __global__ __launch_bounds__((FewShape<T, DP, WIDE>::kWaves * 64)) void attend_f
     map.init(lane);
     // (kept scores: the row of a lane that has one; the list of attention_scored is the cache itself)
     float *kept = a.scores && (lane & 31) < rows ? a.scores + (((long)b * a.Hkv + h) * rows + (lane & 31)) * a.score_ld : nullptr;
-    // One way through the products for masked tiles and others: a second one would have the accumulators in other registers, and heads of
-    // 256 columns in scratch memory (8 tokens against 2048 keys, 8 heads on 2 of 256 columns, the call: bf16 27 us against 37, fp32 91 against 101).
+    // One way through the products for masked tiles and others: a second one would have the accumulators in other registers (8 tokens against
+    // 2048 keys, 8 heads on 2 of 256 columns: bf16 21 us, fp32 53; with a second way 1.37 and 1.11 times that).  fp32 heads of 256
+    // columns still go through scratch memory, 58 accesses a tile.
     bool odd = false;                                    // a tile with masked pairs holds values that are no numbers
 #pragma unroll 1
     for (int it = it0 + wave, buf = 0; it < it1; it += WAVES) {
